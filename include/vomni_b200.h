@@ -142,6 +142,25 @@ VOMNI_API int vomni_cm_attention_local(const void* q, const void* k, const void*
                              int d, float softmax_scale, int flags, void* workspace, size_t workspace_bytes,
                              vomni_stream_t stream);
 
+/* ------------------------------------------------------------------ attention backward
+ * Gradients of softmax(softmax_scale q k^T) v from the forward's output o and log-sum-exp lse (VOMNI_CM_LSE: the
+ * training outputs of ring_attention_const_max_fwd.py:1062-1065); the probabilities are recomputed. q, grad_o, o:
+ * bf16 [b, s_q, hq, d], k, v [b, s_kv, hkv, d] with any strides: `strides` is a host array of 5 x 3 element strides, the
+ * (token, head, batch) strides of q, k, v, grad_o, o (positive multiples of 8 where that extent is over 1; d dense,
+ * d = 128). lse: fp32 [b, hq, 128, ceil(s_q/128)] dense. hq % hkv == 0: query head h reads key head h / (hq / hkv), whose
+ * gradients are summed over its query heads. dq, dk, dv: bf16, dense, token-major. q_lens / kv_lens (host arrays of b
+ * counts, or NULL): the tokens of each batch element; those behind are neither read nor counted, whatever they hold,
+ * and their gradients are 0. A row whose lse is -inf has no probabilities. Given the lse of a whole sequence
+ * and a part of its keys, the result is that part's share (the parts' dq add up). Bitwise reproducible (no
+ * atomics). workspace: vomni_attention_bwd_workspace_bytes (depends on the current device's size; 0 =
+ * unsupported shape), not shared by calls that may overlap. */
+VOMNI_API size_t vomni_attention_bwd_workspace_bytes(int b, int s_q, int s_kv, int hq, int hkv, int d);
+VOMNI_API int vomni_attention_bwd(const void* grad_o, const void* q, const void* k, const void* v, const void* o,
+                                  const float* lse, int b, int s_q, int s_kv, int hq, int hkv, int d,
+                                  const long long* strides, const int* q_lens, const int* kv_lens, float softmax_scale,
+                                  void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes,
+                                  vomni_stream_t stream);
+
 /* ------------------------------------------------------------------ fused adaLN + FP8 quant
  * Replaces adaln_quant_kernel (kernels/nkilib/experimental/norm/adaln_quant.py:117-810) as called
  * by the bridge adaln_modulate (diffusion/quantization/adaln_kernels.py:87-201):
@@ -157,6 +176,51 @@ VOMNI_API int vomni_adaln_modulate(const void* hidden, const void* residual, con
                                    const float* gate, long long rows, int h, long long rows_per_mod, float eps,
                                    int norm_type, int quant, int ocp, int packed, void* out, void* out_scale,
                                    void* residual_out, vomni_stream_t stream);
+
+/* ------------------------------------------------------------------ norms around a block
+ * The gated residual of adaln_modulate with a norm before it as well as after, and its gradients:
+ *   y = post(x) * post_weight;  r = residual + gate * y -> residual_out = bf16(r);
+ *   out = bf16(norm(r) * mul + add), from the unrounded r.
+ * x, residual, residual_out, out: bf16 [rows, h], h <= 8192, h % 8 == 0; vectors fp32, each optional: post_weight
+ * [h]; gate, mul, add [rows / rows_per_mod, h] where their VOMNI_PER_* bit is set in per_mod, else [h] (shared).
+ * post_norm / norm_type: 0 layer / 1 rms / 2 none, variance + eps. rows % rows_per_mod == 0. x NULL: r = residual
+ * (then gate, post_weight and residual_out must be NULL). residual_out may alias x or residual, and out may alias either.
+ *
+ * _bwd: from the gradients of residual_out and out (either may be NULL: zero), x and the stored residual_out it
+ * writes dx (x NULL: NULL), dresidual (bf16) and, where the pointer is not NULL, the fp32 column sums dgate,
+ * dpost_weight, dmul, dadd in their vectors' shapes. dx and dresidual may alias the gradients. Bitwise
+ * reproducible (no atomics). workspace: vomni_sandwich_norm_workspace_bytes, which depends on the current
+ * device's size; 0 = unsupported shape. rows / rows_per_mod <= 65535 in _bwd. */
+#define VOMNI_PER_GATE 1
+#define VOMNI_PER_MUL 2
+#define VOMNI_PER_ADD 4
+VOMNI_API int vomni_sandwich_norm(const void* x, const void* residual, const float* gate, const float* post_weight,
+                                  const float* mul, const float* add, long long rows, int h, long long rows_per_mod,
+                                  int per_mod, float eps, int post_norm, int norm_type, void* residual_out, void* out,
+                                  vomni_stream_t stream);
+VOMNI_API size_t vomni_sandwich_norm_workspace_bytes(long long rows, int h, long long rows_per_mod);
+VOMNI_API int vomni_sandwich_norm_bwd(const void* grad_residual_out, const void* grad_out, const void* x,
+                                      const void* residual_out, const float* gate, const float* post_weight,
+                                      const float* mul, long long rows, int h, long long rows_per_mod, int per_mod,
+                                      float eps, int post_norm, int norm_type, void* dx, void* dresidual, float* dgate,
+                                      float* dpost_weight, float* dmul, float* dadd, void* workspace,
+                                      size_t workspace_bytes, vomni_stream_t stream);
+
+/* ------------------------------------------------------------------ rotary positions with several axes
+ * WanRotaryPosEmbed + apply_rotary_emb_wan (diffusion/layers/rope.py:8-114) from the positions themselves, for q and
+ * (k_heads > 0) k in one launch: a head's d values are d / 2 pairs; axis a owns the next axes_dims[a] / 2 of them and
+ * turns its pair i by positions[.., a] * theta^(-2 i / axes_dims[a]). pairing 0: pair p = values (2p, 2p + 1); 1: (p,
+ * p + d / 2). inverse != 0: the negative angles (the gradient). q, k: [b, s, heads, d] with dense heads, the given row
+ * (token) and batch strides in elements (multiples of 16 bytes); outputs dense, not aliasing the inputs. positions:
+ * [s, n_axes], or [b, s, n_axes] when pos_per_batch, of pos_type 0 int32 / 1 int64 / 2 fp32. axes_dims: host array of
+ * n_axes (1..4) even counts summing to d; d % 16 == 0, d <= 256. dtype 0 bf16 / 1 fp16 / 2 fp32; fp32 arithmetic, angles
+ * reduced in fp64. */
+VOMNI_API int vomni_rotary_axes(const void* q, void* q_out, int q_heads, long long q_row_stride,
+                                long long q_batch_stride, const void* k, void* k_out, int k_heads,
+                                long long k_row_stride, long long k_batch_stride, int b, int s, int d,
+                                const void* positions, int pos_type, int pos_per_batch, int n_axes,
+                                const int* axes_dims, double theta, int pairing, int inverse, int dtype,
+                                vomni_stream_t stream);
 
 /* ------------------------------------------------------------------ FP8 QKV projection
  * Replaces qkv(quantization_type=ROW_MX) -> _qkv_cte_mx_impl (kernels/nkilib/core/qkv/qkv_cte.py:

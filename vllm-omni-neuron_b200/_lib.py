@@ -15,6 +15,7 @@ LIB_PATH = HERE / "libvomni_b200.so"
 HEADER = HERE.parent / "include" / "vomni_b200.h"
 
 c_int, c_float, c_size_t, c_void_p, c_char_p = ctypes.c_int, ctypes.c_float, ctypes.c_size_t, ctypes.c_void_p, ctypes.c_char_p
+c_longlong = ctypes.c_longlong
 P = c_void_p  # any device pointer / stream handle
 
 # name -> (restype, argtypes); mirrors include/vomni_b200.h
@@ -81,6 +82,26 @@ SIGNATURES = {
         c_int,
         [P, P, P, P, P, P, c_int, c_int, c_int, c_int, ctypes.c_longlong, ctypes.c_longlong, c_float, c_int, P],
     ),
+    "vomni_attention_bwd_workspace_bytes": (c_size_t, [c_int] * 6),
+    "vomni_attention_bwd": (
+        c_int,
+        [P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, ctypes.POINTER(c_longlong), ctypes.POINTER(c_int),
+         ctypes.POINTER(c_int), c_float, P, P, P, P, c_size_t, P],
+    ),
+    "vomni_rotary_axes": (
+        c_int,
+        [P, P, c_int, c_longlong, c_longlong, P, P, c_int, c_longlong, c_longlong, c_int, c_int, c_int, P, c_int, c_int,
+         c_int, ctypes.POINTER(c_int), ctypes.c_double, c_int, c_int, c_int, P],
+    ),
+    "vomni_sandwich_norm": (
+        c_int,
+        [P, P, P, P, P, P, c_longlong, c_int, c_longlong, c_int, c_float, c_int, c_int, P, P, P],
+    ),
+    "vomni_sandwich_norm_workspace_bytes": (c_size_t, [c_longlong, c_int, c_longlong]),
+    "vomni_sandwich_norm_bwd": (
+        c_int,
+        [P, P, P, P, P, P, P, c_longlong, c_int, c_longlong, c_int, c_float, c_int, c_int, P, P, P, P, P, P, P, c_size_t, P],
+    ),
     "vomni_cm_attention_local_noalloc": (
         c_int,
         [P, P, P, P, P, c_int, c_int, c_int, c_int, c_float, c_int, P],
@@ -133,6 +154,17 @@ def check(code: int, what: str) -> None:
 
 def call(name: str, *args) -> None:
     check(getattr(load(), name)(*args), name)
+
+
+def one_device(*tensors):
+    """The CUDA device that all the given tensors (None entries aside) live on."""
+    devs = {t.device for t in tensors if t is not None}
+    for d in devs:
+        if d.type != "cuda":
+            raise RuntimeError(f"expected CUDA tensors (the B200 kernels have no CPU path), got one on {d}")
+    if len(devs) != 1:
+        raise ValueError(f"tensors are on different devices: {sorted(map(str, devs))}")
+    return devs.pop()
 
 
 def device_status(clear: bool = True) -> int:

@@ -20,10 +20,14 @@ strided copies straight out of the token-major host layout) overlaps the attenti
 the result of group i returns to pinned host memory while group i+1 computes. Heads are
 independent, so the result is identical to the device-resident call; the output is a pinned CPU
 tensor, complete on return.
+
+Training: :func:`wan_attention` is the differentiable form, made of :func:`attention_fwd` (output and log-sum-exp; keys of
+another sequence, shared key heads and uneven batches included) and :func:`attention_bwd` (the gradients).
 """
 
 from __future__ import annotations
 
+import ctypes
 import math
 
 import torch
@@ -264,3 +268,160 @@ def wan_cp_self_attention(query, key, value, scale, cp_size, cp_group, cp_replic
         query, key, value, replica_groups=cp_replica_groups, num_workers=int(cp_size), softmax_scale=scale,
         group=group, out_layout="bhds",
     )
+
+
+# ---------------------------------------------------------------- training
+
+
+def _lens(name: str, lens, b: int, s: int):
+    """Host token counts per batch element, or None."""
+    if lens is None:
+        return None
+    if isinstance(lens, torch.Tensor):
+        raise TypeError(f"{name} must be a sequence of {b} ints on the host (they size the launch), got a tensor")
+    lens = [int(n) for n in lens]
+    if len(lens) != b or any(not 0 <= n <= s for n in lens):
+        raise ValueError(f"{name} must be {b} counts between 0 and {s}, got {lens}")
+    return lens
+
+
+def _check_training(q, k, v, q_lens, kv_lens):
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if t.dim() != 4:
+            raise ValueError(f"{name} must be token-major [b, s, heads, {_HEAD_DIM}], got {tuple(t.shape)}")
+        if t.dtype != torch.bfloat16:
+            raise TypeError(f"{name} must be bfloat16, got {t.dtype}")
+    b, sq, hq, d = q.shape
+    skv, hkv = k.shape[1:3]
+    if d != _HEAD_DIM:
+        raise ValueError(f"head_dim must be {_HEAD_DIM}, got {d}")
+    if k.shape != v.shape or k.shape[0] != b or k.shape[3] != d:
+        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must be [{b}, s_kv, heads, {d}]")
+    if hkv == 0 or hq % hkv:
+        raise ValueError(f"query heads ({hq}) must be a multiple of key heads ({hkv})")
+    return b, sq, skv, hq, hkv, _lens("q_lens", q_lens, b, sq), _lens("kv_lens", kv_lens, b, skv)
+
+
+def _cross_fwd(q, k, v, scale):
+    """(o [b, h, s_q, d], lse) of whole sequences with equal head counts."""
+    b, sq, h, d = q.shape
+    skv = k.shape[1]
+    q, qs = token_major(q)
+    k, ks = token_major(k)
+    v, vs = token_major(v)
+    if ks != vs:
+        k, v = k.contiguous(), v.contiguous()
+        ks = h * d
+    lib = _lib.load()
+    o = torch.empty((b, h, sq, d), dtype=torch.bfloat16, device=q.device)
+    lse = torch.full((b, h, 128, -(-sq // 128)), -math.inf, dtype=torch.float32, device=q.device)
+    ws_bytes = lib.vomni_cm_workspace_bytes(b, sq, h, d)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+    rc = lib.vomni_cm_attention_cross(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), b, sq, skv, h, d,
+                                      qs, ks, scale, _lib.CM_LSE, ws.data_ptr(), ws_bytes, _stream_ptr(q.device))
+    _lib.check(rc, "vomni_cm_attention_cross")
+    return o, lse
+
+
+def attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, softmax_scale: float | None = None, *, q_lens=None,
+                  kv_lens=None):
+    """``(o [b, hq, s_q, 128] bf16, lse [b, hq, 128, ceil(s_q / 128)] fp32)`` of ``softmax(softmax_scale q k^T) v``.
+
+    ``q [b, s_q, hq, 128]``, ``k, v [b, s_kv, hkv, 128]`` token-major bf16, ``hq % hkv == 0`` (query head ``h`` reads key head
+    ``h // (hq // hkv)``). ``lse[.., r, g]`` belongs to token ``128 g + r``, as in :func:`ring_attention_const_max_fwd`.
+    ``q_lens`` / ``kv_lens``: tokens of each batch element (host ints); rows behind them are not read, and their output
+    is 0 with an lse of -inf, as is that of rows without keys. ``softmax_scale`` defaults to ``1 / sqrt(128)``.
+    """
+    b, sq, skv, hq, hkv, q_lens, kv_lens = _check_training(q, k, v, q_lens, kv_lens)
+    dev = _lib.one_device(q, k, v)
+    scale = 1.0 / math.sqrt(_HEAD_DIM) if softmax_scale is None else float(softmax_scale)
+    with torch.cuda.device(dev):
+        if hkv != hq:
+            k, v = (t.repeat_interleave(hq // hkv, dim=2) for t in (k, v))
+        if q_lens is None and kv_lens is None and b * sq * hq and skv:
+            return _cross_fwd(q, k, v, scale)
+        o = torch.zeros((b, hq, sq, _HEAD_DIM), dtype=torch.bfloat16, device=dev)
+        lse = torch.full((b, hq, 128, -(-sq // 128)), -math.inf, dtype=torch.float32, device=dev)
+        for i in range(b):
+            m, n = q_lens[i] if q_lens else sq, kv_lens[i] if kv_lens else skv
+            if m and n and hq:
+                oi, li = _cross_fwd(q[i : i + 1, :m], k[i : i + 1, :n], v[i : i + 1, :n], scale)
+                o[i, :, :m] = oi[0]
+                lse[i, :, :, : li.shape[-1]] = li[0]
+        return o, lse
+
+
+def _any_strides(t: torch.Tensor) -> torch.Tensor:
+    """``t`` as it is where TMA can address its strides (d dense, the others positive multiples of 8), else a copy."""
+    ok = t.stride(3) == 1 and t.data_ptr() % 16 == 0
+    ok = ok and all(n == 1 or (st > 0 and st % 8 == 0) for n, st in zip(t.shape[:3], t.stride()[:3]))
+    if ok:
+        return t
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def attention_bwd(grad_o: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, lse: torch.Tensor,
+                  softmax_scale: float | None = None, *, q_lens=None, kv_lens=None):
+    """``(dq, dk, dv)``, dense bf16 in the shapes of ``q, k, v``, of the attention whose output and log-sum-exp are ``o``, ``lse``.
+
+    ``o`` / ``grad_o [b, hq, s_q, 128]`` bf16 (any strides) and ``lse`` as :func:`attention_fwd` or
+    ``ring_attention_const_max_fwd(training=True)`` return them; the other arguments as in :func:`attention_fwd`. The
+    probabilities are recomputed as ``exp(softmax_scale q k^T - lse)``, so with the ``lse`` and ``o`` of a whole sequence
+    and a part of its keys the result is that part's share of the gradients (for a context-parallel ring: the parts'
+    ``dq`` add up). Rows behind ``q_lens`` / ``kv_lens`` are not read and get zero gradients; a row whose lse is -inf
+    contributes nothing. The same call gives the same bits (no atomics).
+    """
+    b, sq, skv, hq, hkv, q_lens, kv_lens = _check_training(q, k, v, q_lens, kv_lens)
+    for name, t in (("grad_o", grad_o), ("o", o)):
+        if t.dtype != torch.bfloat16:
+            raise TypeError(f"{name} must be bfloat16, got {t.dtype}")
+        if tuple(t.shape) != (b, hq, sq, _HEAD_DIM):
+            raise ValueError(f"{name} must be [{b}, {hq}, {sq}, {_HEAD_DIM}], got {tuple(t.shape)}")
+    if not lse.is_floating_point() or tuple(lse.shape) != (b, hq, 128, -(-sq // 128)):
+        raise ValueError(f"lse must be [{b}, {hq}, 128, {-(-sq // 128)}], got {lse.dtype} {tuple(lse.shape)}")
+    dev = _lib.one_device(grad_o, q, k, v, o, lse)
+    scale = 1.0 / math.sqrt(_HEAD_DIM) if softmax_scale is None else float(softmax_scale)
+    empty = not (b and sq and skv and hq)
+    make = torch.zeros if empty else torch.empty
+    dq, dk, dv = (make(t.shape, dtype=torch.bfloat16, device=dev) for t in (q, k, v))
+    if empty:
+        return dq, dk, dv
+    with torch.cuda.device(dev):
+        lib = _lib.load()
+        src = [_any_strides(t) for t in (q, k, v, grad_o.transpose(1, 2), o.transpose(1, 2))]
+        strides = (ctypes.c_longlong * 15)(*(t.stride(i) for t in src for i in (1, 2, 0)))
+        lse = lse.to(torch.float32).contiguous()
+        ints = lambda lens: (ctypes.c_int * b)(*lens) if lens is not None else None
+        ws_bytes = lib.vomni_attention_bwd_workspace_bytes(b, sq, skv, hq, hkv, _HEAD_DIM)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        rc = lib.vomni_attention_bwd(
+            src[3].data_ptr(), src[0].data_ptr(), src[1].data_ptr(), src[2].data_ptr(), src[4].data_ptr(), lse.data_ptr(), b, sq,
+            skv, hq, hkv, _HEAD_DIM, strides, ints(q_lens), ints(kv_lens), scale, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+            ws.data_ptr(), ws_bytes, _stream_ptr(dev))
+        _lib.check(rc, "vomni_attention_bwd")
+    return dq, dk, dv
+
+
+class _WanAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, scale, q_lens, kv_lens):
+        o, lse = attention_fwd(q, k, v, scale, q_lens=q_lens, kv_lens=kv_lens)
+        ctx.save_for_backward(q, k, v, o, lse)
+        ctx.rest = (scale, q_lens, kv_lens)
+        return o
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_o):
+        scale, q_lens, kv_lens = ctx.rest
+        grads = attention_bwd(grad_o, *ctx.saved_tensors, scale, q_lens=q_lens, kv_lens=kv_lens)
+        return tuple(g if need else None for g, need in zip(grads, ctx.needs_input_grad)) + (None, None, None)
+
+
+def wan_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, softmax_scale: float | None = None, *, q_lens=None,
+                  kv_lens=None) -> torch.Tensor:
+    """Differentiable attention ``[b, hq, s_q, 128]`` of one device's ``q [b, s_q, hq, 128]``, ``k, v [b, s_kv, hkv, 128]``;
+    the arguments are those of :func:`attention_fwd`, the gradients those of :func:`attention_bwd`."""
+    q_lens, kv_lens = (tuple(n) if isinstance(n, (list, tuple)) else n for n in (q_lens, kv_lens))
+    return _WanAttention.apply(q, k, v, softmax_scale, q_lens, kv_lens)

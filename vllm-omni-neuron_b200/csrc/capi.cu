@@ -137,6 +137,26 @@ int make_tmap_3d_bf16(CUtensorMap* map, const void* base, uint64_t dim0, uint64_
   return r == CUDA_SUCCESS ? VOMNI_OK : VOMNI_ECUDA;
 }
 
+int make_tmap_4d_bf16(CUtensorMap* map, const void* base, const uint64_t (&dims)[4], const long long (&strides)[3],
+                      uint32_t box0, uint32_t box1) {
+  int rc = get_encoder();
+  if (rc) return rc;
+  if (reinterpret_cast<uintptr_t>(base) & 15) return VOMNI_EALIGN;
+  cuuint64_t d[4] = {dims[0], dims[1], dims[2], dims[3]};
+  cuuint64_t st[3];
+  for (int i = 0; i < 3; ++i) {
+    const long long e = dims[i + 1] == 1 ? static_cast<long long>((dims[0] + 7) / 8 * 8) : strides[i];
+    if (e <= 0 || e % 8) return VOMNI_EALIGN;
+    st[i] = static_cast<cuuint64_t>(e) * 2;
+  }
+  cuuint32_t box[4] = {box0, box1, 1, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), d, st, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? VOMNI_OK : VOMNI_ECUDA;
+}
+
 int make_tmap_3d_bf16_plain(CUtensorMap* map, const void* base, uint64_t dim0, uint64_t dim1, uint64_t dim2,
                             uint32_t box0, uint32_t box1) {
   int rc = get_encoder();

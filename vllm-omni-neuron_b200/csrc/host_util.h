@@ -35,6 +35,10 @@ int* device_status_ptr();
 // elements apart (0 = dense), box {box0, box1, 1}, 128-byte swizzle, out-of-bounds reads as zero.
 int make_tmap_3d_bf16(CUtensorMap* map, const void* base, uint64_t dim0, uint64_t dim1, uint64_t dim2, uint32_t box0,
                       uint32_t box1, uint64_t row_pitch_elems = 0);
+// Rank-4 bf16 tensor map over [dim3][dim2][dim1][dim0] with dense dim0 and the given strides (elements, multiples
+// of 8; the stride of an extent of 1 is ignored), box {box0, box1, 1, 1}, 128-byte swizzle, OOB reads as zero.
+int make_tmap_4d_bf16(CUtensorMap* map, const void* base, const uint64_t (&dims)[4], const long long (&strides)[3],
+                      uint32_t box0, uint32_t box1);
 // Rank-3 bf16 tensor map over a dense [dim2][dim1][dim0] tensor without swizzle (boxes land in
 // shared memory as plain row-major [box1][box0]), OOB reads as zero.
 int make_tmap_3d_bf16_plain(CUtensorMap* map, const void* base, uint64_t dim0, uint64_t dim1, uint64_t dim2,

@@ -1,0 +1,242 @@
+// Rotary positions with several axes (frame, row, column of a video; row, column of an image), and
+// their gradient, for query and key heads in one launch.
+//
+// A head of d values is d / 2 pairs, split among the axes: axis a owns n_a / 2 consecutive pairs
+// (sum n_a = d), its pair i turning by
+//     angle = position[a] * theta^(-2 i / n_a),  (x1, x2) -> (x1 cos - x2 sin, x2 cos + x1 sin),
+// with (x1, x2) = (x[2p], x[2p+1]) (interleaved) or (x[p], x[p + d/2]) (rotate-half). The gradient is
+// the rotation by the negative angle. With axes (44, 42, 42) and interleaved pairs this is
+// WanRotaryPosEmbed + apply_rotary_emb_wan (vllm_omni_neuron/diffusion/layers/rope.py:8-114) without
+// their per-token tables.
+//
+// Angles: the frequency is kept as turns per position (theta^(-2i/n) / 2 pi) in fp64, the product
+// with the position is reduced to [-1/2, 1/2] turns in fp64 and only then rounded to fp32, so a
+// far position costs no accuracy (2^-24 relative of the reduced angle; an fp32 product at position
+// 10^6 would be off by 0.06 rad). A pair group's cosines and sines are formed once per token by the
+// threads that use them and stay in registers over all its heads.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cmath>
+
+#include "common.cuh"
+#include "host_util.h"
+
+namespace vomni {
+namespace rotary {
+
+constexpr int kMaxDim = 256;
+constexpr int kMaxAxes = 4;
+constexpr int kGroup = 8;  // pairs per thread and head: 16 values, two 16-byte loads in 16-bit types
+constexpr int kThreads = 256;
+
+struct Tensor {
+  const void* x;
+  void* y;  // dense [b, s, heads, d]
+  int heads;
+  long long row_stride, batch_stride;  // of x, in elements
+};
+
+struct Params {
+  Tensor t[2];
+  long long tokens;  // b * s
+  int s, d, n_axes;
+  int head_blocks;  // CTAs that share a token's heads
+  const void* pos;  // [s, n_axes] or [b, s, n_axes]
+  int pos_type;     // 0 int32, 1 int64, 2 fp32
+  int pos_batch;    // positions differ per batch element
+  int half;         // rotate-half pairs
+  float sign;       // -1: the inverse rotation (the gradient)
+  unsigned char axis[kMaxDim / 2];
+  double turns[kMaxDim / 2];  // turns per unit of position
+};
+
+template <typename T>
+struct Io;
+template <>
+struct Io<__nv_bfloat16> {
+  static VOMNI_DEV void load8(const __nv_bfloat16* p, float (&v)[8]) {
+    const uint4 w = __ldcs(reinterpret_cast<const uint4*>(p));
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = __uint_as_float(u[i] << 16);
+      v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+    }
+  }
+  static VOMNI_DEV void store8(__nv_bfloat16* p, const float (&v)[8]) {
+    __stcs(reinterpret_cast<uint4*>(p), make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]),
+                                                   pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])));
+  }
+};
+template <>
+struct Io<__half> {
+  static VOMNI_DEV void load8(const __half* p, float (&v)[8]) {
+    const uint4 w = __ldcs(reinterpret_cast<const uint4*>(p));
+    const __half2* h = reinterpret_cast<const __half2*>(&w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __half22float2(h[i]);
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
+    }
+  }
+  static VOMNI_DEV void store8(__half* p, const float (&v)[8]) {
+    uint4 w;
+    __half2* h = reinterpret_cast<__half2*>(&w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+    __stcs(reinterpret_cast<uint4*>(p), w);
+  }
+};
+template <>
+struct Io<float> {
+  static VOMNI_DEV void load8(const float* p, float (&v)[8]) {
+    const float4 a = __ldcs(reinterpret_cast<const float4*>(p)), b = __ldcs(reinterpret_cast<const float4*>(p) + 1);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  }
+  static VOMNI_DEV void store8(float* p, const float (&v)[8]) {
+    __stcs(reinterpret_cast<float4*>(p), make_float4(v[0], v[1], v[2], v[3]));
+    __stcs(reinterpret_cast<float4*>(p) + 1, make_float4(v[4], v[5], v[6], v[7]));
+  }
+};
+
+// One CTA per token (and share of its heads). Thread t keeps pair group t % (d / 16) and walks heads
+// t / (d / 16), + kThreads / (d / 16), ...; d / 16 need not divide kThreads: the threads past the
+// last whole head idle.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ Params p) {
+  const int groups = p.d / (2 * kGroup);
+  const int lanes = kThreads / groups;  // heads in flight
+  const int g = threadIdx.x % groups, lane = threadIdx.x / groups;
+  const long long token = blockIdx.x / p.head_blocks;
+  const int share = blockIdx.x % p.head_blocks;
+  if (lane >= lanes) return;
+  const long long bi = token / p.s, si = token % p.s;
+
+  float c[kGroup], sn[kGroup];
+  const long long prow = (p.pos_batch ? token : si) * p.n_axes;
+#pragma unroll
+  for (int i = 0; i < kGroup; ++i) {
+    const int pair = g * kGroup + i;
+    const long long at = prow + p.axis[pair];
+    const double pos = p.pos_type == 0   ? static_cast<double>(static_cast<const int*>(p.pos)[at])
+                       : p.pos_type == 1 ? static_cast<double>(static_cast<const long long*>(p.pos)[at])
+                                         : static_cast<double>(static_cast<const float*>(p.pos)[at]);
+    double t = pos * p.turns[pair];
+    t -= rint(t);
+    sincospif(2.f * static_cast<float>(t), &sn[i], &c[i]);
+    sn[i] *= p.sign;
+  }
+
+  // values of the group: interleaved 16 consecutive ones, rotate-half 8 of each half of the head
+  const int o1 = p.half ? g * kGroup : g * 2 * kGroup;
+  const int o2 = p.half ? o1 + p.d / 2 : o1 + kGroup;
+  const int all = p.t[0].heads + p.t[1].heads;
+  for (int h = share * lanes + lane; h < all; h += p.head_blocks * lanes) {
+    const int which = h >= p.t[0].heads;
+    const Tensor& t = p.t[which];
+    const int hh = which ? h - p.t[0].heads : h;
+    const T* x = static_cast<const T*>(t.x) + bi * t.batch_stride + si * t.row_stride + static_cast<long long>(hh) * p.d;
+    T* y = static_cast<T*>(t.y) + (token * t.heads + hh) * p.d;
+    float a[8], b[8];
+    Io<T>::load8(x + o1, a);
+    Io<T>::load8(x + o2, b);
+    if (p.half) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float x1 = a[i], x2 = b[i];
+        a[i] = x1 * c[i] - x2 * sn[i];
+        b[i] = x2 * c[i] + x1 * sn[i];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x1 = a[2 * i], x2 = a[2 * i + 1], z1 = b[2 * i], z2 = b[2 * i + 1];
+        a[2 * i] = x1 * c[i] - x2 * sn[i];
+        a[2 * i + 1] = x2 * c[i] + x1 * sn[i];
+        b[2 * i] = z1 * c[4 + i] - z2 * sn[4 + i];
+        b[2 * i + 1] = z2 * c[4 + i] + z1 * sn[4 + i];
+      }
+    }
+    Io<T>::store8(y + o1, a);
+    Io<T>::store8(y + o2, b);
+  }
+}
+
+int check_tensor(const void* x, const void* y, int heads, long long row_stride, long long batch_stride, int b, int s,
+                 int d, int esize) {
+  if (heads < 0 || heads > (1 << 20)) return VOMNI_EBADSHAPE;
+  if (heads == 0) return VOMNI_OK;
+  if (!x || !y) return VOMNI_EINVAL;
+  if (s > 1 && row_stride < static_cast<long long>(heads) * d) return VOMNI_EBADSHAPE;
+  if (b > 1 && batch_stride < 0) return VOMNI_EBADSHAPE;
+  if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y)) & 15) return VOMNI_EALIGN;
+  if ((row_stride * esize) % 16 || (batch_stride * esize) % 16) return VOMNI_EALIGN;
+  return VOMNI_OK;
+}
+
+}  // namespace rotary
+}  // namespace vomni
+
+using namespace vomni;
+
+extern "C" int vomni_rotary_axes(const void* q, void* q_out, int q_heads, long long q_row_stride,
+                                 long long q_batch_stride, const void* k, void* k_out, int k_heads,
+                                 long long k_row_stride, long long k_batch_stride, int b, int s, int d,
+                                 const void* positions, int pos_type, int pos_per_batch, int n_axes,
+                                 const int* axes_dims, double theta, int pairing, int inverse, int dtype,
+                                 vomni_stream_t stream) {
+  if (!positions || !axes_dims) return VOMNI_EINVAL;
+  if (pos_type < 0 || pos_type > 2 || pairing < 0 || pairing > 1 || dtype < 0 || dtype > 2) return VOMNI_EINVAL;
+  if (!(theta > 0.0) || !std::isfinite(theta)) return VOMNI_EINVAL;
+  if (b <= 0 || s <= 0 || d <= 0 || d > rotary::kMaxDim || d % 16) return VOMNI_EBADSHAPE;
+  if (n_axes < 1 || n_axes > rotary::kMaxAxes) return VOMNI_EBADSHAPE;
+  const int esize = dtype == 2 ? 4 : 2;
+  int rc = rotary::check_tensor(q, q_out, q_heads, q_row_stride, q_batch_stride, b, s, d, esize);
+  if (rc) return rc;
+  rc = rotary::check_tensor(k, k_out, k_heads, k_row_stride, k_batch_stride, b, s, d, esize);
+  if (rc) return rc;
+  if (q_heads + k_heads == 0) return VOMNI_EBADSHAPE;
+  if (reinterpret_cast<uintptr_t>(positions) & (pos_type == 1 ? 7 : 3)) return VOMNI_EALIGN;
+  rotary::Params p = {};
+  int pair = 0;
+  for (int a = 0; a < n_axes; ++a) {
+    if (axes_dims[a] <= 0 || axes_dims[a] % 2 || pair + axes_dims[a] / 2 > d / 2) return VOMNI_EBADSHAPE;
+    for (int i = 0; i < axes_dims[a] / 2; ++i, ++pair) {
+      p.axis[pair] = static_cast<unsigned char>(a);
+      p.turns[pair] = std::pow(theta, -2.0 * i / axes_dims[a]) / 6.283185307179586476925286766559;
+    }
+  }
+  if (pair != d / 2) return VOMNI_EBADSHAPE;
+  rc = require_sm100();
+  if (rc) return rc;
+  p.t[0] = {q, q_out, q_heads, q_row_stride, q_batch_stride};
+  p.t[1] = {k, k_out, k_heads, k_row_stride, k_batch_stride};
+  p.tokens = static_cast<long long>(b) * s;
+  p.s = s;
+  p.d = d;
+  p.n_axes = n_axes;
+  p.pos = positions;
+  p.pos_type = pos_type;
+  p.pos_batch = pos_per_batch != 0;
+  p.half = pairing;
+  p.sign = inverse ? -1.f : 1.f;
+  // Few tokens: their heads are shared among CTAs until every thread has one group.
+  const int lanes = rotary::kThreads / (d / (2 * rotary::kGroup));
+  const int most = (q_heads + k_heads + lanes - 1) / lanes;
+  const long long want = (static_cast<long long>(num_sms()) * 4 + p.tokens - 1) / p.tokens;
+  p.head_blocks = static_cast<int>(want < most ? want : most);
+  const long long blocks = p.tokens * p.head_blocks;
+  if (blocks > 0x7fffffffll) return VOMNI_EBADSHAPE;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (dtype == 0)
+    rotary::rotary_kernel<__nv_bfloat16><<<static_cast<unsigned>(blocks), rotary::kThreads, 0, st>>>(p);
+  else if (dtype == 1)
+    rotary::rotary_kernel<__half><<<static_cast<unsigned>(blocks), rotary::kThreads, 0, st>>>(p);
+  else
+    rotary::rotary_kernel<float><<<static_cast<unsigned>(blocks), rotary::kThreads, 0, st>>>(p);
+  VOMNI_CUDA_TRY(cudaGetLastError());
+  return VOMNI_OK;
+}

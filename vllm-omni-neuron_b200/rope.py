@@ -8,11 +8,24 @@
 * :func:`deinterleave_perm`, :func:`deinterleave_qk_columns`, :func:`deinterleave_gamma_row` —
   vllm_omni_neuron/diffusion/quantization/row_mx_loaders.py:26-71: the per-head channel permutation
   that lets a rotate-half RoPE reproduce Wan's interleaved RoPE.
+
+On the device, from positions instead of tables:
+
+* :func:`rotary_axes` — rotary positions with several axes for query and key heads, differentiable.
+* :func:`wan_grid_positions` — the ``(frame, row, column)`` positions of a latent's patches.
 """
 
 from __future__ import annotations
 
+import ctypes
+
 import torch
+
+from . import _lib
+
+_PAIRINGS = {"interleaved": 0, "half": 1}
+_ROTARY_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_POSITION_DTYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
 
 
 def _rope_1d(dim: int, max_seq_len: int, theta: float):
@@ -77,3 +90,123 @@ def deinterleave_gamma_row(gamma: torch.Tensor, head_dim: int) -> torch.Tensor:
     perm = deinterleave_perm(head_dim).to(gamma.device)
     n = gamma.numel() // head_dim
     return gamma.reshape(n, head_dim).index_select(-1, perm).reshape(1, n * head_dim)
+
+
+# ---------------------------------------------------------------- rotary positions with several axes
+
+
+def wan_grid_positions(latent_fhw, patch_size=(1, 2, 2), device=None) -> torch.Tensor:
+    """``[S, 3]`` int32 ``(frame, row, column)`` of every patch of a ``(frames, height, width)`` latent, in the token
+    order of :func:`wan_rotary_freqs`."""
+    f, h, w = (n // p for n, p in zip(latent_fhw, patch_size))
+    i = torch.arange(f * h * w, dtype=torch.int32, device=device)
+    return torch.stack([i // (h * w), i // max(w, 1) % max(h, 1), i % max(w, 1)], dim=-1)
+
+
+def _rotary_source(t: torch.Tensor):
+    """(tensor, row stride, batch stride) as the kernel reads it: heads dense inside a token, strides of 16 bytes
+    (column slices of a fused projection pass as they are); anything else is copied."""
+    b, s, h, d = t.shape
+    esz = t.element_size()
+    row, batch = t.stride(1) if s > 1 else h * d, t.stride(0) if b > 1 else s * h * d
+    dense = (t.stride(3) == 1 or d == 1) and (h == 1 or t.stride(2) == d)
+    if dense and row >= h * d and batch >= 0 and (row * esz) % 16 == 0 and (batch * esz) % 16 == 0 and t.data_ptr() % 16 == 0:
+        return t, row, batch
+    t = t.contiguous()
+    t = t if t.data_ptr() % 16 == 0 else t.clone()
+    return t, h * d, s * h * d
+
+
+def _rotary(q, k, positions, axes_dims, theta, pairing, inverse):
+    b, s, hq, d = q.shape
+    dev = q.device
+    with torch.cuda.device(dev):
+        outs, args, keep = [], [], []
+        for t in (q, k):
+            if t is None or t.numel() == 0:
+                outs.append(None if t is None else torch.empty(t.shape, dtype=t.dtype, device=dev))
+                args += [None, None, 0, 0, 0]
+                continue
+            src, row, batch = _rotary_source(t)
+            out = torch.empty(t.shape, dtype=t.dtype, device=dev)
+            keep.append(src)
+            outs.append(out)
+            args += [src.data_ptr(), out.data_ptr(), t.shape[2], row, batch]
+        if keep:
+            pos = positions.contiguous()
+            axes = (ctypes.c_int * len(axes_dims))(*axes_dims)
+            rc = _lib.load().vomni_rotary_axes(
+                *args, b, s, d, pos.data_ptr(), _POSITION_DTYPES[pos.dtype], int(pos.dim() == 3), len(axes_dims), axes,
+                float(theta), pairing, int(inverse), _ROTARY_DTYPES[q.dtype], torch.cuda.current_stream(dev).cuda_stream)
+            _lib.check(rc, "vomni_rotary_axes")
+    return outs
+
+
+class _RotaryAxes(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, positions, axes_dims, theta, pairing, inverse):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(positions)
+        ctx.rest = (axes_dims, theta, pairing, inverse)
+        return tuple(_rotary(q, k, positions, axes_dims, theta, pairing, inverse))
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gq, gk):
+        (positions,) = ctx.saved_tensors
+        axes_dims, theta, pairing, inverse = ctx.rest
+        gq = gq if ctx.needs_input_grad[0] else None
+        gk = gk if ctx.needs_input_grad[1] else None
+        if gq is None and gk is None:
+            return (None,) * 7
+        first, second = (gq, gk) if gq is not None else (gk, None)
+        out = _rotary(first, second, positions, axes_dims, theta, pairing, not inverse)
+        dq, dk = out if gq is not None else (None, out[0])
+        return dq, dk, None, None, None, None, None
+
+
+def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, axes_dims, *, theta: float = 10000.0,
+                pairing: str = "interleaved", inverse: bool = False):
+    """Rotary positions with several axes, for query and key heads in one pass; differentiable in ``q`` and ``k``.
+
+    A head's ``d`` values are ``d / 2`` pairs, axis ``a`` owning the next ``axes_dims[a] / 2``; its pair ``i`` turns by
+    ``positions[..., a] * theta ** (-2 i / axes_dims[a])``. ``axes_dims=(44, 42, 42)`` with interleaved pairs is Wan's
+    rotary embedding (``WanRotaryPosEmbed`` + ``apply_rotary_emb_wan``, vllm_omni_neuron/diffusion/layers/rope.py:8-114).
+
+    * ``q [b, s, hq, d]``, ``k [b, s, hk, d]`` (or None) token-major, bf16 / fp16 / fp32, ``d % 16 == 0``, ``d <= 256``; the
+      column slices of a fused projection are read in place, other strides are copied first.
+    * ``positions`` ``[s, n_axes]`` or ``[b, s, n_axes]``, int32 / int64 / fp32 (fractions for interpolated positions),
+      any magnitude: angles are reduced in 64 bits. Not differentiated.
+    * ``pairing``: ``"interleaved"`` pairs values ``(2p, 2p + 1)``, ``"half"`` pairs ``(p, p + d / 2)``.
+    * ``inverse`` turns by the negative angles (what the gradient does).
+
+    Returns ``(q', k')``, dense tensors of the inputs' dtype (``q'`` alone when ``k`` is None); fp32 arithmetic, rounded once.
+    """
+    if pairing not in _PAIRINGS:
+        raise ValueError(f"unknown pairing {pairing!r}")
+    axes_dims = tuple(int(n) for n in axes_dims)
+    for name, t in (("q", q), ("k", k)):
+        if t is None and name == "k":
+            continue
+        if t.dim() != 4:
+            raise ValueError(f"{name} must be token-major [b, s, heads, d], got {tuple(t.shape)}")
+        if t.dtype not in _ROTARY_DTYPES:
+            raise TypeError(f"{name} must be bfloat16, float16 or float32, got {t.dtype}")
+    b, s, _, d = q.shape
+    if k is not None and (k.shape[0], k.shape[1], k.shape[3]) != (b, s, d):
+        raise ValueError(f"k {tuple(k.shape)} must match q {tuple(q.shape)} but for the heads")
+    if k is not None and k.dtype != q.dtype:
+        raise TypeError(f"q and k must have one dtype, got {q.dtype} and {k.dtype}")
+    if d % 16 or not 0 < d <= 256:
+        raise ValueError(f"head dim {d} unsupported (needs d % 16 == 0 and d <= 256)")
+    if not 1 <= len(axes_dims) <= 4 or any(n <= 0 or n % 2 for n in axes_dims) or sum(axes_dims) != d:
+        raise ValueError(f"axes_dims {axes_dims} must be 1 to 4 even counts that sum to the head dim {d}")
+    if positions.dtype not in _POSITION_DTYPES:
+        raise TypeError(f"positions must be int32, int64 or float32, got {positions.dtype}")
+    if tuple(positions.shape) not in ((s, len(axes_dims)), (b, s, len(axes_dims))):
+        raise ValueError(f"positions must be [{s}, {len(axes_dims)}] or [{b}, {s}, {len(axes_dims)}], got {tuple(positions.shape)}")
+    if not (theta > 0 and theta < float("inf")):
+        raise ValueError(f"theta must be positive and finite, got {theta}")
+    _lib.one_device(q, k, positions)
+    out = _RotaryAxes.apply(q, k, positions, axes_dims, float(theta), _PAIRINGS[pairing], bool(inverse))
+    return out[0] if k is None else out
