@@ -22,6 +22,8 @@
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
+
 #include "common.cuh"
 #include "host_util.h"
 
@@ -29,7 +31,8 @@ namespace vomni {
 namespace sandwich {
 
 constexpr int kMaxH = 8192;  // 8 columns a thread, 1024 threads
-constexpr int kLayer = 0, kNone = 2;  // 1: RMSNorm
+constexpr int kLayer = 0, kRms = 1, kNone = 2, kAsked = 3;
+constexpr size_t kSmemPerSm = 200 * 1024;
 constexpr int kPerGate = 1, kPerMul = 2, kPerAdd = 4;
 
 struct Params {
@@ -47,208 +50,515 @@ struct Params {
   float eps, inv_h;
   __nv_bfloat16* out0;  // forward: residual_out; backward: dx
   __nv_bfloat16* out1;  // forward: out; backward: dresidual
-  float* parts;         // backward: [n_mod][gridDim.x][3][H]
+  float* parts;         // backward: [n_mod][lanes][3][H]
+  int* status;          // device status word (bounded-wait timeouts)
+  int slots;            // ring slots
 };
+constexpr int kBuf = 8 * 32;  // up to eight sums of 32 warps
 
-VOMNI_DEV void unpack8(const uint4& w, float (&v)[8]) {
-  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[2 * i] = __uint_as_float(u[i] << 16);
-    v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
-  }
-}
-VOMNI_DEV uint4 pack8(const float (&v)[8]) {
-  return make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
-}
 VOMNI_DEV void load8(const float* p, float (&v)[8]) {
   const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
   v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
 }
 
-// Sums N values over the threads of a row: one warp (kWarpRow), or the whole CTA through shared memory.
-// Every thread ends with the same sums, added in the same order. `turn` alternates between two
-// buffers: a buffer is written again only after a barrier that follows its last read.
+// ---------------------------------------------------------------- sums over a row
+// Sums N values over a warp with N - 1 + log2(32 / N) shuffles: halves of the lanes exchange halves of the values until
+// each group of 32 / N lanes holds one value. Returns the sum of value lane / (32 / N).
+template <int N>
+VOMNI_DEV float warp_fold(float (&v)[N]) {
+  const int lane = threadIdx.x & 31;
+  int width = 16;
+#pragma unroll
+  for (int n = N; n > 1; n /= 2, width /= 2) {
+    const bool upper = lane & width;
+#pragma unroll
+    for (int i = 0; i < n / 2; ++i) {
+      const float send = upper ? v[i] : v[i + n / 2], keep = upper ? v[i + n / 2] : v[i];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, send, width);
+    }
+  }
+#pragma unroll
+  for (; width > 0; width /= 2) v[0] += __shfl_xor_sync(0xffffffffu, v[0], width);
+  return v[0];
+}
+
+// Sums N values over the threads that share a row (or a few rows): one warp (kWarpRow), or the whole CTA through
+// shared memory. Every thread ends with the same sums, added in an order that only the CTA's size sets. `turn`
+// alternates between two buffers: a buffer is written again only after a barrier that follows its last read. Entries
+// of warps that the CTA does not have are zero from the start.
 template <int N, bool kWarpRow>
-VOMNI_DEV void row_sum(float (&v)[N], float (*buf)[32 * 2], int& turn) {
+VOMNI_DEV void row_sum(float (&v)[N], float (*buf)[kBuf], int& turn) {
+  constexpr int kGroup = 32 / N;
+  const int lane = threadIdx.x & 31;
+  float s = warp_fold<N>(v);
+  if (!kWarpRow) {
+    float* b = buf[turn];
+    turn ^= 1;
+    if (lane % kGroup == 0) b[lane / kGroup * 32 + (threadIdx.x >> 5)] = s;
+    __syncthreads();
+    b += lane * N;  // value lane / kGroup, N of its 32 warps
+    if constexpr (N == 8) {
+      const float4 x = reinterpret_cast<const float4*>(b)[0], y = reinterpret_cast<const float4*>(b)[1];
+      s = ((x.x + x.y) + (x.z + x.w)) + ((y.x + y.y) + (y.z + y.w));
+    } else if constexpr (N == 4) {
+      const float4 x = *reinterpret_cast<const float4*>(b);
+      s = (x.x + x.y) + (x.z + x.w);
+    } else if constexpr (N == 2) {
+      const float2 x = *reinterpret_cast<const float2*>(b);
+      s = x.x + x.y;
+    } else {
+      s = b[0];
+    }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
-  if (kWarpRow) return;
-  static_assert(N <= 2, "buffer holds two values per warp");
-  float* b = buf[turn];
-  turn ^= 1;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-  if (lane == 0)
-#pragma unroll
-    for (int i = 0; i < N; ++i) b[i * 32 + warp] = v[i];
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = lane < warps ? b[i * 32 + lane] : 0.f;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
-}
-
-// v -> its normalised values; returns 1 / deviation. Two passes (mean, then squared deviations) in fp32.
-template <bool kWarpRow>
-VOMNI_DEV float normalise(float (&v)[8], int kind, bool in, const Params& p, float (*buf)[64], int& turn) {
-  if (kind == kNone) return 1.f;
-  float s[1];
-  if (kind == kLayer) {
-    s[0] = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
-    row_sum<1, kWarpRow>(s, buf, turn);
-    const float mean = s[0] * p.inv_h;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = in ? v[i] - mean : 0.f;
+    for (int o = kGroup / 2; o > 0; o /= 2) s += __shfl_xor_sync(0xffffffffu, s, o);
   }
-  s[0] = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) s[0] = fmaf(v[i], v[i], s[0]);
-  row_sum<1, kWarpRow>(s, buf, turn);
-  const float rstd = rsqrtf(s[0] * p.inv_h + p.eps);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] *= rstd;
-  return rstd;
+  for (int i = 0; i < N; ++i) v[i] = __shfl_sync(0xffffffffu, s, i * kGroup);
 }
 
-// d -> the gradient behind normalise(): rstd (d - [mean d] - hat mean(d hat)).
-template <bool kWarpRow>
-VOMNI_DEV void normalise_grad(float (&d)[8], const float (&hat)[8], float rstd, int kind, const Params& p,
-                              float (*buf)[64], int& turn) {
+// The values of R rows that a thread owns (C of each) as fp32 pairs: the packed arithmetic halves the instructions,
+// which bound the backward pass before it (87 a value, 64 % of the issue slots at half the present speed).
+template <int R, int C>
+struct Vals {
+  uint64_t v[R][C / 2];
+};
+VOMNI_DEV uint64_t both(float x) { return f2_pack(x, x); }
+VOMNI_DEV float halves_sum(uint64_t v) {
+  float a, b;
+  f2_unpack(v, a, b);
+  return a + b;
+}
+
+// x -> its normalised values. Two passes (mean, then squared deviations) in fp32. Columns behind
+// the row's end (whole chunks: in[j] false) hold zeros before and after.
+template <int R, int C, bool kWarpRow>
+VOMNI_DEV void normalise(Vals<R, C>& x, int kind, const bool (&in)[C / 8], const Params& p, float (*buf)[kBuf],
+                         int& turn) {
   if (kind == kNone) return;
-  float s[2] = {0.f, 0.f};
+  float s[R];
+  if (kind == kLayer) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    s[0] += d[i];
-    s[1] = fmaf(d[i], hat[i], s[1]);
+    for (int r = 0; r < R; ++r) {
+      uint64_t t = x.v[r][0];
+#pragma unroll
+      for (int i = 1; i < C / 2; ++i) t = f2_add(t, x.v[r][i]);
+      s[r] = halves_sum(t);
+    }
+    row_sum<R, kWarpRow>(s, buf, turn);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+#pragma unroll
+      for (int j = 0; j < C / 8; ++j) {
+        const uint64_t neg = both(in[j] ? -s[r] * p.inv_h : 0.f);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x.v[r][4 * j + i] = f2_add(x.v[r][4 * j + i], neg);
+      }
+    }
   }
-  row_sum<2, kWarpRow>(s, buf, turn);
-  const float m0 = kind == kLayer ? s[0] * p.inv_h : 0.f, m1 = s[1] * p.inv_h;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) d[i] = rstd * (d[i] - m0 - hat[i] * m1);
-}
-
-// A row per warp (kWarpRow: H <= 256, blockDim.y rows a CTA) or per CTA.
-template <int kMaxThreads, bool kWarpRow>
-__global__ void __launch_bounds__(kMaxThreads) sandwich_fwd_kernel(const Params p) {
-  __shared__ float buf[2][64];
-  int turn = 0;
-  const int c = threadIdx.x * 8;
-  const bool in = c < p.H;
-  const long long step = static_cast<long long>(gridDim.x) * blockDim.y;
-  for (long long row = static_cast<long long>(blockIdx.x) * blockDim.y + threadIdx.y; row < p.rows; row += step) {
-    const long long at = row * p.H + c;
-    const long long mod = row / p.rows_per_mod;
-    float r[8] = {};
-    if (in) unpack8(__ldcs(reinterpret_cast<const uint4*>(p.residual + at)), r);
-    if (p.x) {
-      float y[8] = {};
-      if (in) unpack8(__ldcs(reinterpret_cast<const uint4*>(p.x + at)), y);
-      normalise<kWarpRow>(y, p.post, in, p, buf, turn);
-      if (in) {
-        float w[8];
-        if (p.post_w) {
-          load8(p.post_w + c, w);
+  for (int r = 0; r < R; ++r) {
+    uint64_t t = f2_mul(x.v[r][0], x.v[r][0]);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) y[i] *= w[i];
-        }
-        if (p.gate) {
-          load8(p.gate + mod * p.gate_step + c, w);
+    for (int i = 1; i < C / 2; ++i) t = f2_fma(x.v[r][i], x.v[r][i], t);
+    s[r] = halves_sum(t);
+  }
+  row_sum<R, kWarpRow>(s, buf, turn);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) r[i] = fmaf(w[i], y[i], r[i]);
-        } else {
+  for (int r = 0; r < R; ++r) {
+    const uint64_t rstd = both(rsqrtf(s[r] * p.inv_h + p.eps));
 #pragma unroll
-          for (int i = 0; i < 8; ++i) r[i] += y[i];
-        }
-        __stcs(reinterpret_cast<uint4*>(p.out0 + at), pack8(r));
-      }
-    }
-    normalise<kWarpRow>(r, p.norm, in, p, buf, turn);
-    if (in) {
-      float m[8], a[8];
-      if (p.mul) {
-        load8(p.mul + mod * p.mul_step + c, m);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) r[i] *= m[i];
-      }
-      if (p.add) {
-        load8(p.add + mod * p.add_step + c, a);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) r[i] += a[i];
-      }
-      __stcs(reinterpret_cast<uint4*>(p.out1 + at), pack8(r));
-    }
+    for (int i = 0; i < C / 2; ++i) x.v[r][i] = f2_mul(x.v[r][i], rstd);
   }
 }
 
-// gridDim.y modulation rows; the rows of one are dealt to gridDim.x CTAs (x blockDim.y warps).
-template <int kMaxThreads, bool kWarpRow>
-__global__ void __launch_bounds__(kMaxThreads) sandwich_bwd_kernel(const Params p) {
-  __shared__ float buf[2][64];
-  int turn = 0;
-  const int c = threadIdx.x * 8;
-  const bool in = c < p.H;
-  const long long mod = blockIdx.y;
-  const long long end = (mod + 1) * p.rows_per_mod;
-  const int lanes = gridDim.x * blockDim.y, lane = blockIdx.x * blockDim.y + threadIdx.y;
-  float sum_a[8] = {}, sum_m[8] = {}, sum_d[8] = {};
-  for (long long row = mod * p.rows_per_mod + lane; row < end; row += lanes) {
-    const long long at = row * p.H + c;
-    float dr[8] = {}, n[8] = {}, w[8];
-    if (in && p.d_res) unpack8(__ldcs(reinterpret_cast<const uint4*>(p.d_res + at)), dr);
-    if (p.d_out) {
-      float g[8] = {};
-      if (in) {
-        unpack8(__ldcs(reinterpret_cast<const uint4*>(p.d_out + at)), g);
-        unpack8(__ldcs(reinterpret_cast<const uint4*>(p.residual + at)), n);
-      }
-      const float rstd = normalise<kWarpRow>(n, p.norm, in, p, buf, turn);
+// ---------------------------------------------------------------- rows in shared memory
+// A CTA's rows come R at a time (adjacent rows: one bulk copy per tensor) through a ring of `slots` slots; one thread
+// issues the copies, slots - 1 groups ahead.
+constexpr int kMaxSlots = 4;
+constexpr int kSiteRowWait = 0x48, kSiteRowDrain = 0x49;
+
+struct Ring {
+  uint4* mem;  // [slots][tensors][R * H / 8]
+  uint64_t* full;
+  int slots, tensors, chunks;  // chunks: R * H / 8
+};
+
+template <int R>
+VOMNI_DEV void ring_issue(const Ring& g, const __nv_bfloat16* const (&src)[4], long long row, long long end, int H, int slot) {
+  if (row >= end) return;
+  const uint32_t bytes = static_cast<uint32_t>(min(static_cast<long long>(R), end - row)) * H * 2u;
+  mbar_expect_tx(&g.full[slot], bytes * g.tensors);
+  uint4* dst = g.mem + static_cast<size_t>(slot) * g.tensors * g.chunks;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        sum_m[i] = fmaf(g[i], n[i], sum_m[i]);
-        sum_d[i] += g[i];
-      }
-      if (p.mul && in) {
-        load8(p.mul + mod * p.mul_step + c, w);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) g[i] *= w[i];
-      }
-      normalise_grad<kWarpRow>(g, n, rstd, p.norm, p, buf, turn);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) dr[i] = in ? dr[i] + g[i] : 0.f;
+  for (int t = 0, n = 0; t < 4; ++t)
+    if (src[t]) bulk_g2s(dst + (n++) * g.chunks, src[t] + row * H, bytes, &g.full[slot]);
+}
+
+// The walk of a CTA over its groups of R rows of one modulation row: groups lane, lane + lanes, ... of
+// ceil(rows_per_mod / R). body(row, rows, slot base) runs between the wait for the group and the barrier that frees
+// its slot.
+template <int R, typename Body>
+VOMNI_DEV void walk_rows(const Params& p, const __nv_bfloat16* const (&src)[4], int tensors, uint8_t* smem, uint64_t* full,
+                         int* abort_flag, Body&& body) {
+  Ring g{reinterpret_cast<uint4*>(smem), full, p.slots, tensors, R * p.H / 8};
+  volatile int* abort = abort_flag;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < g.slots; ++s) mbar_init(&full[s], 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+  const long long begin = static_cast<long long>(blockIdx.y) * p.rows_per_mod, end = begin + p.rows_per_mod;
+  const long long first = begin + static_cast<long long>(blockIdx.x) * R, step = static_cast<long long>(gridDim.x) * R;
+  long long ahead = first;
+  if (threadIdx.x == 0)
+    for (int s = 0; s < g.slots - 1; ++s, ahead += step) ring_issue<R>(g, src, ahead, end, p.H, s);
+  int slot = 0;
+  uint32_t phase = 0;
+  long long row = first;
+  for (; row < end; row += step) {
+    if (threadIdx.x == 0) {  // into the slot that the last barrier freed
+      fence_proxy_async_smem();
+      ring_issue<R>(g, src, ahead, end, p.H, slot == 0 ? g.slots - 1 : slot - 1);
+      ahead += step;
     }
-    if (in) __stcs(reinterpret_cast<uint4*>(p.out1 + at), pack8(dr));
-    if (p.x) {
-      float y[8] = {};
-      if (in) unpack8(__ldcs(reinterpret_cast<const uint4*>(p.x + at)), y);
-      const float rstd = normalise<kWarpRow>(y, p.post, in, p, buf, turn);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) sum_a[i] = fmaf(dr[i], y[i], sum_a[i]);
-      if (in && p.gate) {
-        load8(p.gate + mod * p.gate_step + c, w);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) dr[i] *= w[i];
-      }
-      if (in && p.post_w) {
-        load8(p.post_w + c, w);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) dr[i] *= w[i];
-      }
-      normalise_grad<kWarpRow>(dr, y, rstd, p.post, p, buf, turn);
-      if (in) __stcs(reinterpret_cast<uint4*>(p.out0 + at), pack8(dr));
+    const bool ok = mbar_wait(&full[slot], phase, abort, p.status, VOMNI_DEV_TIMEOUT_BASE + kSiteRowWait);
+    body(row, static_cast<int>(min(static_cast<long long>(R), end - row)),
+         g.mem + static_cast<size_t>(slot) * tensors * g.chunks, g.chunks);
+    if (__syncthreads_or(!ok)) break;
+    if (++slot == g.slots) {
+      slot = 0;
+      phase ^= 1;
     }
   }
-  if (!in) return;
-  float* part = p.parts + (mod * lanes + lane) * 3 * p.H + c;
+  if (*abort && threadIdx.x == 0) {  // copies still in flight into this CTA's memory: groups from `row` on
+    for (; row < end && row < ahead; row += step) {
+      int ignored = 0;
+      if (!mbar_wait(&full[slot], phase, &ignored, p.status, VOMNI_DEV_TIMEOUT_BASE + kSiteRowDrain)) break;
+      if (++slot == g.slots) {
+        slot = 0;
+        phase ^= 1;
+      }
+    }
+  }
+}
+
+// A thread's columns of the vectors: constant over a CTA's rows, as all of them belong to one modulation row.
+template <int C>
+struct Vecs {
+  uint64_t gw[C / 2], mul[C / 2], add[C / 2];  // gate * post_w, mul, add (1, 1 and 0 where absent)
+};
+template <int C>
+VOMNI_DEV void times(const float* p, const bool (&in)[C / 8], int stride, uint64_t (&v)[C / 2]) {
+#pragma unroll
+  for (int j = 0; j < C / 8; ++j)
+    if (in[j]) {
+      float t[8];
+      load8(p + j * stride, t);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[4 * j + i] = f2_mul(v[4 * j + i], f2_pack(t[2 * i], t[2 * i + 1]));
+    }
+}
+template <int C>
+VOMNI_DEV void load_vecs(const Params& p, long long mod, int c, int stride, const bool (&in)[C / 8], Vecs<C>& w) {
+  const uint64_t one = both(1.f);
+#pragma unroll
+  for (int i = 0; i < C / 2; ++i) {
+    w.gw[i] = w.mul[i] = one;
+    w.add[i] = p.add ? one : 0ull;
+  }
+  if (p.gate) times<C>(p.gate + mod * p.gate_step + c, in, stride, w.gw);
+  if (p.post_w) times<C>(p.post_w + c, in, stride, w.gw);
+  if (p.mul) times<C>(p.mul + mod * p.mul_step + c, in, stride, w.mul);
+  if (p.add) times<C>(p.add + mod * p.add_step + c, in, stride, w.add);
+}
+
+// One group of R rows, forward. load(t, r, v): the thread's values of row r of tensor t (0 x, 1 residual; zero behind the
+// row's end); store(t, r, v): to output t.
+template <int R, int NV, bool kWarpRow, typename Load, typename Store>
+VOMNI_DEV void forward_rows(const Params& p, const Vecs<NV * 8>& w, const bool (&in)[NV], float (*buf)[kBuf], int& turn,
+                            Load&& load, Store&& store) {
+  constexpr int C = NV * 8;
+  Vals<R, C> x;
+#pragma unroll
+  for (int r = 0; r < R; ++r) load(p.x ? 0 : 1, r, x.v[r]);
+  if (p.x) {
+    normalise<R, C, kWarpRow>(x, p.post, in, p, buf, turn);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      uint64_t res[C / 2];
+      load(1, r, res);
+#pragma unroll
+      for (int i = 0; i < C / 2; ++i) x.v[r][i] = f2_fma(x.v[r][i], w.gw[i], res[i]);
+      store(0, r, x.v[r]);
+    }
+  }
+  normalise<R, C, kWarpRow>(x, p.norm, in, p, buf, turn);
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+#pragma unroll
+    for (int i = 0; i < C / 2; ++i) x.v[r][i] = f2_fma(x.v[r][i], w.mul[i], w.add[i]);
+    store(1, r, x.v[r]);
+  }
+}
+
+// One group of R rows, backward. load(t, r, v): the thread's values of row r of tensor t (0 x, 1 residual_out, 2 d_res,
+// 3 d_out; zero behind the row's end); store(t, r, v): to output t. x and residual_out are read from the
+// slot again for each of their statistics instead of being kept: the accumulators and vectors leave registers for two
+// tensors of values.
+// kPost, kNorm: the kinds, or kAsked to go by the call's; kAll: x, d_res and d_out are all there.
+template <int R, int NV, bool kWarpRow, int kPost, int kNorm, bool kAll, typename Load, typename Store>
+VOMNI_DEV void backward_rows(const Params& p, const Vecs<NV * 8>& w, const bool (&in)[NV], float (*buf)[kBuf], int& turn,
+                             uint64_t (&sum_a)[NV * 4], uint64_t (&sum_m)[NV * 4], uint64_t (&sum_d)[NV * 4], Load&& load,
+                             Store&& store) {
+  constexpr int C = NV * 8, P = C / 2;
+  // statistics of both tensors: 2 r the residual's row r, 2 r + 1 x's
+  float mean[2 * R] = {}, rstd[2 * R], s[2 * R];
+  const bool has_x = kAll || p.x, has_out = kAll || p.d_out, has_res = kAll || p.d_res;
+  const int kind[2] = {kNorm != kAsked ? kNorm : has_out ? p.norm : kNone, kPost != kAsked ? kPost : has_x ? p.post : kNone};
+  auto centred = [&](int q, int r, uint64_t (&v)[P]) {
+    load(q ? 0 : 1, r, v);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const uint64_t neg = both(in[j] ? -mean[2 * r + q] : 0.f);
+#pragma unroll
+      for (int i = 4 * j; i < 4 * j + 4; ++i) v[i] = f2_add(v[i], neg);
+    }
+  };
+  auto hat = [&](int q, int r, uint64_t (&v)[P]) {
+    centred(q, r, v);
+#pragma unroll
+    for (int i = 0; i < P; ++i) v[i] = f2_mul(v[i], both(rstd[2 * r + q]));
+  };
+  if (kind[0] == kLayer || kind[1] == kLayer) {
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        s[2 * r + q] = 0.f;
+        if (kind[q] != kLayer) continue;
+        uint64_t v[P];
+        load(q ? 0 : 1, r, v);
+        uint64_t t = v[0];
+#pragma unroll
+        for (int i = 1; i < P; ++i) t = f2_add(t, v[i]);
+        s[2 * r + q] = halves_sum(t);
+      }
+    row_sum<2 * R, kWarpRow>(s, buf, turn);
+#pragma unroll
+    for (int i = 0; i < 2 * R; ++i) mean[i] = s[i] * p.inv_h;
+  }
+  if (kind[0] != kNone || kind[1] != kNone) {
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        s[2 * r + q] = 0.f;
+        if (kind[q] == kNone) continue;
+        uint64_t v[P];
+        centred(q, r, v);
+        uint64_t t = f2_mul(v[0], v[0]);
+#pragma unroll
+        for (int i = 1; i < P; ++i) t = f2_fma(v[i], v[i], t);
+        s[2 * r + q] = halves_sum(t);
+      }
+    row_sum<2 * R, kWarpRow>(s, buf, turn);
+  }
+#pragma unroll
+  for (int i = 0; i < 2 * R; ++i) rstd[i] = kind[i & 1] == kNone ? 1.f : rsqrtf(s[i] * p.inv_h + p.eps);
+
+  // the sums that normalise's gradient needs of g and g * hat
+  auto pair_sums = [&](int r, const uint64_t (&g)[P], const uint64_t (&h)[P]) {
+    uint64_t t = g[0], u = f2_mul(g[0], h[0]);
+#pragma unroll
+    for (int i = 1; i < P; ++i) {
+      t = f2_add(t, g[i]);
+      u = f2_fma(g[i], h[i], u);
+    }
+    s[2 * r] = halves_sum(t);
+    s[2 * r + 1] = halves_sum(u);
+  };
+  // g -> rstd (g - [mean g] - hat mean(g hat))
+  auto behind = [&](int q, int r, uint64_t (&g)[P], const uint64_t (&h)[P]) {
+    const float k = rstd[2 * r + q];
+    const uint64_t c1 = both(-k * (s[2 * r + 1] * p.inv_h)), k2 = both(k);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const uint64_t c0 = both(in[j] && kind[q] == kLayer ? -k * (s[2 * r] * p.inv_h) : 0.f);
+#pragma unroll
+      for (int i = 4 * j; i < 4 * j + 4; ++i) g[i] = f2_fma(g[i], k2, f2_fma(h[i], c1, c0));
+    }
+  };
+  uint64_t d[R][P], h[R][P], v[P];  // h: the normalised rows of the tensor at hand
+  if (has_out) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      hat(0, r, h[r]);
+      load(3, r, d[r]);
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        sum_m[i] = f2_fma(d[r][i], h[r][i], sum_m[i]);
+        sum_d[i] = f2_add(sum_d[i], d[r][i]);
+        d[r][i] = f2_mul(d[r][i], w.mul[i]);
+      }
+      pair_sums(r, d[r], h[r]);
+    }
+    if (kind[0] != kNone) {
+      row_sum<2 * R, kWarpRow>(s, buf, turn);
+#pragma unroll
+      for (int r = 0; r < R; ++r) behind(0, r, d[r], h[r]);
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    if (!has_out) {
+      load(2, r, d[r]);
+    } else if (has_res) {
+      load(2, r, v);
+#pragma unroll
+      for (int i = 0; i < P; ++i) d[r][i] = f2_add(d[r][i], v[i]);
+    }
+    store(1, r, d[r]);
+    if (!has_x) continue;
+    hat(1, r, h[r]);
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      sum_a[i] = f2_fma(d[r][i], h[r][i], sum_a[i]);
+      d[r][i] = f2_mul(d[r][i], w.gw[i]);
+    }
+    pair_sums(r, d[r], h[r]);
+  }
+  if (!has_x) return;
+  if (kind[1] != kNone) row_sum<2 * R, kWarpRow>(s, buf, turn);
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    if (kind[1] != kNone) behind(1, r, d[r], h[r]);
+    store(0, r, d[r]);
+  }
+}
+
+VOMNI_DEV void unpack_pairs(const uint4& w, uint64_t* v) {
+  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = f2_pack(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xffff0000u));
+}
+VOMNI_DEV uint4 pack_pairs(const uint64_t* v) {
+  uint32_t u[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float a, b;
+    f2_unpack(v[i], a, b);
+    u[i] = pack_bf16x2(a, b);
+  }
+  return make_uint4(u[0], u[1], u[2], u[3]);
+}
+
+template <int C>
+VOMNI_DEV void store_sums(float* part, int H, int stride, const bool (&in)[C / 8], const uint64_t (&a)[C / 2],
+                          const uint64_t (&m)[C / 2], const uint64_t (&d)[C / 2]) {
 #pragma unroll
   for (int q = 0; q < 3; ++q) {
-    const float(&s)[8] = q == 0 ? sum_a : q == 1 ? sum_m : sum_d;
-    reinterpret_cast<float4*>(part + static_cast<size_t>(q) * p.H)[0] = make_float4(s[0], s[1], s[2], s[3]);
-    reinterpret_cast<float4*>(part + static_cast<size_t>(q) * p.H)[1] = make_float4(s[4], s[5], s[6], s[7]);
+    const uint64_t(&s)[C / 2] = q == 0 ? a : q == 1 ? m : d;
+#pragma unroll
+    for (int j = 0; j < C / 8; ++j) {
+      if (!in[j]) continue;
+      ulonglong2* at = reinterpret_cast<ulonglong2*>(part + static_cast<size_t>(q) * H + j * stride);
+      at[0] = make_ulonglong2(s[4 * j], s[4 * j + 1]);
+      at[1] = make_ulonglong2(s[4 * j + 2], s[4 * j + 3]);
+    }
   }
+}
+
+// A CTA takes R rows at a time; a thread owns chunks (8 columns) threadIdx.x + j * blockDim.x, j < NV.
+// kFull: the threads' chunks tile the row exactly, so none carries a predicate.
+template <int R, int NV, int kMaxThreads, bool kFull, bool kBackward, int kPost = kAsked, int kNorm = kAsked, bool kAll = false>
+__global__ void __launch_bounds__(kMaxThreads, 1) sandwich_kernel(const __grid_constant__ Params p) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ __align__(8) uint64_t full[kMaxSlots];
+  __shared__ int abort_flag;
+  __shared__ __align__(16) float buf[2][kBuf];
+  for (int i = threadIdx.x; i < 2 * kBuf; i += blockDim.x) buf[i / kBuf][i % kBuf] = 0.f;  // walk_rows begins with a barrier
+  constexpr int C = NV * 8;
+  int turn = 0;
+  const int c = threadIdx.x * 8, stride = blockDim.x * 8;
+  bool in[NV];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) in[j] = kFull || c + j * stride < p.H;
+  const __nv_bfloat16* src[4] = {p.x, (kBackward && !p.d_out) ? nullptr : p.residual, p.d_res, p.d_out};
+  int at[4], tensors = 0;
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    at[t] = kAll ? t : tensors;
+    tensors = kAll ? 4 : tensors + (src[t] != nullptr);
+  }
+  Vecs<C> w;
+  load_vecs<C>(p, blockIdx.y, c, stride, in, w);
+  uint64_t sum_a[C / 2] = {}, sum_m[C / 2] = {}, sum_d[C / 2] = {};
+  walk_rows<R>(p, src, tensors, smem, full, &abort_flag, [&](long long row, int rows, uint4* slot, int chunks) {
+    const int pitch = p.H >> 3;
+    if (R > 1 && rows < R) {  // the last group: zeros in place of the missing rows (a thread reads only its own chunks)
+      for (int t = 0; t < tensors; ++t)
+        for (int r = rows; r < R; ++r)
+#pragma unroll
+          for (int j = 0; j < NV; ++j)
+            if (in[j]) slot[t * chunks + r * pitch + threadIdx.x + j * blockDim.x] = make_uint4(0, 0, 0, 0);
+    }
+    auto load = [&](int t, int r, uint64_t (&x)[C / 2]) {
+      const uint4* s = slot + at[t] * chunks + r * pitch + threadIdx.x;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (in[j]) v = s[j * blockDim.x];
+        unpack_pairs(v, &x[4 * j]);
+      }
+    };
+    auto store = [&](int t, int r, const uint64_t (&x)[C / 2]) {
+      __nv_bfloat16* out = (t ? p.out1 : p.out0) + (row + r) * p.H + c;
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+        if (in[j] && (R == 1 || r < rows)) __stcs(reinterpret_cast<uint4*>(out + j * stride), pack_pairs(&x[4 * j]));
+    };
+    if constexpr (kBackward)
+      backward_rows<R, NV, false, kPost, kNorm, kAll>(p, w, in, buf, turn, sum_a, sum_m, sum_d, load, store);
+    else
+      forward_rows<R, NV, false>(p, w, in, buf, turn, load, store);
+  });
+  if constexpr (kBackward)
+    store_sums<C>(p.parts + (static_cast<long long>(blockIdx.y) * gridDim.x + blockIdx.x) * 3 * p.H + c, p.H, stride, in, sum_a,
+                  sum_m, sum_d);
+}
+
+// Short rows (H <= 256): a row per warp, four warps a CTA, straight from global memory.
+template <bool kBackward>
+__global__ void __launch_bounds__(128) sandwich_warp_kernel(const __grid_constant__ Params p) {
+  const int c = threadIdx.x * 8;
+  const bool in[1] = {c < p.H};
+  const long long end = (static_cast<long long>(blockIdx.y) + 1) * p.rows_per_mod;
+  const int lanes = gridDim.x * blockDim.y, lane = blockIdx.x * blockDim.y + threadIdx.y;
+  Vecs<8> w;
+  load_vecs<8>(p, blockIdx.y, c, 0, in, w);
+  uint64_t sum_a[4] = {}, sum_m[4] = {}, sum_d[4] = {};
+  int turn = 0;
+  const __nv_bfloat16* src[4] = {p.x, p.residual, p.d_res, p.d_out};
+  for (long long row = static_cast<long long>(blockIdx.y) * p.rows_per_mod + lane; row < end; row += lanes) {
+    const long long at = row * p.H + c;
+    uint4 raw[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      raw[t] = make_uint4(0, 0, 0, 0);
+      if (in[0] && src[t]) raw[t] = __ldcs(reinterpret_cast<const uint4*>(src[t] + at));
+    }
+    auto load = [&](int t, int, uint64_t (&x)[4]) { unpack_pairs(raw[t], x); };
+    auto store = [&](int t, int, const uint64_t (&x)[4]) {
+      if (in[0]) __stcs(reinterpret_cast<uint4*>((t ? p.out1 : p.out0) + at), pack_pairs(x));
+    };
+    if constexpr (kBackward)
+      backward_rows<1, 1, true, kAsked, kAsked, false>(p, w, in, nullptr, turn, sum_a, sum_m, sum_d, load, store);
+    else
+      forward_rows<1, 1, true>(p, w, in, nullptr, turn, load, store);
+  }
+  if constexpr (kBackward)
+    store_sums<8>(p.parts + (static_cast<long long>(blockIdx.y) * lanes + lane) * 3 * p.H + c, p.H, 0, in, sum_a, sum_m, sum_d);
 }
 
 struct SumParams {
@@ -298,28 +608,103 @@ __global__ void __launch_bounds__(256) sandwich_sum_kernel(const SumParams p) {
   }
 }
 
-// Threads of a row (a multiple of 32) and rows per CTA.
+// How a call is laid out: a row per warp, or R rows at a time per CTA with NV chunks a thread.
 struct Shape {
-  int tx, ty;
+  bool warp_row;
+  int nv, rows, threads;  // rows: R
+  int lanes;              // CTAs (x warps) that share a modulation row's tokens
+  unsigned blocks;        // gridDim.x
+  int slots;
+  size_t smem;
 };
-Shape shape_of(int h) {
+Shape shape_of(long long rows_per_mod, long long n_mod, int h, int tensors, bool backward) {
+  Shape s = {};
   const int chunks = h / 8;
-  if (chunks <= 32) return {32, 4};
-  return {(chunks + 31) / 32 * 32, 1};
-}
-// Lanes (CTAs x rows per CTA) that share a modulation row's tokens in the backward pass: enough to fill
-// the device once over all modulation rows.
-int bwd_blocks(long long rows_per_mod, long long n_mod, const Shape& sh) {
-  const int per_sm = 1024 / (sh.tx * sh.ty) > 0 ? 1024 / (sh.tx * sh.ty) : 1;
+  s.warp_row = chunks <= 32;
+  if (s.warp_row) {
+    const long long need = (rows_per_mod + 3) / 4, cap = (static_cast<long long>(num_sms()) * 8 + n_mod - 1) / n_mod;
+    s.blocks = static_cast<unsigned>(need < cap ? need : cap);
+    s.lanes = static_cast<int>(s.blocks) * 4;
+    return s;
+  }
+  // Few rows: one at a time, so that they spread over the device. Else a thread of the backward pass takes two chunks
+  // of a row and two rows, of the forward pass one and four (kernel_of says why).
+  const bool many = rows_per_mod * n_mod >= 4ll * num_sms();
+  s.nv = chunks > 640 || (backward && many) ? 2 : 1;
+  s.threads = ((chunks + s.nv - 1) / s.nv + 31) / 32 * 32;
+  s.rows = chunks > 640 || !many ? 1 : backward ? 2 : 4;
+  const size_t slot = static_cast<size_t>(s.rows) * h * 2 * tensors;
+  const int per_sm = std::max(1, std::min((backward && many ? 320 : 640) / s.threads, 8));
+  const size_t room = (kSmemPerSm / per_sm);
+  s.slots = static_cast<int>(std::max<size_t>(2, std::min<size_t>(kMaxSlots, room / slot)));
+  s.smem = slot * s.slots;
+  const long long need = (rows_per_mod + s.rows - 1) / s.rows;
   const long long cap = (static_cast<long long>(num_sms()) * per_sm + n_mod - 1) / n_mod;
-  const long long need = (rows_per_mod + sh.ty - 1) / sh.ty;
-  return static_cast<int>(need < cap ? need : cap);
+  s.blocks = static_cast<unsigned>(need < cap ? need : cap);
+  s.lanes = static_cast<int>(s.blocks);
+  return s;
 }
 
-int check(long long rows, int h, long long rows_per_mod, int post, int norm) {
+typedef void (*Kernel)(Params);
+
+// The backward kernels that know their norms at compile time (430 us instead of 574 at 32760 x 5120): those of a call
+// with a branch and both gradients.
+template <int R, int NV, int kMaxThreads, bool kFull>
+Kernel backward_of(const Params& p) {
+  if (!p.x || !p.d_res || !p.d_out) return sandwich_kernel<R, NV, kMaxThreads, kFull, true>;
+  switch (p.post * 3 + p.norm) {
+    case 0: return sandwich_kernel<R, NV, kMaxThreads, kFull, true, 0, 0, true>;
+    case 1: return sandwich_kernel<R, NV, kMaxThreads, kFull, true, 0, 1, true>;
+    case 2: return sandwich_kernel<R, NV, kMaxThreads, kFull, true, 0, 2, true>;
+    case 3: return sandwich_kernel<R, NV, kMaxThreads, kFull, true, 1, 0, true>;
+    case 4: return sandwich_kernel<R, NV, kMaxThreads, kFull, true, 1, 1, true>;
+    case 5: return sandwich_kernel<R, NV, kMaxThreads, kFull, true, 1, 2, true>;
+    case 6: return sandwich_kernel<R, NV, kMaxThreads, kFull, true, 2, 0, true>;
+    case 7: return sandwich_kernel<R, NV, kMaxThreads, kFull, true, 2, 1, true>;
+    default: return sandwich_kernel<R, NV, kMaxThreads, kFull, true, 2, 2, true>;
+  }
+}
+
+// Rows at a time and chunks a thread. The reductions cost a warp the same for one value a thread as for many and all
+// warps wait for each other in them, so more of both is better while registers and shared memory last. Measured at
+// 32760 x 5120: forward 393 / 299 / 228 us with 1 / 2 / 4 rows of one chunk; backward 402 us with two rows of one
+// chunk (640 threads), 381 us with two rows of two (320), 624 us with one row of two, 740 us with one row of four.
+template <bool kBackward>
+Kernel kernel_of(const Params& p, const Shape& s) {
+  const bool full = s.threads * s.nv * 8 == p.H;
+  if constexpr (kBackward) {
+    if (s.rows == 2) return full ? backward_of<2, 2, 320, true>(p) : backward_of<2, 2, 320, false>(p);
+    if (s.nv == 2) return backward_of<1, 2, 512, false>(p);
+    return sandwich_kernel<1, 1, 640, false, true>;
+  } else {
+    if (s.rows == 4) return full ? sandwich_kernel<4, 1, 640, true, false> : sandwich_kernel<4, 1, 640, false, false>;
+    if (s.nv == 2) return sandwich_kernel<1, 2, 512, false, false>;
+    return sandwich_kernel<1, 1, 640, false, false>;
+  }
+}
+
+template <bool kBackward>
+int launch(Params p, long long n_mod, const Shape& s, cudaStream_t st) {
+  p.slots = s.slots;
+  p.status = device_status_ptr();
+  const dim3 grid(s.blocks, static_cast<unsigned>(n_mod));
+  if (s.warp_row) {
+    sandwich_warp_kernel<kBackward><<<grid, dim3(32, 4), 0, st>>>(p);
+  } else {
+    const Kernel kern = kernel_of<kBackward>(p, s);
+    int rc = ensure_max_smem(kern, static_cast<int>(s.smem));
+    if (rc) return rc;
+    kern<<<grid, s.threads, s.smem, st>>>(p);
+  }
+  VOMNI_CUDA_TRY(cudaGetLastError());
+  return VOMNI_OK;
+}
+
+int check(long long rows, int h, long long rows_per_mod, int post, int norm, float eps) {
   if (rows <= 0 || rows > 0x7fffffffLL || h <= 0 || h > kMaxH || h % 8) return VOMNI_EBADSHAPE;
   if (rows_per_mod <= 0 || rows % rows_per_mod) return VOMNI_EBADSHAPE;
   if (post < 0 || post > 2 || norm < 0 || norm > 2) return VOMNI_EINVAL;
+  if (!(eps > 0.f && eps <= 3.0e38f)) return VOMNI_EINVAL;  // rows behind the last one are zero: eps keeps them finite
   return VOMNI_OK;
 }
 bool misaligned(const void* a, const void* b = nullptr, const void* c = nullptr, const void* d = nullptr) {
@@ -358,35 +743,26 @@ extern "C" int vomni_sandwich_norm(const void* x, const void* residual, const fl
   using namespace sandwich;
   if (!residual || !out || (x && !residual_out) || (per_mod & ~7)) return VOMNI_EINVAL;
   if (!x && (gate || post_weight)) return VOMNI_EINVAL;
-  int rc = check(rows, h, rows_per_mod, post_norm, norm_type);
+  int rc = check(rows, h, rows_per_mod, post_norm, norm_type, eps);
   if (rc) return rc;
   if (misaligned(x, residual, residual_out, out) || misaligned(gate, post_weight, mul, add)) return VOMNI_EALIGN;
   rc = require_sm100();
   if (rc) return rc;
+  if (rows / rows_per_mod > 65535) return VOMNI_EBADSHAPE;
   Params p = {};
   fill(p, x, residual, gate, post_weight, mul, add, rows, h, rows_per_mod, per_mod, eps, post_norm, norm_type);
   p.out0 = static_cast<__nv_bfloat16*>(residual_out);
   p.out1 = static_cast<__nv_bfloat16*>(out);
-  const Shape sh = shape_of(h);
-  const dim3 block(sh.tx, sh.ty);
-  const unsigned grid = static_cast<unsigned>((rows + sh.ty - 1) / sh.ty);
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (sh.tx == 32)
-    sandwich_fwd_kernel<128, true><<<grid, block, 0, st>>>(p);
-  else if (sh.tx <= 512)
-    sandwich_fwd_kernel<512, false><<<grid, block, 0, st>>>(p);
-  else
-    sandwich_fwd_kernel<1024, false><<<grid, block, 0, st>>>(p);
-  VOMNI_CUDA_TRY(cudaGetLastError());
-  return VOMNI_OK;
+  const long long n_mod = rows / rows_per_mod;
+  return launch<false>(p, n_mod, shape_of(rows_per_mod, n_mod, h, x ? 2 : 1, false),
+                       reinterpret_cast<cudaStream_t>(stream));
 }
 
 extern "C" size_t vomni_sandwich_norm_workspace_bytes(long long rows, int h, long long rows_per_mod) {
   using namespace sandwich;
-  if (check(rows, h, rows_per_mod, 0, 0)) return 0;
-  const Shape sh = shape_of(h);
+  if (check(rows, h, rows_per_mod, 0, 0, 1.f)) return 0;
   const long long n_mod = rows / rows_per_mod;
-  return static_cast<size_t>(n_mod) * bwd_blocks(rows_per_mod, n_mod, sh) * sh.ty * 3 * h * sizeof(float);
+  return static_cast<size_t>(n_mod) * shape_of(rows_per_mod, n_mod, h, 4, true).lanes * 3 * h * sizeof(float);
 }
 
 extern "C" int vomni_sandwich_norm_bwd(const void* grad_residual_out, const void* grad_out, const void* x,
@@ -399,7 +775,7 @@ extern "C" int vomni_sandwich_norm_bwd(const void* grad_residual_out, const void
   if ((!grad_residual_out && !grad_out) || !dresidual || !workspace || (per_mod & ~7)) return VOMNI_EINVAL;
   if (grad_out && !residual_out) return VOMNI_EINVAL;
   if (x ? !dx : (gate || post_weight || dgate || dpost_weight || dx)) return VOMNI_EINVAL;
-  int rc = check(rows, h, rows_per_mod, post_norm, norm_type);
+  int rc = check(rows, h, rows_per_mod, post_norm, norm_type, eps);
   if (rc) return rc;
   const long long n_mod = rows / rows_per_mod;
   if (n_mod > 65535) return VOMNI_EBADSHAPE;
@@ -416,17 +792,10 @@ extern "C" int vomni_sandwich_norm_bwd(const void* grad_residual_out, const void
   p.out0 = static_cast<__nv_bfloat16*>(dx);
   p.out1 = static_cast<__nv_bfloat16*>(dresidual);
   p.parts = static_cast<float*>(workspace);
-  const Shape sh = shape_of(h);
-  const dim3 block(sh.tx, sh.ty);
-  const dim3 grid(bwd_blocks(rows_per_mod, n_mod, sh), static_cast<unsigned>(n_mod));
+  const Shape sh = shape_of(rows_per_mod, n_mod, h, 4, true);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (sh.tx == 32)
-    sandwich_bwd_kernel<128, true><<<grid, block, 0, st>>>(p);
-  else if (sh.tx <= 512)
-    sandwich_bwd_kernel<512, false><<<grid, block, 0, st>>>(p);
-  else
-    sandwich_bwd_kernel<1024, false><<<grid, block, 0, st>>>(p);
-  VOMNI_CUDA_TRY(cudaGetLastError());
+  rc = launch<true>(p, n_mod, sh, st);
+  if (rc) return rc;
   if (!dgate && !dpost_weight && !dmul && !dadd) return VOMNI_OK;
   SumParams s = {};
   s.parts = p.parts;
@@ -434,7 +803,7 @@ extern "C" int vomni_sandwich_norm_bwd(const void* grad_residual_out, const void
   s.post_w = post_weight;
   s.gate_step = p.gate_step;
   s.H = h;
-  s.lanes = static_cast<int>(grid.x) * sh.ty;
+  s.lanes = sh.lanes;
   s.n_mod = static_cast<int>(n_mod);
   s.per = per_mod;
   s.dgate = dgate;

@@ -62,8 +62,10 @@ def _vector(name: str, v: torch.Tensor | None, batch: int, hidden: int):
     return (v if v.data_ptr() % 16 == 0 else v.clone()), per
 
 
-def _plan(x, residual, vectors, post_norm, norm_type):
-    """Checked (batch, hidden, rows, rows_per_mod, per bits, fp32 vectors) of a call."""
+def _plan(x, residual, vectors, eps, post_norm, norm_type):
+    """Checked (hidden, rows, rows_per_mod, per bits, fp32 vectors) of a call."""
+    if not 0 < eps < float("inf"):
+        raise ValueError(f"eps must be positive and finite, got {eps}")
     if post_norm not in _NORMS:
         raise ValueError(f"unsupported post_norm {post_norm!r}")
     if norm_type not in _NORMS:
@@ -92,7 +94,7 @@ def _ptr(t):
 
 def _forward(x, residual, gate, mul, add, post_weight, eps, post_norm, norm_type):
     hidden, rows, per_mod, bits, v = _plan(
-        x, residual, {"gate": gate, "mul": mul, "add": add, "post_weight": post_weight}, post_norm, norm_type)
+        x, residual, {"gate": gate, "mul": mul, "add": add, "post_weight": post_weight}, eps, post_norm, norm_type)
     dev = _lib.one_device(x, residual, gate, mul, add, post_weight)
     x = None if x is None else _rows("x", x, residual.shape)
     residual = _rows("residual", residual, residual.shape)
@@ -110,7 +112,7 @@ def _forward(x, residual, gate, mul, add, post_weight, eps, post_norm, norm_type
 
 def _backward(grad_res, grad_out, x, residual_out, gate, mul, add, post_weight, eps, post_norm, norm_type, need):
     vectors = {"gate": gate, "mul": mul, "add": add, "post_weight": post_weight}
-    hidden, rows, per_mod, bits, v = _plan(x, residual_out, vectors, post_norm, norm_type)
+    hidden, rows, per_mod, bits, v = _plan(x, residual_out, vectors, eps, post_norm, norm_type)
     dev = _lib.one_device(grad_res, grad_out, x, residual_out, *vectors.values())
     shape = residual_out.shape
     grad_res = None if grad_res is None else _rows("grad_residual_out", grad_res, shape)
@@ -177,7 +179,7 @@ def sandwich_norm(
       is ``residual`` itself (``gate`` and ``post_weight`` must be None, ``post_norm`` is ignored).
     * ``gate`` / ``mul`` / ``add``: ``[B, 1, H]`` or ``[H]`` / ``[1, H]`` in fp32, bf16 or fp16, or None (1, 1, 0);
       ``post_weight``: ``[H]``. They are used in fp32.
-    * ``post_norm`` / ``norm_type``: ``"layer_norm"``, ``"rms_norm"`` or ``"none"``; ``eps`` is added to both variances.
+    * ``post_norm`` / ``norm_type``: ``"layer_norm"``, ``"rms_norm"`` or ``"none"``; ``eps > 0`` is added to both variances.
 
     Arithmetic is fp32; ``out`` comes from the unrounded residual, and each result is rounded to bf16 once. The backward pass
     reads ``x`` and ``residual_out`` and recomputes the statistics; it gives the same bits every time.
