@@ -10,6 +10,8 @@ import ctypes
 import threading
 from pathlib import Path
 
+import torch
+
 HERE = Path(__file__).resolve().parent
 LIB_PATH = HERE / "libvomni_b200.so"
 HEADER = HERE.parent / "include" / "vomni_b200.h"
@@ -156,15 +158,40 @@ def call(name: str, *args) -> None:
     check(getattr(load(), name)(*args), name)
 
 
-def one_device(*tensors):
-    """The CUDA device that all the given tensors (None entries aside) live on."""
-    devs = {t.device for t in tensors if t is not None}
-    for d in devs:
-        if d.type != "cuda":
-            raise RuntimeError(f"expected CUDA tensors (the B200 kernels have no CPU path), got one on {d}")
-    if len(devs) != 1:
-        raise ValueError(f"tensors are on different devices: {sorted(map(str, devs))}")
-    return devs.pop()
+def one_device(*tensors) -> int:
+    """Index of the CUDA device that all the given tensors (None entries aside) live on."""
+    index = None
+    for t in tensors:
+        if t is None:
+            continue
+        i = t.get_device()
+        if i < 0:
+            raise RuntimeError(f"expected CUDA tensors (the B200 kernels have no CPU path), got one on {t.device}")
+        if index is None:
+            index = i
+        elif i != index:
+            raise ValueError(f"tensors are on different devices: cuda:{index} and cuda:{i}")
+    return index
+
+
+def on_device(index: int, fn, *args):
+    """``fn(*args)`` with device ``index`` current."""
+    if torch.cuda.current_device() == index:
+        return fn(*args)
+    with torch.cuda.device(index):
+        return fn(*args)
+
+
+def launch(index: int, name: str, *args) -> None:
+    """Call a stream-ordered entry point on device ``index`` and its current stream (the entry's last argument)."""
+    check(on_device(index, getattr(load(), name), *args, torch._C._cuda_getCurrentRawStream(index)), name)
+
+
+def dense(t):
+    """``t``, or a contiguous 16-byte-aligned copy of it."""
+    if not t.is_contiguous():
+        t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 def device_status(clear: bool = True) -> int:

@@ -335,13 +335,14 @@ def attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, softmax_sca
     b, sq, skv, hq, hkv, q_lens, kv_lens = _check_training(q, k, v, q_lens, kv_lens)
     dev = _lib.one_device(q, k, v)
     scale = 1.0 / math.sqrt(_HEAD_DIM) if softmax_scale is None else float(softmax_scale)
+    device = q.device
     with torch.cuda.device(dev):
         if hkv != hq:
             k, v = (t.repeat_interleave(hq // hkv, dim=2) for t in (k, v))
         if q_lens is None and kv_lens is None and b * sq * hq and skv:
             return _cross_fwd(q, k, v, scale)
-        o = torch.zeros((b, hq, sq, _HEAD_DIM), dtype=torch.bfloat16, device=dev)
-        lse = torch.full((b, hq, 128, -(-sq // 128)), -math.inf, dtype=torch.float32, device=dev)
+        o = torch.zeros((b, hq, sq, _HEAD_DIM), dtype=torch.bfloat16, device=device)
+        lse = torch.full((b, hq, 128, -(-sq // 128)), -math.inf, dtype=torch.float32, device=device)
         for i in range(b):
             m, n = q_lens[i] if q_lens else sq, kv_lens[i] if kv_lens else skv
             if m and n and hq:
@@ -351,14 +352,17 @@ def attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, softmax_sca
         return o, lse
 
 
-def _any_strides(t: torch.Tensor) -> torch.Tensor:
-    """``t`` as it is where TMA can address its strides (d dense, the others positive multiples of 8), else a copy."""
-    ok = t.stride(3) == 1 and t.data_ptr() % 16 == 0
-    ok = ok and all(n == 1 or (st > 0 and st % 8 == 0) for n, st in zip(t.shape[:3], t.stride()[:3]))
-    if ok:
-        return t
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+def _any_strides(t: torch.Tensor, head_major: bool = False):
+    """(tensor, its token, head and batch strides): ``t`` as it is where TMA can address its strides (d dense, the others
+    positive multiples of 8), else a copy. ``head_major``: ``t`` is ``[b, heads, s, d]``."""
+    st, sh = t.stride(), t.shape
+    ok = st[3] == 1 and t.data_ptr() % 16 == 0
+    for i in range(3):
+        ok = ok and (sh[i] == 1 or (st[i] > 0 and st[i] % 8 == 0))
+    if not ok:
+        t = _lib.dense(t)
+        st = t.stride()
+    return t, ((st[2], st[1], st[0]) if head_major else (st[1], st[2], st[0]))
 
 
 def attention_bwd(grad_o: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, lse: torch.Tensor,
@@ -376,30 +380,27 @@ def attention_bwd(grad_o: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: tor
     for name, t in (("grad_o", grad_o), ("o", o)):
         if t.dtype != torch.bfloat16:
             raise TypeError(f"{name} must be bfloat16, got {t.dtype}")
-        if tuple(t.shape) != (b, hq, sq, _HEAD_DIM):
+        if t.shape != (b, hq, sq, _HEAD_DIM):
             raise ValueError(f"{name} must be [{b}, {hq}, {sq}, {_HEAD_DIM}], got {tuple(t.shape)}")
-    if not lse.is_floating_point() or tuple(lse.shape) != (b, hq, 128, -(-sq // 128)):
+    if not lse.is_floating_point() or lse.shape != (b, hq, 128, -(-sq // 128)):
         raise ValueError(f"lse must be [{b}, {hq}, 128, {-(-sq // 128)}], got {lse.dtype} {tuple(lse.shape)}")
     dev = _lib.one_device(grad_o, q, k, v, o, lse)
     scale = 1.0 / math.sqrt(_HEAD_DIM) if softmax_scale is None else float(softmax_scale)
     empty = not (b and sq and skv and hq)
     make = torch.zeros if empty else torch.empty
-    dq, dk, dv = (make(t.shape, dtype=torch.bfloat16, device=dev) for t in (q, k, v))
+    dq, dk, dv = (make(t.shape, dtype=torch.bfloat16, device=q.device) for t in (q, k, v))
     if empty:
         return dq, dk, dv
-    with torch.cuda.device(dev):
-        lib = _lib.load()
-        src = [_any_strides(t) for t in (q, k, v, grad_o.transpose(1, 2), o.transpose(1, 2))]
-        strides = (ctypes.c_longlong * 15)(*(t.stride(i) for t in src for i in (1, 2, 0)))
-        lse = lse.to(torch.float32).contiguous()
-        ints = lambda lens: (ctypes.c_int * b)(*lens) if lens is not None else None
-        ws_bytes = lib.vomni_attention_bwd_workspace_bytes(b, sq, skv, hq, hkv, _HEAD_DIM)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-        rc = lib.vomni_attention_bwd(
-            src[3].data_ptr(), src[0].data_ptr(), src[1].data_ptr(), src[2].data_ptr(), src[4].data_ptr(), lse.data_ptr(), b, sq,
-            skv, hq, hkv, _HEAD_DIM, strides, ints(q_lens), ints(kv_lens), scale, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-            ws.data_ptr(), ws_bytes, _stream_ptr(dev))
-        _lib.check(rc, "vomni_attention_bwd")
+    src = (_any_strides(q), _any_strides(k), _any_strides(v), _any_strides(grad_o, True), _any_strides(o, True))
+    strides = (ctypes.c_longlong * 15)(*(n for _, st in src for n in st))
+    q, k, v, grad_o, o = (t for t, _ in src)
+    lse = _lib.dense(lse if lse.dtype == torch.float32 else lse.float())
+    ints = lambda lens: (ctypes.c_int * b)(*lens) if lens is not None else None
+    ws_bytes = _lib.on_device(dev, _lib.load().vomni_attention_bwd_workspace_bytes, b, sq, skv, hq, hkv, _HEAD_DIM)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+    _lib.launch(dev, "vomni_attention_bwd", grad_o.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
+                lse.data_ptr(), b, sq, skv, hq, hkv, _HEAD_DIM, strides, ints(q_lens), ints(kv_lens), scale, dq.data_ptr(),
+                dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), ws_bytes)
     return dq, dk, dv
 
 

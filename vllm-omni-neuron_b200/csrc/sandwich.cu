@@ -31,7 +31,7 @@ namespace vomni {
 namespace sandwich {
 
 constexpr int kMaxH = 8192;  // 8 columns a thread, 1024 threads
-constexpr int kLayer = 0, kRms = 1, kNone = 2, kAsked = 3;
+constexpr int kLayer = 0, kNone = 2, kAsked = 3;  // 1: RMSNorm
 constexpr size_t kSmemPerSm = 200 * 1024;
 constexpr int kPerGate = 1, kPerMul = 2, kPerAdd = 4;
 

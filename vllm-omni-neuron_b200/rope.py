@@ -107,38 +107,33 @@ def _rotary_source(t: torch.Tensor):
     """(tensor, row stride, batch stride) as the kernel reads it: heads dense inside a token, strides of 16 bytes
     (column slices of a fused projection pass as they are); anything else is copied."""
     b, s, h, d = t.shape
-    esz = t.element_size()
-    row, batch = t.stride(1) if s > 1 else h * d, t.stride(0) if b > 1 else s * h * d
-    dense = (t.stride(3) == 1 or d == 1) and (h == 1 or t.stride(2) == d)
-    if dense and row >= h * d and batch >= 0 and (row * esz) % 16 == 0 and (batch * esz) % 16 == 0 and t.data_ptr() % 16 == 0:
+    sb, ss, sh, sd = t.stride()
+    row, batch = ss if s > 1 else h * d, sb if b > 1 else s * h * d
+    unit = 16 // t.element_size()
+    if (sd == 1 and (h == 1 or sh == d) and row >= h * d and batch >= 0 and row % unit == 0 and batch % unit == 0
+            and t.data_ptr() % 16 == 0):
         return t, row, batch
-    t = t.contiguous()
-    t = t if t.data_ptr() % 16 == 0 else t.clone()
-    return t, h * d, s * h * d
+    return _lib.dense(t), h * d, s * h * d
 
 
 def _rotary(q, k, positions, axes_dims, theta, pairing, inverse):
-    b, s, hq, d = q.shape
-    dev = q.device
-    with torch.cuda.device(dev):
-        outs, args, keep = [], [], []
-        for t in (q, k):
-            if t is None or t.numel() == 0:
-                outs.append(None if t is None else torch.empty(t.shape, dtype=t.dtype, device=dev))
-                args += [None, None, 0, 0, 0]
-                continue
-            src, row, batch = _rotary_source(t)
-            out = torch.empty(t.shape, dtype=t.dtype, device=dev)
-            keep.append(src)
-            outs.append(out)
-            args += [src.data_ptr(), out.data_ptr(), t.shape[2], row, batch]
-        if keep:
-            pos = positions.contiguous()
-            axes = (ctypes.c_int * len(axes_dims))(*axes_dims)
-            rc = _lib.load().vomni_rotary_axes(
-                *args, b, s, d, pos.data_ptr(), _POSITION_DTYPES[pos.dtype], int(pos.dim() == 3), len(axes_dims), axes,
-                float(theta), pairing, int(inverse), _ROTARY_DTYPES[q.dtype], torch.cuda.current_stream(dev).cuda_stream)
-            _lib.check(rc, "vomni_rotary_axes")
+    b, s, _, d = q.shape
+    outs, args, keep = [], [], []
+    for t in (q, k):
+        if t is None or t.numel() == 0:
+            outs.append(None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device))
+            args += (None, None, 0, 0, 0)
+            continue
+        src, row, batch = _rotary_source(t)
+        out = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+        keep.append(src)
+        outs.append(out)
+        args += (src.data_ptr(), out.data_ptr(), t.shape[2], row, batch)
+    if keep:
+        pos = positions if positions.is_contiguous() else positions.contiguous()
+        axes = (ctypes.c_int * len(axes_dims))(*axes_dims)
+        _lib.launch(q.get_device(), "vomni_rotary_axes", *args, b, s, d, pos.data_ptr(), _POSITION_DTYPES[pos.dtype],
+                    int(pos.dim() == 3), len(axes_dims), axes, theta, pairing, int(inverse), _ROTARY_DTYPES[q.dtype])
     return outs
 
 
@@ -203,10 +198,14 @@ def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor
         raise ValueError(f"axes_dims {axes_dims} must be 1 to 4 even counts that sum to the head dim {d}")
     if positions.dtype not in _POSITION_DTYPES:
         raise TypeError(f"positions must be int32, int64 or float32, got {positions.dtype}")
-    if tuple(positions.shape) not in ((s, len(axes_dims)), (b, s, len(axes_dims))):
+    if positions.shape != (s, len(axes_dims)) and positions.shape != (b, s, len(axes_dims)):
         raise ValueError(f"positions must be [{s}, {len(axes_dims)}] or [{b}, {s}, {len(axes_dims)}], got {tuple(positions.shape)}")
     if not (theta > 0 and theta < float("inf")):
         raise ValueError(f"theta must be positive and finite, got {theta}")
     _lib.one_device(q, k, positions)
-    out = _RotaryAxes.apply(q, k, positions, axes_dims, float(theta), _PAIRINGS[pairing], bool(inverse))
-    return out[0] if k is None else out
+    args = (q, k, positions, axes_dims, float(theta), _PAIRINGS[pairing], bool(inverse))
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        out = _RotaryAxes.apply(*args)
+    else:
+        out = _rotary(*args)
+    return out[0] if k is None else tuple(out)

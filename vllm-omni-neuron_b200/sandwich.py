@@ -40,10 +40,9 @@ class SandwichGrads(NamedTuple):
 def _rows(name: str, t: torch.Tensor, shape) -> torch.Tensor:
     if t.dtype != torch.bfloat16:
         raise TypeError(f"{name} must be bfloat16, got {t.dtype}")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name} shape {tuple(t.shape)} must be {tuple(shape)}")
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+    return _lib.dense(t)
 
 
 def _vector(name: str, v: torch.Tensor | None, batch: int, hidden: int):
@@ -52,14 +51,16 @@ def _vector(name: str, v: torch.Tensor | None, batch: int, hidden: int):
         return None, False
     if v.dtype not in (torch.float32, torch.bfloat16, torch.float16):
         raise TypeError(f"{name} must be float32, bfloat16 or float16, got {v.dtype}")
-    per = v.dim() == 3
-    if per and (name == "post_weight" or tuple(v.shape) != (batch, 1, hidden)):
-        raise ValueError(f"per-batch {name} must be [{batch}, 1, {hidden}], got {tuple(v.shape)}" if name != "post_weight"
-                         else f"post_weight must be [{hidden}], got {tuple(v.shape)}")
-    if not per and tuple(v.shape) not in ((hidden,), (1, hidden)):
-        raise ValueError(f"{name} must be [{batch}, 1, {hidden}], [{hidden}] or [1, {hidden}], got {tuple(v.shape)}")
-    v = v.to(torch.float32).contiguous()
-    return (v if v.data_ptr() % 16 == 0 else v.clone()), per
+    shape = v.shape
+    if len(shape) == 3 and name != "post_weight":
+        if shape != (batch, 1, hidden):
+            raise ValueError(f"per-batch {name} must be [{batch}, 1, {hidden}], got {tuple(shape)}")
+        per = True
+    elif shape != (hidden,) and shape != (1, hidden):
+        raise ValueError(f"{name} must be {'' if name == 'post_weight' else f'[{batch}, 1, {hidden}] or '}[{hidden}], got {tuple(shape)}")
+    else:
+        per = False
+    return _lib.dense(v if v.dtype == torch.float32 else v.float()), per
 
 
 def _plan(x, residual, vectors, eps, post_norm, norm_type):
@@ -101,12 +102,9 @@ def _forward(x, residual, gate, mul, add, post_weight, eps, post_norm, norm_type
     res_out = None if x is None else torch.empty_like(residual)
     out = torch.empty_like(residual)
     if rows:
-        with torch.cuda.device(dev):
-            rc = _lib.load().vomni_sandwich_norm(
-                _ptr(x), residual.data_ptr(), _ptr(v["gate"]), _ptr(v["post_weight"]), _ptr(v["mul"]), _ptr(v["add"]), rows,
-                hidden, per_mod, bits, float(eps), _NORMS[post_norm], _NORMS[norm_type], _ptr(res_out), out.data_ptr(),
-                torch.cuda.current_stream(dev).cuda_stream)
-        _lib.check(rc, "vomni_sandwich_norm")
+        _lib.launch(dev, "vomni_sandwich_norm", _ptr(x), residual.data_ptr(), _ptr(v["gate"]), _ptr(v["post_weight"]), _ptr(v["mul"]),
+                    _ptr(v["add"]), rows, hidden, per_mod, bits, eps, _NORMS[post_norm], _NORMS[norm_type], _ptr(res_out),
+                    out.data_ptr())
     return res_out, out
 
 
@@ -122,19 +120,15 @@ def _backward(grad_res, grad_out, x, residual_out, gate, mul, add, post_weight, 
     dx = None if x is None else torch.empty_like(x)
     dres = torch.empty_like(residual_out)
     make = torch.empty if rows else torch.zeros
-    sums = {n: make(t.shape, dtype=torch.float32, device=dev) if t is not None and need[n] else None for n, t in vectors.items()}
+    sums = {n: make(t.shape, dtype=torch.float32, device=residual_out.device) if t is not None and need[n] else None for n, t in vectors.items()}
     if rows:
-        lib = _lib.load()
-        with torch.cuda.device(dev):
-            ws_bytes = lib.vomni_sandwich_norm_workspace_bytes(rows, hidden, per_mod)
-            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-            rc = lib.vomni_sandwich_norm_bwd(
-                _ptr(grad_res), _ptr(grad_out), _ptr(x), residual_out.data_ptr(), _ptr(v["gate"]), _ptr(v["post_weight"]),
-                _ptr(v["mul"]), rows, hidden, per_mod, bits, float(eps), _NORMS[post_norm], _NORMS[norm_type], _ptr(dx),
-                dres.data_ptr(), _ptr(sums["gate"]), _ptr(sums["post_weight"]), _ptr(sums["mul"]), _ptr(sums["add"]),
-                ws.data_ptr(), ws_bytes, torch.cuda.current_stream(dev).cuda_stream)
-        _lib.check(rc, "vomni_sandwich_norm_bwd")
-    done = {n: None if t is None else t.to(vectors[n].dtype) for n, t in sums.items()}
+        ws_bytes = _lib.on_device(dev, _lib.load().vomni_sandwich_norm_workspace_bytes, rows, hidden, per_mod)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=residual_out.device)
+        _lib.launch(dev, "vomni_sandwich_norm_bwd", _ptr(grad_res), _ptr(grad_out), _ptr(x), residual_out.data_ptr(), _ptr(v["gate"]),
+                    _ptr(v["post_weight"]), _ptr(v["mul"]), rows, hidden, per_mod, bits, eps, _NORMS[post_norm], _NORMS[norm_type],
+                    _ptr(dx), dres.data_ptr(), _ptr(sums["gate"]), _ptr(sums["post_weight"]), _ptr(sums["mul"]), _ptr(sums["add"]),
+                    ws.data_ptr(), ws_bytes)
+    done = {n: t if t is None or vectors[n].dtype == torch.float32 else t.to(vectors[n].dtype) for n, t in sums.items()}
     return SandwichGrads(dx, dres, done["gate"], done["mul"], done["add"], done["post_weight"])
 
 
@@ -184,8 +178,11 @@ def sandwich_norm(
     Arithmetic is fp32; ``out`` comes from the unrounded residual, and each result is rounded to bf16 once. The backward pass
     reads ``x`` and ``residual_out`` and recomputes the statistics; it gives the same bits every time.
     """
-    res = _SandwichNorm.apply(x, residual, gate, mul, add, post_weight, float(eps), post_norm, norm_type)
-    return (residual, res) if x is None else res
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, gate, mul, add, post_weight)):
+        res = _SandwichNorm.apply(x, residual, gate, mul, add, post_weight, float(eps), post_norm, norm_type)
+        return (residual, res) if x is None else res
+    res_out, out = _forward(x, residual, gate, mul, add, post_weight, float(eps), post_norm, norm_type)
+    return (residual if x is None else res_out), out
 
 
 def sandwich_norm_bwd(
