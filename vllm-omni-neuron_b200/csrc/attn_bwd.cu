@@ -16,8 +16,12 @@
 // Both use tcgen05 cta_group::2 (M = 256, N = 128): each CTA stages half of every streamed operand, split by rows for
 // the S and dP products and by head dimension for the others, as a one-CTA M = 128 product would need 128 B of
 // shared-memory operands a clock and leave no room for the loads.
-// Warps: 0 TMA producer, 1 MMA issuer (the even CTA's), 2..9 exponentials and gradients of the scores: a thread owns
-// one TMEM lane (a key in dkdv, a query in dq), warpgroup wg the columns [64 wg, 64 wg + 64).
+// Warps: 0 TMA producer, 1 and 2 MMA issuers (the even CTA's), 4..19 exponentials and gradients of the scores: a thread
+// owns one TMEM lane (a key in dkdv, a query in dq), warpgroup wg the columns [32 wg, 32 wg + 32).
+// A wait costs an issuer some 170 to 300 clocks after its last MMA, and the tensor pipe queues about one, so each issuer
+// waits once a step: on one barrier that counts the score warps' arrivals and the bytes of every operand of that step.
+// The products that depend on different events are issued by different warps, so that one's wait is filled with the
+// other's products: issuer X the gradients and the scores that follow them in the same TMEM columns, issuer Y dP.
 // Matrix products per 128 x 128 scores of a CTA: 512 clocks each; exponentials: 1024 clocks of the MUFU unit.
 //
 // Rounding: P and dS are rounded to bf16 as tensor-core operands (2^-8 relative each, at most); everything else is fp32 until the
@@ -28,6 +32,7 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "common.cuh"
 #include "host_util.h"
@@ -37,29 +42,32 @@ namespace abwd {
 
 constexpr int kD = 128;
 constexpr int kTile = 128;              // columns of a step (queries in dkdv, keys in dq); rows of a CTA
-constexpr int kThreads = 64 + 256;
+constexpr int kGroups = 4;              // score warpgroups: each owns kCols columns of a step's scores
+constexpr int kCols = kTile / kGroups;  // 32: one TMEM load
+constexpr int kControl = 4;             // warps ahead of them: TMA producer, two MMA issuers, one idle
+constexpr int kThreads = 32 * kControl + 128 * kGroups;
 constexpr int kMaxSeqs = 16;            // batch elements of a launch with lengths of their own
 constexpr uint32_t kBox = 64 * 64 * 2;  // 8 KB: one TMA box, 64 rows x 64 dims, 128-byte swizzled
 constexpr uint32_t kTileBytes = 4 * kBox;  // resident operand: [2 dim halves][2 row halves] boxes
 constexpr uint32_t kHalfTile = 2 * kBox;   // a CTA's half of a streamed operand
-constexpr float kNoKeys = 1e30f;        // log2-sum-exp of a row without keys: its probabilities are 0
+constexpr float kNoKeys = 1e30f;        // -lse / scale of a row without keys (its sign that of -scale): no probabilities
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr uint32_t kScoreWarps = 16;    // score warps of both CTAs: arrivals per READY phase
+constexpr uint32_t kScoreWarps = 8 * kGroups;  // score warps of both CTAs: arrivals per READY phase
 
 // One set of maps for a batch of equal lengths (the batch element is a coordinate), or one per batch element
 // whose extents end at its lengths: rows behind them read as zero, whatever they hold.
 template <int N>
 struct Maps {
   CUtensorMap q[N], k[N], v[N], d_o[N];
+  CUtensorMap stats;  // Params::stats as [b * hq * rows][8]
 };
 
 struct Params {
   int b0;                     // first batch element of this launch
   int s_q, s_kv, hq, hkv, group;
   int q_len[kMaxSeqs], kv_len[kMaxSeqs];  // of each batch element (of the launch); [0] for all in a uniform one
-  int rows;                   // row pitch of lse2 / delta: s_q rounded up to whole tiles
-  const float* lse2;          // [b * hq, rows]: log2(e) * lse, kNoKeys behind the last query
-  const float* delta;         // [b * hq, rows], 0 behind the last query
+  int rows;                   // row pitch of stats: s_q rounded up to whole tiles
+  const uint4* stats;         // [b * hq, rows]: -lse / scale and -delta, three bf16 pieces each (stats_of)
   float scale, scale_log2;
   int splits, per_split;      // the walked tiles are dealt to splits of per_split tiles
   void* out0;                 // dq | dk: bf16 [b, s, heads, 128], or fp32 parts [split][b, s, heads, 128]
@@ -69,18 +77,19 @@ struct Params {
 };
 
 // P / dS in TMEM: the bf16 values of columns [16 kk, 16 kk + 16) sit in the 8 TMEM columns from pcol(kk). Each
-// warpgroup writes over the score columns that it has read itself (wg 0: columns 0-63, wg 1: 64-127).
-__host__ __device__ constexpr uint32_t pcol(int kk) { return kk * 8 + (kk >= 4 ? 32 : 0); }
+// warpgroup writes over score columns that it has read itself.
+__host__ __device__ constexpr uint32_t pcol(int kk) { return (kk >> 1) * kCols + (kk & 1) * 8; }
 
 constexpr uint32_t kIdescScores = idesc_bf16(256, 128, false);
 constexpr uint32_t kIdescGrad = idesc_bf16(256, 128, true);
 
-// scores[256 x 128] = A (resident, 128 rows in each CTA) B^T (streamed, 64 rows in each CTA), both K-major over d.
-VOMNI_DEV void issue_scores(uint32_t d, uint64_t a, uint64_t b) {
+// scores[256 x 128] = A (resident, 128 rows in each CTA) B^T (streamed, 64 rows in each CTA), both K-major over d; added to
+// what the columns hold where `add`.
+VOMNI_DEV void issue_scores(uint32_t d, uint64_t a, uint64_t b, bool add = false) {
 #pragma unroll
   for (int kk = 0; kk < 8; ++kk)
     mma_f16_ss_pair(d, a + (((kk >> 2) * 2 * kBox + (kk & 3) * 32) >> 4), b + (((kk >> 2) * kBox + (kk & 3) * 32) >> 4),
-                    kIdescScores, kk > 0);
+                    kIdescScores, (kk > 0 || add) ? 1u : 0u);
 }
 // grad[256 x 128] += W (TMEM, 128 columns) B (streamed: 128 rows, 64 dims in each CTA, MN-major).
 VOMNI_DEV void issue_grad(uint32_t d, uint32_t w, uint64_t b, bool accumulate) {
@@ -105,40 +114,39 @@ VOMNI_DEV void load_dims(const CUtensorMap* m, uint32_t bar, uint8_t* dst, int r
   tma_load_4d_pair(m, bar, dst + kBox, rank * 64, row + 64, h, b);
 }
 
-// This warp's columns are in TMEM (its stores completed): one arrival on the leader's barrier.
-VOMNI_DEV void publish(uint32_t bar_cluster) {
-  tmem_st_wait();
+// One arrival of this warp on the leader's barrier: its loads from TMEM have completed (signal), or its stores too (publish).
+VOMNI_DEV void signal(uint32_t bar_cluster) {
   tc_fence_before();
   __syncwarp();
   if ((threadIdx.x & 31) == 0) mbar_arrive_cluster(bar_cluster);
 }
+VOMNI_DEV void publish(uint32_t bar_cluster) {
+  tmem_st_wait();
+  signal(bar_cluster);
+}
 
-// 64 columns of one row of a gradient, times `scale`, to the output row (bf16, or fp32 parts). `computed`: the columns
+// kCols columns of one row of a gradient, times `scale`, to the output row (bf16, or fp32 parts). `computed`: the columns
 // hold sums (uniform over the CTA); rows that are not in the sequence (`in`) are written as zero, `ok`: in the tensor.
-VOMNI_DEV void store_half_row(uint32_t col, float scale, bool computed, bool in, bool ok, bool parts, void* out,
-                              long long at) {
-#pragma unroll 1
-  for (int ch = 0; ch < 2; ++ch) {
-    uint32_t o[32];
-    if (computed) {
-      tmem_ld32(col + ch * 32, o);
-      tmem_ld_wait(o);
-    }
-    if (!ok) continue;
-    float v[32];
+VOMNI_DEV void store_share(uint32_t col, float scale, bool computed, bool in, bool ok, bool parts, void* out, long long at) {
+  uint32_t o[kCols];
+  if (computed) {
+    tmem_ld32(col, o);
+    tmem_ld_wait(o);
+  }
+  if (!ok) return;
+  float v[kCols];
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = computed && in ? __uint_as_float(o[i]) * scale : 0.f;
-    if (parts) {
-      float4* dst = reinterpret_cast<float4*>(static_cast<float*>(out) + at + ch * 32);
+  for (int i = 0; i < kCols; ++i) v[i] = computed && in ? __uint_as_float(o[i]) * scale : 0.f;
+  if (parts) {
+    float4* dst = reinterpret_cast<float4*>(static_cast<float*>(out) + at);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) dst[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-    } else {
-      uint4* dst = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(out) + at + ch * 32);
+    for (int i = 0; i < kCols / 4; ++i) dst[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+  } else {
+    uint4* dst = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(out) + at);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        dst[i] = make_uint4(pack_bf16x2(v[8 * i], v[8 * i + 1]), pack_bf16x2(v[8 * i + 2], v[8 * i + 3]),
-                            pack_bf16x2(v[8 * i + 4], v[8 * i + 5]), pack_bf16x2(v[8 * i + 6], v[8 * i + 7]));
-    }
+    for (int i = 0; i < kCols / 8; ++i)
+      dst[i] = make_uint4(pack_bf16x2(v[8 * i], v[8 * i + 1]), pack_bf16x2(v[8 * i + 2], v[8 * i + 3]),
+                          pack_bf16x2(v[8 * i + 4], v[8 * i + 5]), pack_bf16x2(v[8 * i + 6], v[8 * i + 7]));
   }
 }
 
@@ -152,36 +160,92 @@ VOMNI_DEV void drain(uint64_t* bar, int uses, int* status, int code) {
 // Device status sites (VOMNI_DEV_TIMEOUT_BASE + site).
 enum Site : int { kSiteProducer = 0x40, kSiteMma = 0x41, kSiteScores = 0x42, kSiteOut = 0x43, kSiteDrain = 0x44 };
 
+// A float as the sum of three bf16 (8 bits each: 2^-24 relative), in the low halves of three words.
+VOMNI_DEV void pieces_of(float v, uint32_t (&w)[3]) {
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    const __nv_bfloat16 h = __float2bfloat16_rn(v);
+    w[i] = __bfloat16_as_ushort(h);
+    v -= __bfloat162float(h);
+  }
+}
+VOMNI_DEV uint4 stats_of(float neg_lse_over_scale, float neg_delta) {
+  uint32_t l[3], d[3];
+  pieces_of(neg_lse_over_scale, l);
+  pieces_of(neg_delta, d);
+  return make_uint4(l[0] | l[1] << 16, l[2] | d[0] << 16, d[1] | d[2] << 16, 0);
+}
+// Back to -log2(e) lse and -delta.
+VOMNI_DEV void sum_stats(const uint4& w, float scale_log2, float& nlse2, float& neg_delta) {
+  auto lo = [](uint32_t u) { return __uint_as_float(u << 16); };
+  auto hi = [](uint32_t u) { return __uint_as_float(u & 0xffff0000u); };
+  nlse2 = (lo(w.x) + hi(w.x) + lo(w.y)) * scale_log2;
+  neg_delta = hi(w.y) + lo(w.z) + hi(w.z);
+}
+
+// The shared prologue and epilogue of both kernels: barriers, TMEM, and their release.
+VOMNI_DEV uint32_t open_cta(uint64_t* bars, int n, int counted0, int counted1, uint32_t* tmem_slot, volatile int* abort_flag) {
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < n; ++i) mbar_init(&bars[i], i >= counted0 && i < counted1 ? kScoreWarps + 1 : 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (threadIdx.x >> 5 == 1) {
+    tmem_alloc_pair(tmem_slot, 512);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  cluster_sync();
+  tc_fence_after();
+  return *tmem_slot;
+}
+VOMNI_DEV void close_cta(uint32_t tbase) {
+  tc_fence_before();
+  cluster_sync();  // no CTA leaves while its pair may still touch its barriers or TMEM
+  if (threadIdx.x >> 5 == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tbase, 512);
+  }
+}
+
 // ================================================================ dK, dV
 namespace dkdv {
 // Streamed operands of a query tile, two slots each: Q and dO by rows (for S^T, dP^T), dO and Q by dims (for dV, dK).
 constexpr uint32_t kSmemK = 0, kSmemV = kTileBytes, kSmemStream = 2 * kTileBytes;
 constexpr int kSlots = 2, kLSlots = 4;
-constexpr uint32_t kSlotBytes = kHalfTile;  // 16 KB
-constexpr uint32_t smem_of(int kind, int slot) { return kSmemStream + (kind * kSlots + slot) * kSlotBytes; }
+constexpr uint32_t smem_of(int kind, int step) { return kSmemStream + (kind * kSlots + (step & 1)) * kHalfTile; }
 constexpr int kQr = 0, kOr = 1, kOd = 2, kQd = 3;
-constexpr uint32_t kSmemL = kSmemStream + 4 * kSlots * kSlotBytes;  // [kLSlots][lse2 128 | delta 128] fp32
-constexpr uint32_t kSmemBar = kSmemL + kLSlots * 1024;
+// A query's lse and delta belong to a column of the scores, so every thread would need them all: read from shared
+// memory they took 1024 of the step's wavefronts, which the products' operands need (3650 clocks a step instead of 2670
+// without them). They are added by the tensor cores instead, as one more step of 16 of each product: B holds the
+// columns' pieces (stats, 16 bytes a query), A ones where the pieces are (columns 0-2 for S, 3-5 for dP) and zeros
+// elsewhere. Unswizzled core matrices of 8 rows x 16 bytes; B's second half of the 16 is its first again, times zeros.
+constexpr uint32_t kAuxBytes = 64 * 16, kOnesBytes = 128 * 32;
+constexpr uint32_t kSmemAux = kSmemStream + 4 * kSlots * kHalfTile;  // [kLSlots] stats of this CTA's 64 queries of a step
+constexpr uint32_t kSmemOnes = kSmemAux + kLSlots * kAuxBytes;       // A for S, A for dP
+constexpr uint32_t kSmemBar = kSmemOnes + 2 * kOnesBytes;
 constexpr uint32_t kSmemBytes = kSmemBar + 256 + 1024;
-// TMEM columns: S^T / P^T, dP^T / dS^T, dV, dK.
-constexpr uint32_t kColS = 0, kColDp = 128, kColDv = 256, kColDk = 384;
+// TMEM columns: two score regions, dV, dK. Step j works in region j % 2, which holds S^T, then (once the score warps have
+// read it) dP^T, then P^T and dS^T side by side, so that S^T of the next step is formed in the other one meanwhile.
+constexpr uint32_t kColR = 0, kColDv = 256, kColDk = 384;
+constexpr uint32_t kDs = kCols / 2;  // dS^T beside P^T: the second half of each warpgroup's columns
 
-// Slot-indexed barriers complete once every kSlots steps. S_FULL + s and DP_FULL + s also tell the producers which
-// slots are free: MMAs complete in issue order, so S of step j + 1 complete means dV of step j complete, and dP of
-// step j + 1 means dK of step j. Each is waited for before the load that its next phase depends on, so no
-// wait can miss a phase.
+// Two barriers of a kind serve steps in turn; each is waited for before anything that its next phase depends on, so no
+// wait can miss a phase. X issues dV(j), dK(j), S(j+2) in this order and MMAs of one thread complete in order, so S
+// of step j complete frees the slots of dV(j-2) and dK(j-2) too.
 enum Bar : int {
-  KV_FULL = 0,
-  FULL = 1,                        // + kind * kSlots + slot
-  L_FULL = FULL + 4 * kSlots,      // + step % kLSlots, this CTA's own
-  S_FULL = L_FULL + kLSlots,       // + step % 2
-  DP_FULL = S_FULL + 2,            // + step % 2
-  P_READY = DP_FULL + 2,
-  DS_READY = P_READY + 1,
-  OUT_FULL = DS_READY + 1,
+  START = 0,             // K and the first two tiles' Q rows and stats
+  S_FULL = 1,            // + step % 2, as all below
+  DP_FULL = S_FULL + 2,
+  S_READ = DP_FULL + 2,  // Y's: the score warps hold S of step j; dO's rows of j (and V, for the first) are there
+  PD_READY = S_READ + 2, // X's: P and dS of step j; dO's and Q's dims of j and Q's rows and stats of j + 2 are there
+  OUT_FULL = PD_READY + 2,
   NBAR = OUT_FULL + 1
 };
 static_assert(NBAR * 8 + 8 <= 256, "barriers, TMEM slot and abort flag fit their area");
+
+VOMNI_DEV uint64_t desc_aux(const void* p) { return make_sdesc(smem_u32(p), 0, 128, 0); }
+VOMNI_DEV uint64_t desc_ones(const void* p) { return make_sdesc(smem_u32(p), 128, 256, 0); }
 
 template <int N>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
@@ -189,7 +253,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kSmemBar);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + kSmemBar + NBAR * 8);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + kSmemBar + NBAR * 8 + 4);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
@@ -206,208 +269,189 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const int last = min(first + p.per_split, q_tiles * p.group);
   const int steps = pair_row < kv_len ? max(last - first, 0) : 0;
 
-  if (steps > 0) {
-    if (threadIdx.x == 0) {
-      for (int i = 0; i < NBAR; ++i) mbar_init(&bars[i], i == P_READY || i == DS_READY ? kScoreWarps : 1);
-      *abort_flag = 0;
-      fence_mbar_init();
-    }
-    if (warp == 1) {
-      tmem_alloc_pair(tmem_slot, 512);
-      tmem_relinquish_pair();
-    }
-    tc_fence_before();
-    cluster_sync();
-    tc_fence_after();
+  if (steps > 0 && threadIdx.x < 256) {  // row threadIdx.x % 128 of one of the two A tiles of ones
+    const int r = threadIdx.x & 127, which = threadIdx.x >> 7;
+    uint4* row = reinterpret_cast<uint4*>(smem + kSmemOnes + which * kOnesBytes + (r >> 3) * 256 + (r & 7) * 16);
+    constexpr uint32_t one = 0x3F80u;  // bf16 1
+    row[0] = which ? make_uint4(0, one << 16, one | one << 16, 0) : make_uint4(one | one << 16, one, 0, 0);
+    row[8] = make_uint4(0, 0, 0, 0);
+    fence_proxy_async_smem();
   }
-  const uint32_t tbase = steps > 0 ? *tmem_slot : 0;
+  uint32_t tbase = 0;
+  if (steps > 0)
+    tbase = open_cta(bars, NBAR, S_READ, OUT_FULL, reinterpret_cast<uint32_t*>(smem + kSmemBar + NBAR * 8), abort_flag);
   const uint32_t lead_bars = mapa_shared(smem_u32(bars), 0);
+  auto wait = [&](int bar, uint32_t use, int site) {  // for phase `use` of a barrier
+    return mbar_wait_spin(&bars[bar], use & 1, abort_flag, p.status, VOMNI_DEV_TIMEOUT_BASE + site);
+  };
   bool out_ok = steps == 0;
 
   if (steps > 0 && warp == 0) {
     if (lane == 0) {
-      const uint32_t kv_bar = lead_bars + KV_FULL * 8;
-      if (leader) mbar_expect_tx(&bars[KV_FULL], 4 * kTileBytes);
-      load_resident(&maps.k[mi], kv_bar, smem + kSmemK, row0, hk, bz);
-      load_resident(&maps.v[mi], kv_bar, smem + kSmemV, row0, hk, bz);
-      int issued[4] = {};  // loads of each kind
-      bool ok = true;
-      for (int j = 0; j < steps && ok; ++j) {
-        const int s = j & 1, t = first + j;
-        const int h = hk * p.group + t / q_tiles, row = (t % q_tiles) * kTile;
-        const uint32_t full = lead_bars + (FULL + s) * 8;
-        auto arm = [&](int kind) {
-          if (leader) mbar_expect_tx(&bars[FULL + kind * kSlots + s], 2 * kSlotBytes);
-          ++issued[kind];
-          return full + kind * kSlots * 8;
-        };
-        auto wait = [&](int bar, int step) {
-          return mbar_wait_spin(&bars[bar + (step & 1)], (step >> 1) & 1, abort_flag, p.status,
-                                VOMNI_DEV_TIMEOUT_BASE + kSiteProducer);
-        };
-        // lse2 and delta of the step (slot's last reader: step j - 4, long done once dP of step j - 2 is)
-        if (j >= kSlots && !(ok = wait(S_FULL, j - 2))) break;
-        uint32_t bar = arm(kQr);
-        load_rows(&maps.q[mi], bar, smem + smem_of(kQr, s), row, h, bz, rank);
-        if (j >= kSlots && !(ok = wait(DP_FULL, j - 2))) break;
-        bar = arm(kOr);
-        load_rows(&maps.d_o[mi], bar, smem + smem_of(kOr, s), row, h, bz, rank);
-        const int l = j % kLSlots;
-        const long long at = (static_cast<long long>(b) * p.hq + h) * p.rows + row;
-        mbar_expect_tx(&bars[L_FULL + l], 1024);
-        bulk_g2s(smem + kSmemL + l * 1024, p.lse2 + at, 512, &bars[L_FULL + l]);
-        bulk_g2s(smem + kSmemL + l * 1024 + 512, p.delta + at, 512, &bars[L_FULL + l]);
-        if (j >= kSlots && !(ok = wait(S_FULL, j - 1))) break;
-        bar = arm(kOd);
-        load_dims(&maps.d_o[mi], bar, smem + smem_of(kOd, s), row, h, bz, rank);
-        if (j >= kSlots && !(ok = wait(DP_FULL, j - 1))) break;
-        bar = arm(kQd);
-        load_dims(&maps.q[mi], bar, smem + smem_of(kQd, s), row, h, bz, rank);
+      auto arm = [&](int bar, uint32_t bytes) {  // the bytes of both CTAs' loads, on the leader's barrier
+        if (leader) mbar_expect_tx(&bars[bar], 2 * bytes);
+        return lead_bars + bar * 8;
+      };
+      auto place = [&](int j, int& h, int& row) {
+        h = hk * p.group + (first + j) / q_tiles;
+        row = (first + j) % q_tiles * kTile;
+      };
+      int h, row;
+      auto stats = [&](int j, uint32_t bar) {  // of this CTA's half of a tile's queries
+        tma_load_2d_pair(&maps.stats, bar, smem + kSmemAux + (j % kLSlots) * kAuxBytes, 0,
+                         (b * p.hq + h) * p.rows + row + static_cast<int>(rank) * 64);
+      };
+      const int ahead = min(steps, 2);
+      uint32_t bar = arm(START, kTileBytes + ahead * (kHalfTile + kAuxBytes));
+      load_resident(&maps.k[mi], bar, smem + kSmemK, row0, hk, bz);
+      for (int j = 0; j < ahead; ++j) {
+        place(j, h, row);
+        load_rows(&maps.q[mi], bar, smem + smem_of(kQr, j), row, h, bz, rank);
+        stats(j, bar);
       }
-      if (*abort_flag) {
+      bar = arm(S_READ, kTileBytes + kHalfTile);
+      load_resident(&maps.v[mi], bar, smem + kSmemV, row0, hk, bz);
+      for (int j = 0; j < ahead; ++j) {
+        if (j > 0) bar = arm(S_READ + j, kHalfTile);
+        place(j, h, row);
+        load_rows(&maps.d_o[mi], bar, smem + smem_of(kOr, j), row, h, bz, rank);
+      }
+      int pd = 0, sr = ahead;  // steps whose loads on PD_READY / S_READ were issued
+      for (int j = 0; j < steps; ++j) {
+        if (!wait(S_FULL + (j & 1), j >> 1, kSiteProducer)) break;
+        const bool more = j + 2 < steps;
+        bar = arm(PD_READY + (j & 1), more ? 3 * kHalfTile + kAuxBytes : 2 * kHalfTile);
+        ++pd;
+        place(j, h, row);
+        load_dims(&maps.d_o[mi], bar, smem + smem_of(kOd, j), row, h, bz, rank);
+        load_dims(&maps.q[mi], bar, smem + smem_of(kQd, j), row, h, bz, rank);
+        if (!more) continue;
+        place(j + 2, h, row);
+        stats(j + 2, bar);  // the slot's last readers, S and dP of step j - 2, are done: S(j) follows that step's gradients
+        load_rows(&maps.q[mi], bar, smem + smem_of(kQr, j), row, h, bz, rank);
+        if (!wait(DP_FULL + (j & 1), j >> 1, kSiteProducer)) break;
+        bar = arm(S_READ + (j & 1), kHalfTile);
+        ++sr;
+        load_rows(&maps.d_o[mi], bar, smem + smem_of(kOr, j), row, h, bz, rank);
+      }
+      if (*abort_flag) {  // copies in flight: the last use of every barrier that counts bytes
         if (leader) {
-          drain(&bars[KV_FULL], 1, p.status, VOMNI_DEV_TIMEOUT_BASE + kSiteDrain);
-          for (int kind = 0; kind < 4; ++kind)
-            for (int s = 0; s < kSlots; ++s)
-              drain(&bars[FULL + kind * kSlots + s], (issued[kind] + kSlots - 1 - s) / kSlots, p.status,
-                    VOMNI_DEV_TIMEOUT_BASE + kSiteDrain);
+          drain(&bars[START], 1, p.status, VOMNI_DEV_TIMEOUT_BASE + kSiteDrain);
+          for (int s = 0; s < 2; ++s) {
+            drain(&bars[PD_READY + s], (pd + 1 - s) / 2, p.status, VOMNI_DEV_TIMEOUT_BASE + kSiteDrain);
+            drain(&bars[S_READ + s], (sr + 1 - s) / 2, p.status, VOMNI_DEV_TIMEOUT_BASE + kSiteDrain);
+          }
         }
-        for (int l = 0; l < kLSlots; ++l)
-          drain(&bars[L_FULL + l], (issued[kOr] + kLSlots - 1 - l) / kLSlots, p.status,
-                VOMNI_DEV_TIMEOUT_BASE + kSiteDrain);
       }
     }
   } else if (steps > 0 && warp == 1) {
-    // Order per step j: dV(j), S(j+1) over P(j), dK(j), dP(j+1) over dS(j): while one of P and dS is formed, the
-    // tensor pipe works on the other.
-    if (leader && lane == 0) {
-      const uint64_t dk_a = desc_k(smem + kSmemK), dv_a = desc_k(smem + kSmemV);
-      auto wait = [&](int bar, uint32_t parity) {
-        return mbar_wait_spin(&bars[bar], parity, abort_flag, p.status, VOMNI_DEV_TIMEOUT_BASE + kSiteMma);
-      };
-      auto full = [&](int kind, int j) { return wait(FULL + kind * kSlots + (j & 1), (j >> 1) & 1); };
+    if (leader && lane == 0) {  // X
+      const uint64_t a = desc_k(smem + kSmemK), ones = desc_ones(smem + kSmemOnes);
       auto scores = [&](int j) {
-        if (!full(kQr, j)) return false;
-        tc_fence_after();
-        issue_scores(tbase + kColS, dk_a, desc_k(smem + smem_of(kQr, j & 1)));
+        const uint32_t region = tbase + kColR + (j & 1) * 128;
+        mma_f16_ss_pair(region, ones, desc_aux(smem + kSmemAux + (j % kLSlots) * kAuxBytes), kIdescScores, 0);
+        issue_scores(region, a, desc_k(smem + smem_of(kQr, j)), true);
         tc_commit_pair(&bars[S_FULL + (j & 1)]);
-        return true;
       };
-      auto dprobs = [&](int j) {
-        if (!full(kOr, j)) return false;
+      bool ok = wait(START, 0, kSiteMma);
+      if (ok) {
         tc_fence_after();
-        issue_scores(tbase + kColDp, dv_a, desc_k(smem + smem_of(kOr, j & 1)));
-        tc_commit_pair(&bars[DP_FULL + (j & 1)]);
-        return true;
-      };
-      bool ok = wait(KV_FULL, 0) && scores(0) && dprobs(0);
+        scores(0);
+        if (steps > 1) scores(1);
+      }
       for (int j = 0; ok && j < steps; ++j) {
-        if (!(ok = wait(P_READY, j & 1) && full(kOd, j))) break;
+        if (!(ok = wait(PD_READY + (j & 1), j >> 1, kSiteMma))) break;
         tc_fence_after();
-        issue_grad(tbase + kColDv, tbase + kColS, desc_mn(smem + smem_of(kOd, j & 1)), j > 0);
-        if (j + 1 < steps && !(ok = scores(j + 1))) break;
-        if (!(ok = wait(DS_READY, j & 1) && full(kQd, j))) break;
-        tc_fence_after();
-        issue_grad(tbase + kColDk, tbase + kColDp, desc_mn(smem + smem_of(kQd, j & 1)), j > 0);
-        if (j + 1 < steps && !(ok = dprobs(j + 1))) break;
+        const uint32_t region = tbase + kColR + (j & 1) * 128;
+        issue_grad(tbase + kColDv, region, desc_mn(smem + smem_of(kOd, j)), j > 0);
+        issue_grad(tbase + kColDk, region + kDs, desc_mn(smem + smem_of(kQd, j)), j > 0);
+        if (j + 2 < steps) scores(j + 2);
       }
       tc_commit_pair(&bars[OUT_FULL]);
     }
-  } else if (steps > 0) {
-    const int wg = (warp - 2) >> 2, quad = warp & 3;
-    const uint32_t lane_addr = static_cast<uint32_t>(quad * 32) << 16;
-    const uint32_t col_s = tbase + lane_addr + kColS, col_dp = tbase + lane_addr + kColDp;
+  } else if (steps > 0 && warp == 2) {
+    if (leader && lane == 0) {  // Y
+      const uint64_t a = desc_k(smem + kSmemV), ones = desc_ones(smem + kSmemOnes + kOnesBytes);
+      for (int j = 0; j < steps; ++j) {
+        if (!wait(S_READ + (j & 1), j >> 1, kSiteMma)) break;
+        tc_fence_after();
+        const uint32_t region = tbase + kColR + (j & 1) * 128;
+        mma_f16_ss_pair(region, ones, desc_aux(smem + kSmemAux + (j % kLSlots) * kAuxBytes), kIdescScores, 0);
+        issue_scores(region, a, desc_k(smem + smem_of(kOr, j)), true);
+        tc_commit_pair(&bars[DP_FULL + (j & 1)]);
+      }
+    }
+  } else if (steps > 0 && warp >= kControl) {
+    const int wg = (warp - kControl) >> 2, quad = warp & 3;
+    const uint32_t lane_col = tbase + (static_cast<uint32_t>(quad * 32) << 16) + kColR + kCols * wg;  // this warp's columns
     const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2);
-    auto wait = [&](int bar, uint32_t parity) {
-      return mbar_wait_spin(&bars[bar], parity, abort_flag, p.status, VOMNI_DEV_TIMEOUT_BASE + kSiteScores);
-    };
     bool ok = true;
     for (int j = 0; j < steps && ok; ++j) {
-      const float* lse2 = reinterpret_cast<const float*>(smem + kSmemL + (j % kLSlots) * 1024) + 64 * wg;
-      const float* delta = lse2 + 128;
-      if (!(ok = wait(L_FULL + j % kLSlots, (j / kLSlots) & 1) && wait(S_FULL + (j & 1), (j >> 1) & 1))) break;
+      const uint32_t col = lane_col + (j & 1) * 128;
+      if (!(ok = wait(S_FULL + (j & 1), j >> 1, kSiteScores))) break;
       tc_fence_after();
-      float pr[64];
+      float pr[kCols];
+      uint32_t s[kCols], pk[kCols / 2];
+      tmem_ld32(col, s);
+      tmem_ld_wait(s);
+      signal(lead_bars + (S_READ + (j & 1)) * 8);
 #pragma unroll
-      for (int ch = 0; ch < 2; ++ch) {
-        uint32_t s[32], pk[16];
-        tmem_ld32(col_s + 64 * wg + 32 * ch, s);
-        tmem_ld_wait(s);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float2 l = *reinterpret_cast<const float2*>(lse2 + 32 * ch + 2 * i);
-          float x0, x1;
-          f2_unpack(f2_fma(f2_pack(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), scale2, f2_pack(-l.x, -l.y)),
-                    x0, x1);
-          pr[32 * ch + 2 * i] = ex2_approx(x0);
-          pr[32 * ch + 2 * i + 1] = ex2_approx(x1);
-          pk[i] = pack_bf16x2(pr[32 * ch + 2 * i], pr[32 * ch + 2 * i + 1]);
-        }
-        tmem_st16(col_s + pcol(4 * wg + 2 * ch), pk);
+      for (int i = 0; i < kCols; i += 2) {
+        float x0, x1;
+        f2_unpack(f2_mul(f2_pack(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), scale2), x0, x1);
+        pr[i] = ex2_approx(x0);
+        pr[i + 1] = ex2_approx(x1);
       }
-      publish(lead_bars + P_READY * 8);
-      if (!(ok = wait(DP_FULL + (j & 1), (j >> 1) & 1))) break;
+      if (!(ok = wait(DP_FULL + (j & 1), j >> 1, kSiteScores))) break;
       tc_fence_after();
+      tmem_ld32(col, s);
+      tmem_ld_wait(s);
 #pragma unroll
-      for (int ch = 0; ch < 2; ++ch) {
-        uint32_t s[32], pk[16];
-        tmem_ld32(col_dp + 64 * wg + 32 * ch, s);
-        tmem_ld_wait(s);
+      for (int i = 0; i < kCols / 2; ++i) pk[i] = pack_bf16x2(pr[2 * i], pr[2 * i + 1]);
+      tmem_st16(col, pk);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float2 d = *reinterpret_cast<const float2*>(delta + 32 * ch + 2 * i);
-          const int c = 32 * ch + 2 * i;
-          pk[i] = pack_bf16x2(pr[c] * (__uint_as_float(s[2 * i]) - d.x), pr[c + 1] * (__uint_as_float(s[2 * i + 1]) - d.y));
-        }
-        tmem_st16(col_dp + pcol(4 * wg + 2 * ch), pk);
-      }
-      publish(lead_bars + DS_READY * 8);
+      for (int i = 0; i < kCols; i += 2)
+        pk[i / 2] = pack_bf16x2(pr[i] * __uint_as_float(s[i]), pr[i + 1] * __uint_as_float(s[i + 1]));
+      tmem_st16(col + kDs, pk);
+      publish(lead_bars + (PD_READY + (j & 1)) * 8);
     }
-    out_ok = ok && mbar_wait_spin(&bars[OUT_FULL], 0, abort_flag, p.status, VOMNI_DEV_TIMEOUT_BASE + kSiteOut);
+    out_ok = ok && wait(OUT_FULL, 0, kSiteOut);
     tc_fence_after();
   }
 
-  if (warp >= 2 && out_ok) {
-    const int wg = (warp - 2) >> 2, quad = warp & 3;
-    const uint32_t lane_addr = static_cast<uint32_t>(quad * 32) << 16;
+  if (warp >= kControl && out_ok) {
+    const int wg = (warp - kControl) >> 2, quad = warp & 3;
+    const uint32_t col = tbase + (static_cast<uint32_t>(quad * 32) << 16) + kCols * wg;
     const int row = row0 + quad * 32 + lane;
     const bool parts = p.splits > 1;
     const long long at = (parts ? split * p.part : 0) +
-                         ((static_cast<long long>(b) * p.s_kv + row) * p.hkv + hk) * kD + 64 * wg;
-    store_half_row(tbase + lane_addr + kColDv + 64 * wg, 1.f, steps > 0, row < kv_len, row < p.s_kv, parts, p.out1, at);
-    store_half_row(tbase + lane_addr + kColDk + 64 * wg, p.scale, steps > 0, row < kv_len, row < p.s_kv, parts, p.out0, at);
+                         ((static_cast<long long>(b) * p.s_kv + row) * p.hkv + hk) * kD + kCols * wg;
+    store_share(col + kColDv, 1.f, steps > 0, row < kv_len, row < p.s_kv, parts, p.out1, at);
+    store_share(col + kColDk, p.scale, steps > 0, row < kv_len, row < p.s_kv, parts, p.out0, at);
   }
-  if (steps > 0) {
-    tc_fence_before();
-    cluster_sync();
-    if (warp == 1) {
-      tc_fence_after();
-      tmem_dealloc_pair(tbase, 512);
-    }
-  }
+  if (steps > 0) close_cta(tbase);
 }
 }  // namespace dkdv
 
 // ================================================================ dQ
 namespace dq {
-// A stage: K and V by rows (S, dP) and K by dims (dQ).
-constexpr int kStages = 3;
-constexpr uint32_t kStageBytes = 3 * kHalfTile;
-constexpr uint32_t kSmemQ = 0, kSmemO = kTileBytes, kSmemStage = 2 * kTileBytes;
-constexpr uint32_t kSmemBar = kSmemStage + kStages * kStageBytes;
+// Streamed operands of a key tile: K by rows (S), V by rows (dP), K by dims (dQ).
+constexpr int kRegions = 3;  // score regions, and slots of K by rows and by dims
+constexpr uint32_t kSmemQ = 0, kSmemO = kTileBytes, kSmemKr = 2 * kTileBytes;
+constexpr uint32_t kSmemVr = kSmemKr + kRegions * kHalfTile, kSmemKd = kSmemVr + 2 * kHalfTile;
+constexpr uint32_t kSmemBar = kSmemKd + kRegions * kHalfTile;
 constexpr uint32_t kSmemBytes = kSmemBar + 256 + 1024;
-constexpr uint32_t kKr = 0, kVr = kHalfTile, kKd = 2 * kHalfTile;
-// TMEM columns: S of even and odd steps, dP / dS, dQ.
-constexpr uint32_t kColS = 0, kColDp = 256, kColDq = 384;
+// TMEM columns: three regions, each of a step's S, then dP, then dS; dQ.
+constexpr uint32_t kColR = 0, kColDq = kRegions * 128;
 
+// As in dkdv: X issues dQ(j), S(j+3), so S of step j complete frees the slots of dQ(j-3); Y issues dP(j).
 enum Bar : int {
-  Q_FULL = 0,
-  FULL = 1,
-  EMPTY = FULL + kStages,
-  S_FULL = EMPTY + kStages,  // + step % 2
-  DP_FULL = S_FULL + 2,
-  DS_READY = DP_FULL + 1,
-  OUT_FULL = DS_READY + 1,
+  START = 0,                    // Q and the first three tiles' K rows
+  S_FULL = 1,                   // + step % 3
+  DP_FULL = S_FULL + kRegions,  // + step % 2
+  S_READ = DP_FULL + 2,         // Y's, + step % 2: S of step j is read; V's rows of j (and dO, for the first) are there
+  DS_READY = S_READ + 2,        // X's, + step % 3: dS of step j; K's dims of j and K's rows of j + 3 are there
+  OUT_FULL = DS_READY + kRegions,
   NBAR = OUT_FULL + 1
 };
 static_assert(NBAR * 8 + 8 <= 256, "barriers, TMEM slot and abort flag fit their area");
@@ -418,7 +462,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kSmemBar);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + kSmemBar + NBAR * 8);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + kSmemBar + NBAR * 8 + 4);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
@@ -433,159 +476,153 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const int last = min(first + p.per_split, (kv_len + kTile - 1) / kTile);
   const int steps = pair_row < q_len ? max(last - first, 0) : 0;
 
-  if (steps > 0) {
-    if (threadIdx.x == 0) {
-      for (int i = 0; i < NBAR; ++i) mbar_init(&bars[i], i == DS_READY ? kScoreWarps : 1);
-      *abort_flag = 0;
-      fence_mbar_init();
-    }
-    if (warp == 1) {
-      tmem_alloc_pair(tmem_slot, 512);
-      tmem_relinquish_pair();
-    }
-    tc_fence_before();
-    cluster_sync();
-    tc_fence_after();
-  }
-  const uint32_t tbase = steps > 0 ? *tmem_slot : 0;
+  uint32_t tbase = 0;
+  if (steps > 0)
+    tbase = open_cta(bars, NBAR, S_READ, OUT_FULL, reinterpret_cast<uint32_t*>(smem + kSmemBar + NBAR * 8), abort_flag);
   const uint32_t lead_bars = mapa_shared(smem_u32(bars), 0);
+  auto wait = [&](int bar, uint32_t use, int site) {
+    return mbar_wait_spin(&bars[bar], use & 1, abort_flag, p.status, VOMNI_DEV_TIMEOUT_BASE + site);
+  };
   bool out_ok = steps == 0;
 
   if (steps > 0 && warp == 0) {
     if (lane == 0) {
-      const uint32_t q_bar = lead_bars + Q_FULL * 8;
-      if (leader) mbar_expect_tx(&bars[Q_FULL], 4 * kTileBytes);
-      load_resident(&maps.q[mi], q_bar, smem + kSmemQ, row0, h, bz);
-      load_resident(&maps.d_o[mi], q_bar, smem + kSmemO, row0, h, bz);
-      int done = 0;
-      for (int j = 0; j < steps; ++j, ++done) {
-        const int st = j % kStages, use = j / kStages;
-        if (use > 0 && !mbar_wait_spin(&bars[EMPTY + st], (use - 1) & 1, abort_flag, p.status,
-                                       VOMNI_DEV_TIMEOUT_BASE + kSiteProducer))
-          break;
-        const uint32_t bar = lead_bars + (FULL + st) * 8;
-        uint8_t* dst = smem + kSmemStage + st * kStageBytes;
-        const int row = (first + j) * kTile;
-        if (leader) mbar_expect_tx(&bars[FULL + st], 2 * kStageBytes);
-        load_rows(&maps.k[mi], bar, dst + kKr, row, hk, bz, rank);
-        load_rows(&maps.v[mi], bar, dst + kVr, row, hk, bz, rank);
-        load_dims(&maps.k[mi], bar, dst + kKd, row, hk, bz, rank);
+      auto arm = [&](int bar, uint32_t bytes) {
+        if (leader) mbar_expect_tx(&bars[bar], 2 * bytes);
+        return lead_bars + bar * 8;
+      };
+      const int ahead = min(steps, kRegions), v_ahead = min(steps, 2);
+      uint32_t bar = arm(START, kTileBytes + ahead * kHalfTile);
+      load_resident(&maps.q[mi], bar, smem + kSmemQ, row0, h, bz);
+      for (int j = 0; j < ahead; ++j)
+        load_rows(&maps.k[mi], bar, smem + kSmemKr + j * kHalfTile, (first + j) * kTile, hk, bz, rank);
+      bar = arm(S_READ, kTileBytes + kHalfTile);
+      load_resident(&maps.d_o[mi], bar, smem + kSmemO, row0, h, bz);
+      for (int j = 0; j < v_ahead; ++j) {
+        if (j > 0) bar = arm(S_READ + j, kHalfTile);
+        load_rows(&maps.v[mi], bar, smem + kSmemVr + j * kHalfTile, (first + j) * kTile, hk, bz, rank);
+      }
+      int ds = 0, sr = v_ahead;  // steps whose loads on DS_READY / S_READ were issued
+      for (int j = 0; j < steps; ++j) {
+        const int r = j % kRegions;
+        if (!wait(S_FULL + r, j / kRegions, kSiteProducer)) break;
+        const bool more = j + kRegions < steps;
+        bar = arm(DS_READY + r, (more ? 2 : 1) * kHalfTile);
+        ++ds;
+        load_dims(&maps.k[mi], bar, smem + kSmemKd + r * kHalfTile, (first + j) * kTile, hk, bz, rank);
+        if (more) load_rows(&maps.k[mi], bar, smem + kSmemKr + r * kHalfTile, (first + j + kRegions) * kTile, hk, bz, rank);
+        if (j + 2 >= steps) continue;
+        if (!wait(DP_FULL + (j & 1), j >> 1, kSiteProducer)) break;
+        bar = arm(S_READ + (j & 1), kHalfTile);
+        ++sr;
+        load_rows(&maps.v[mi], bar, smem + kSmemVr + (j & 1) * kHalfTile, (first + j + 2) * kTile, hk, bz, rank);
       }
       if (*abort_flag && leader) {
-        drain(&bars[Q_FULL], 1, p.status, VOMNI_DEV_TIMEOUT_BASE + kSiteDrain);
-        for (int s = 0; s < kStages; ++s)
-          drain(&bars[FULL + s], (done + kStages - 1 - s) / kStages, p.status, VOMNI_DEV_TIMEOUT_BASE + kSiteDrain);
+        drain(&bars[START], 1, p.status, VOMNI_DEV_TIMEOUT_BASE + kSiteDrain);
+        for (int s = 0; s < kRegions; ++s)
+          drain(&bars[DS_READY + s], (ds + kRegions - 1 - s) / kRegions, p.status, VOMNI_DEV_TIMEOUT_BASE + kSiteDrain);
+        for (int s = 0; s < 2; ++s)
+          drain(&bars[S_READ + s], (sr + 1 - s) / 2, p.status, VOMNI_DEV_TIMEOUT_BASE + kSiteDrain);
       }
     }
   } else if (steps > 0 && warp == 1) {
-    // Order per step j: dQ(j), dP(j+1) over dS(j), S(j+2) over S(j): the scores run two steps ahead, so that the
-    // exponentials of step j + 1 overlap dQ(j) and dP(j+1), and its dS overlaps S(j+2).
-    if (leader && lane == 0) {
-      const uint64_t q_a = desc_k(smem + kSmemQ), o_a = desc_k(smem + kSmemO);
-      auto wait = [&](int bar, uint32_t parity) {
-        return mbar_wait_spin(&bars[bar], parity, abort_flag, p.status, VOMNI_DEV_TIMEOUT_BASE + kSiteMma);
+    if (leader && lane == 0) {  // X
+      const uint64_t a = desc_k(smem + kSmemQ);
+      auto scores = [&](int r) {
+        issue_scores(tbase + kColR + r * 128, a, desc_k(smem + kSmemKr + r * kHalfTile));
+        tc_commit_pair(&bars[S_FULL + r]);
       };
-      auto stage = [&](int j) { return smem + kSmemStage + (j % kStages) * kStageBytes; };
-      auto scores = [&](int j) {  // the first use of its stage
-        if (!wait(FULL + j % kStages, (j / kStages) & 1)) return false;
+      bool ok = wait(START, 0, kSiteMma);
+      if (ok) {
         tc_fence_after();
-        issue_scores(tbase + kColS + (j & 1) * 128, q_a, desc_k(stage(j) + kKr));
-        tc_commit_pair(&bars[S_FULL + (j & 1)]);
-        return true;
-      };
-      auto dprobs = [&](int j) {
-        issue_scores(tbase + kColDp, o_a, desc_k(stage(j) + kVr));
-        tc_commit_pair(&bars[DP_FULL]);
-      };
-      bool ok = wait(Q_FULL, 0) && scores(0);
-      if (ok) dprobs(0);
-      if (ok && steps > 1) ok = scores(1);
-      for (int j = 0; ok && j < steps; ++j) {
-        if (!(ok = wait(DS_READY, j & 1))) break;
+        for (int j = 0; j < min(steps, kRegions); ++j) scores(j);
+      }
+      for (int j = 0, r = 0, use = 0; ok && j < steps; ++j) {
+        if (!(ok = wait(DS_READY + r, use, kSiteMma))) break;
         tc_fence_after();
-        issue_grad(tbase + kColDq, tbase + kColDp, desc_mn(stage(j) + kKd), j > 0);
-        tc_commit_pair(&bars[EMPTY + j % kStages]);
-        if (j + 1 < steps) dprobs(j + 1);
-        if (j + 2 < steps && !(ok = scores(j + 2))) break;
+        issue_grad(tbase + kColDq, tbase + kColR + r * 128, desc_mn(smem + kSmemKd + r * kHalfTile), j > 0);
+        if (j + kRegions < steps) scores(r);
+        if (++r == kRegions) {
+          r = 0;
+          ++use;
+        }
       }
       tc_commit_pair(&bars[OUT_FULL]);
     }
-  } else if (steps > 0) {
-    const int wg = (warp - 2) >> 2, quad = warp & 3;
-    const uint32_t lane_addr = static_cast<uint32_t>(quad * 32) << 16;
-    const uint32_t col_dp = tbase + lane_addr + kColDp;
+  } else if (steps > 0 && warp == 2) {
+    if (leader && lane == 0) {  // Y
+      const uint64_t a = desc_k(smem + kSmemO);
+      for (int j = 0, r = 0; j < steps; ++j) {
+        if (!wait(S_READ + (j & 1), j >> 1, kSiteMma)) break;
+        tc_fence_after();
+        issue_scores(tbase + kColR + r * 128, a, desc_k(smem + kSmemVr + (j & 1) * kHalfTile));
+        tc_commit_pair(&bars[DP_FULL + (j & 1)]);
+        r = r + 1 == kRegions ? 0 : r + 1;
+      }
+    }
+  } else if (steps > 0 && warp >= kControl) {
+    const int wg = (warp - kControl) >> 2, quad = warp & 3;
+    const uint32_t lane_col = tbase + (static_cast<uint32_t>(quad * 32) << 16) + kColR + kCols * wg;
     const int row = row0 + quad * 32 + lane;
     const long long at = (static_cast<long long>(b) * p.hq + h) * p.rows + row;
     const bool known = row < p.rows;  // the pair's second CTA may lie behind the last tile
-    const float nlse = known ? -p.lse2[at] : -kNoKeys, delta = known ? p.delta[at] : 0.f;
+    float nlse = -kNoKeys, neg_delta = 0.f;
+    if (known) sum_stats(p.stats[at], p.scale_log2, nlse, neg_delta);
     const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2), nlse2 = f2_pack(nlse, nlse);
-    auto wait = [&](int bar, uint32_t parity) {
-      return mbar_wait_spin(&bars[bar], parity, abort_flag, p.status, VOMNI_DEV_TIMEOUT_BASE + kSiteScores);
-    };
     bool ok = true;
-    for (int j = 0; j < steps && ok; ++j) {
-      const int valid = kv_len - (first + j) * kTile - 64 * wg;  // this warpgroup's columns that are keys
-      if (!(ok = wait(S_FULL + (j & 1), (j >> 1) & 1))) break;
+    for (int j = 0, r = 0, use = 0; j < steps && ok; ++j) {
+      const int valid = kv_len - (first + j) * kTile - kCols * wg;  // this warpgroup's columns that are keys
+      const uint32_t col = lane_col + r * 128;
+      if (!(ok = wait(S_FULL + r, use, kSiteScores))) break;
       tc_fence_after();
-      float pr[64];
+      float pr[kCols];
+      uint32_t s[kCols], pk[kCols / 2];
+      tmem_ld32(col, s);
+      tmem_ld_wait(s);
+      signal(lead_bars + (S_READ + (j & 1)) * 8);
 #pragma unroll
-      for (int ch = 0; ch < 2; ++ch) {
-        uint32_t s[32];
-        tmem_ld32(tbase + lane_addr + kColS + (j & 1) * 128 + 64 * wg + 32 * ch, s);
-        tmem_ld_wait(s);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          float x0, x1;
-          f2_unpack(f2_fma(f2_pack(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), scale2, nlse2), x0, x1);
-          pr[32 * ch + 2 * i] = ex2_approx(x0);
-          pr[32 * ch + 2 * i + 1] = ex2_approx(x1);
-        }
+      for (int i = 0; i < kCols; i += 2) {
+        float x0, x1;
+        f2_unpack(f2_fma(f2_pack(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), scale2, nlse2), x0, x1);
+        pr[i] = ex2_approx(x0);
+        pr[i + 1] = ex2_approx(x1);
       }
-      if (valid < 64) {  // columns behind the last key (zero scores) have no probability
+      if (valid < kCols) {  // columns behind the last key (zero scores) have no probability
 #pragma unroll
-        for (int i = 0; i < 64; ++i) pr[i] = i < valid ? pr[i] : 0.f;
+        for (int i = 0; i < kCols; ++i) pr[i] = i < valid ? pr[i] : 0.f;
       }
-      if (!(ok = wait(DP_FULL, j & 1))) break;
+      if (!(ok = wait(DP_FULL + (j & 1), j >> 1, kSiteScores))) break;
       tc_fence_after();
+      tmem_ld32(col, s);
+      tmem_ld_wait(s);
 #pragma unroll
-      for (int ch = 0; ch < 2; ++ch) {
-        uint32_t s[32], pk[16];
-        tmem_ld32(col_dp + 64 * wg + 32 * ch, s);
-        tmem_ld_wait(s);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int c = 32 * ch + 2 * i;
-          pk[i] = pack_bf16x2(pr[c] * (__uint_as_float(s[2 * i]) - delta), pr[c + 1] * (__uint_as_float(s[2 * i + 1]) - delta));
-        }
-        tmem_st16(col_dp + pcol(4 * wg + 2 * ch), pk);
+      for (int i = 0; i < kCols; i += 2)
+        pk[i / 2] = pack_bf16x2(pr[i] * (__uint_as_float(s[i]) + neg_delta), pr[i + 1] * (__uint_as_float(s[i + 1]) + neg_delta));
+      tmem_st16(col, pk);
+      publish(lead_bars + (DS_READY + r) * 8);
+      if (++r == kRegions) {
+        r = 0;
+        ++use;
       }
-      publish(lead_bars + DS_READY * 8);
     }
-    out_ok = ok && mbar_wait_spin(&bars[OUT_FULL], 0, abort_flag, p.status, VOMNI_DEV_TIMEOUT_BASE + kSiteOut);
+    out_ok = ok && wait(OUT_FULL, 0, kSiteOut);
     tc_fence_after();
   }
 
-  if (warp >= 2 && out_ok) {
-    const int wg = (warp - 2) >> 2, quad = warp & 3;
+  if (warp >= kControl && out_ok) {
+    const int wg = (warp - kControl) >> 2, quad = warp & 3;
     const int row = row0 + quad * 32 + lane;
     const bool parts = p.splits > 1;
     const long long at = (parts ? split * p.part : 0) +
-                         ((static_cast<long long>(b) * p.s_q + row) * p.hq + h) * kD + 64 * wg;
-    store_half_row(tbase + (static_cast<uint32_t>(quad * 32) << 16) + kColDq + 64 * wg, p.scale, steps > 0,
-                   row < q_len, row < p.s_q, parts, p.out0, at);
+                         ((static_cast<long long>(b) * p.s_q + row) * p.hq + h) * kD + kCols * wg;
+    store_share(tbase + (static_cast<uint32_t>(quad * 32) << 16) + kColDq + kCols * wg, p.scale, steps > 0, row < q_len,
+                row < p.s_q, parts, p.out0, at);
   }
-  if (steps > 0) {
-    tc_fence_before();
-    cluster_sync();
-    if (warp == 1) {
-      tc_fence_after();
-      tmem_dealloc_pair(tbase, 512);
-    }
-  }
+  if (steps > 0) close_cta(tbase);
 }
 }  // namespace dq
 
-// ================================================================ rows: delta and lse2
+// ================================================================ rows: lse and delta
 struct RowParams {
   const __nv_bfloat16* o;
   const __nv_bfloat16* d_o;
@@ -595,8 +632,8 @@ struct RowParams {
   int lens;  // q_len per batch element (b <= kMaxSeqs), else q_len[0]
   int q_len[kMaxSeqs];
   int b0;
-  float* lse2;
-  float* delta;
+  float scale;
+  uint4* stats;
 };
 
 // One half-warp per row, 8 values a lane. Rows behind a sequence's end (up to the tile's) get no probability.
@@ -624,13 +661,14 @@ __global__ void __launch_bounds__(256) attn_bwd_rows_kernel(const __grid_constan
   for (int s = 8; s > 0; s >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, s);
   if (sub == 0) {
     const long long bh = static_cast<long long>(b) * p.hq + h;
-    float l = kNoKeys;
+    const float none = p.scale > 0.f ? -kNoKeys : kNoKeys;
+    float l = none;
     if (in) {
       const float v = p.lse[(bh * 128 + (row & 127)) * p.groups + (row >> 7)];
-      l = v == -INFINITY ? kNoKeys : v * kLog2e;
+      if (!isinf(v)) l = -v / p.scale;
+      if (fabsf(l) > kNoKeys) l = l > 0.f ? kNoKeys : -kNoKeys;
     }
-    p.lse2[bh * p.rows + row] = l;
-    p.delta[bh * p.rows + row] = acc;
+    p.stats[bh * p.rows + row] = stats_of(l, -acc);
   }
 }
 
@@ -681,7 +719,7 @@ Plan plan_of(int b, int s_q, int s_kv, int hq, int hkv) {
   const int walk = q_tiles * (hq / hkv);
   p.k_splits = choose_splits(static_cast<long long>(b) * hkv * ((k_tiles + 1) / 2), walk);
   p.k_per = (walk + p.k_splits - 1) / p.k_splits;
-  p.row_bytes = align_up(static_cast<size_t>(b) * hq * p.rows * sizeof(float), 256);
+  p.row_bytes = align_up(static_cast<size_t>(b) * hq * p.rows * sizeof(uint4), 256);
   const size_t dq = p.q_splits > 1 ? static_cast<size_t>(p.q_splits) * b * s_q * hq * kD * 4 : 0;
   const size_t dkv = p.k_splits > 1 ? 2 * static_cast<size_t>(p.k_splits) * b * s_kv * hkv * kD * 4 : 0;
   p.part_bytes = std::max(dq, dkv);  // the two kernels' parts live one after the other
@@ -690,7 +728,8 @@ Plan plan_of(int b, int s_q, int s_kv, int hq, int hkv) {
 
 bool bad_shape(int b, int s_q, int s_kv, int hq, int hkv, int d) {
   return d != kD || b <= 0 || s_q <= 0 || s_kv <= 0 || hq <= 0 || hkv <= 0 || hq % hkv || hq > 65535 || b > 4095 ||
-         s_q > (1 << 24) || s_kv > (1 << 24) || static_cast<long long>((s_q + 127) / 128) * (hq / hkv) > (1 << 30);
+         s_q > (1 << 24) || s_kv > (1 << 24) ||
+         static_cast<long long>(b) * hq * ((s_q + 127) / 128 * 128) > 0x7fffffffll;
 }
 
 int make_maps(CUtensorMap* q, CUtensorMap* k, CUtensorMap* v, CUtensorMap* o, const void* const (&base)[4],
@@ -723,7 +762,7 @@ using namespace vomni;
 extern "C" size_t vomni_attention_bwd_workspace_bytes(int b, int s_q, int s_kv, int hq, int hkv, int d) {
   if (abwd::bad_shape(b, s_q, s_kv, hq, hkv, d)) return 0;
   const abwd::Plan p = abwd::plan_of(b, s_q, s_kv, hq, hkv);
-  return 2 * p.row_bytes + p.part_bytes;
+  return p.row_bytes + p.part_bytes;
 }
 
 // Launches both kernels for batch elements [p.b0, p.b0 + n) with their maps.
@@ -753,6 +792,7 @@ extern "C" int vomni_attention_bwd(const void* grad_o, const void* q, const void
                                    vomni_stream_t stream) {
   using namespace abwd;
   if (!grad_o || !q || !k || !v || !o || !lse || !strides || !dq || !dk || !dv || !workspace) return VOMNI_EINVAL;
+  if (!(std::fabs(softmax_scale) >= 1e-20f && std::fabs(softmax_scale) <= 1e20f)) return VOMNI_EINVAL;
   if (bad_shape(b, s_q, s_kv, hq, hkv, d)) return VOMNI_EBADSHAPE;
   for (int i = 0; i < b; ++i)
     if ((q_lens && (q_lens[i] < 0 || q_lens[i] > s_q)) || (kv_lens && (kv_lens[i] < 0 || kv_lens[i] > s_kv)))
@@ -764,7 +804,7 @@ extern "C" int vomni_attention_bwd(const void* grad_o, const void* q, const void
   if (al & 15) return VOMNI_EALIGN;
   if (reinterpret_cast<uintptr_t>(lse) & 3) return VOMNI_EALIGN;
   const Plan plan = plan_of(b, s_q, s_kv, hq, hkv);
-  if (workspace_bytes < 2 * plan.row_bytes + plan.part_bytes) return VOMNI_EWORKSPACE;
+  if (workspace_bytes < plan.row_bytes + plan.part_bytes) return VOMNI_EWORKSPACE;
   // strides: (row, head, batch) of q, k, v, grad_o, o in elements, multiples of 8 where the extent is over 1
   long long st4[4][3], so[3];
   for (int t = 0; t < 5; ++t) {
@@ -787,12 +827,11 @@ extern "C" int vomni_attention_bwd(const void* grad_o, const void* q, const void
   p.hkv = hkv;
   p.group = hq / hkv;
   p.rows = plan.rows;
-  p.lse2 = reinterpret_cast<float*>(ws);
-  p.delta = reinterpret_cast<float*>(ws + plan.row_bytes);
+  p.stats = reinterpret_cast<const uint4*>(ws);
   p.scale = softmax_scale;
   p.scale_log2 = softmax_scale * kLog2e;
   p.status = device_status_ptr();
-  void* parts = ws + 2 * plan.row_bytes;
+  void* parts = ws + plan.row_bytes;
 
   const int chunk = lens ? kMaxSeqs : b;
   auto fill_lens = [&](int b0, int n) {
@@ -819,13 +858,19 @@ extern "C" int vomni_attention_bwd(const void* grad_o, const void* q, const void
     r.lens = lens;
     for (int i = 0; i < kMaxSeqs; ++i) r.q_len[i] = p.q_len[i];
     r.b0 = b0;
-    r.lse2 = const_cast<float*>(p.lse2);
-    r.delta = const_cast<float*>(p.delta);
+    r.scale = softmax_scale;
+    r.stats = const_cast<uint4*>(p.stats);
     const long long blocks = (static_cast<long long>(n) * hq * plan.rows * 16 + 255) / 256;
     if (blocks > 0x7fffffffll) return VOMNI_EBADSHAPE;
     attn_bwd_rows_kernel<<<static_cast<unsigned>(blocks), 256, 0, st>>>(r);
     VOMNI_CUDA_TRY(cudaGetLastError());
   }
+  // The maps come after the launches above: encoding one needs the thread's driver context, which a thread that has made no
+  // runtime call yet (autograd's) gets from its first launch.
+  CUtensorMap stats_map;
+  rc = make_tmap_2d_plain(&stats_map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, ws, 8, static_cast<uint64_t>(b) * hq * plan.rows, 16,
+                          8, 64);
+  if (rc) return rc;
   for (int pass = 0; pass < 2; ++pass) {  // dK and dV, then dQ
     p.splits = pass == 0 ? plan.k_splits : plan.q_splits;
     p.per_split = pass == 0 ? plan.k_per : plan.q_per;
@@ -839,12 +884,14 @@ extern "C" int vomni_attention_bwd(const void* grad_o, const void* q, const void
       fill_lens(b0, n);
       if (!lens) {
         Maps<1> maps;
+        maps.stats = stats_map;
         const void* const base[4] = {q, k, v, grad_o};
         rc = make_maps(maps.q, maps.k, maps.v, maps.d_o, base, st4, b, s_q, s_kv, hq, hkv);
         if (rc) return rc;
         rc = launch_pair<1>(maps, p, plan, n, pass, st);
       } else {
         Maps<kMaxSeqs> maps;
+        maps.stats = stats_map;
         for (int i = 0; i < n; ++i) {
           const void* base[4];
           const void* all[4] = {q, k, v, grad_o};
