@@ -6,7 +6,7 @@
 // (vllm_omni_neuron/kernels/nkilib/experimental/attention/ring_attention_const_max_fwd.py:1062-1065), so the gradients
 // of a part of the keys are those of that part of the whole softmax, and parts add up.
 //
-// Two tensor-core kernels, one per side of the score matrix, so that every gradient is summed in one CTA pair's TMEM
+// Two kinds of CTA pairs, one per side of the score matrix, so that every gradient is summed in one CTA pair's TMEM
 // in a fixed order and written once: no atomics, no fp32 gradient in HBM, the same bits every time. The price is
 // that S and dP are formed twice: 7 matrix products instead of the 5 of one pass that adds dQ with atomics.
 //   dkdv: a pair of CTAs holds 256 keys of one key head (128 rows of TMEM in each) and walks the query tiles of every
@@ -21,7 +21,8 @@
 // A wait costs an issuer some 170 to 300 clocks after its last MMA, and the tensor pipe queues about one, so each issuer
 // waits once a step: on one barrier that counts the score warps' arrivals and the bytes of every operand of that step.
 // The products that depend on different events are issued by different warps, so that one's wait is filled with the
-// other's products: issuer X the gradients and the scores that follow them in the same TMEM columns, issuer Y dP.
+// other's products: issuer X the gradients and the scores that follow them in the same TMEM columns, issuer Y dP. The pipe takes
+// two issuers' products in turn, so X lets Y's batch go ahead where the score warps need it first.
 // Matrix products per 128 x 128 scores of a CTA: 512 clocks each; exponentials: 1024 clocks of the MUFU unit.
 //
 // Rounding: P and dS are rounded to bf16 as tensor-core operands (2^-8 relative each, at most); everything else is fp32 until the
@@ -69,12 +70,52 @@ struct Params {
   int rows;                   // row pitch of stats: s_q rounded up to whole tiles
   const uint4* stats;         // [b * hq, rows]: -lse / scale and -delta, three bf16 pieces each (stats_of)
   float scale, scale_log2;
-  int splits, per_split;      // the walked tiles are dealt to splits of per_split tiles
-  void* out0;                 // dq | dk: bf16 [b, s, heads, 128], or fp32 parts [split][b, s, heads, 128]
-  void* out1;                 // dv
-  long long part;             // elements of one part
+  // The launch's CTA pairs: the dK/dV ones first (they walk longer), then the dQ ones. A walk's tiles are dealt to
+  // splits of `per` tiles.
+  int k_pairs;                // pairs of 256 keys, over all key heads, batch elements and splits
+  int k_tiles2, q_tiles2;     // 256-row tiles of a head's keys / queries
+  int k_splits, k_per, q_splits, q_per;
+  void *dq, *dk, *dv;         // bf16 [b, s, heads, 128], or, where split, fp32 parts [split][b, s, heads, 128]
+  long long q_part, k_part;   // elements of one part
   int* status;
 };
+
+// Device status sites (VOMNI_DEV_TIMEOUT_BASE + site).
+enum Site : int { kSiteProducer = 0x40, kSiteMma = 0x41, kSiteScores = 0x42, kSiteOut = 0x43, kSiteDrain = 0x44 };
+
+// mbar_wait without suspension: the thread polls with test_wait (a suspended thread wakes some hundred clocks late), looking
+// at the abort flag and the clock once in 64 polls.
+VOMNI_DEV bool mbar_poll(uint64_t* bar, uint32_t parity, volatile int* abort, int* status, int code) {
+  const uint32_t addr = smem_u32(bar);
+  uint64_t t0 = 0;
+  while (true) {
+#pragma unroll 1
+    for (int i = 0; i < 64; ++i) {
+      uint32_t ok;
+      asm volatile(
+          "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+          : "=r"(ok)
+          : "r"(addr), "r"(parity)
+          : "memory");
+      if (ok) return true;
+    }
+    if (*abort) return false;
+    const uint64_t t = globaltimer();
+    if (t0 == 0) t0 = t;
+    if (t - t0 > kWaitBudgetNs) {
+      *abort = 1;
+      if (status) atomicCAS(status, 0, code);
+      return false;
+    }
+  }
+}
+
+// The issuers poll; the others may be suspended, which leaves them the issue slots and power. (32760 tokens, clocks a step:
+// dkdv 2660 with polling score warps, 2610 with suspended ones; dq 2520 and 2790, so its score warps poll.)
+VOMNI_DEV bool wait_for(uint64_t* bar, uint32_t parity, volatile int* abort, int* status, int site) {
+  const int code = VOMNI_DEV_TIMEOUT_BASE + site;
+  return site == kSiteMma ? mbar_poll(bar, parity, abort, status, code) : mbar_wait_spin(bar, parity, abort, status, code);
+}
 
 // P / dS in TMEM: the bf16 values of columns [16 kk, 16 kk + 16) sit in the 8 TMEM columns from pcol(kk). Each
 // warpgroup writes over score columns that it has read itself.
@@ -125,18 +166,11 @@ VOMNI_DEV void publish(uint32_t bar_cluster) {
   signal(bar_cluster);
 }
 
-// kCols columns of one row of a gradient, times `scale`, to the output row (bf16, or fp32 parts). `computed`: the columns
-// hold sums (uniform over the CTA); rows that are not in the sequence (`in`) are written as zero, `ok`: in the tensor.
-VOMNI_DEV void store_share(uint32_t col, float scale, bool computed, bool in, bool ok, bool parts, void* out, long long at) {
-  uint32_t o[kCols];
-  if (computed) {
-    tmem_ld32(col, o);
-    tmem_ld_wait(o);
-  }
-  if (!ok) return;
+// kCols columns of one row of a gradient (its fp32 sums, raw), times `scale`, to the output row (bf16, or fp32 parts).
+VOMNI_DEV void store_share(const uint32_t (&o)[kCols], float scale, bool parts, void* out, long long at) {
   float v[kCols];
 #pragma unroll
-  for (int i = 0; i < kCols; ++i) v[i] = computed && in ? __uint_as_float(o[i]) * scale : 0.f;
+  for (int i = 0; i < kCols; ++i) v[i] = __uint_as_float(o[i]) * scale;
   if (parts) {
     float4* dst = reinterpret_cast<float4*>(static_cast<float*>(out) + at);
 #pragma unroll
@@ -149,6 +183,10 @@ VOMNI_DEV void store_share(uint32_t col, float scale, bool computed, bool in, bo
                           pack_bf16x2(v[8 * i + 4], v[8 * i + 5]), pack_bf16x2(v[8 * i + 6], v[8 * i + 7]));
   }
 }
+VOMNI_DEV void clear(uint32_t (&o)[kCols]) {
+#pragma unroll
+  for (int i = 0; i < kCols; ++i) o[i] = 0u;
+}
 
 // A CTA that gave up waits (bounded) for the copies it may still have in flight: barrier `bar` has had `uses` loads.
 VOMNI_DEV void drain(uint64_t* bar, int uses, int* status, int code) {
@@ -156,9 +194,6 @@ VOMNI_DEV void drain(uint64_t* bar, int uses, int* status, int code) {
   int ignored = 0;
   mbar_wait(bar, (uses - 1) & 1, &ignored, status, code);
 }
-
-// Device status sites (VOMNI_DEV_TIMEOUT_BASE + site).
-enum Site : int { kSiteProducer = 0x40, kSiteMma = 0x41, kSiteScores = 0x42, kSiteOut = 0x43, kSiteDrain = 0x44 };
 
 // A float as the sum of three bf16 (8 bits each: 2^-24 relative), in the low halves of three words.
 VOMNI_DEV void pieces_of(float v, uint32_t (&w)[3]) {
@@ -248,25 +283,22 @@ VOMNI_DEV uint64_t desc_aux(const void* p) { return make_sdesc(smem_u32(p), 0, 1
 VOMNI_DEV uint64_t desc_ones(const void* p) { return make_sdesc(smem_u32(p), 128, 256, 0); }
 
 template <int N>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-    attn_bwd_dkdv_kernel(const __grid_constant__ Maps<N> maps, const __grid_constant__ Params p) {
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+VOMNI_DEV void body(const Maps<N>& maps, const Params& p, uint8_t* smem, int pair) {
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kSmemBar);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + kSmemBar + NBAR * 8 + 4);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
   const bool leader = rank == 0;
-  const int pair_row = (blockIdx.x >> 1) * 2 * kTile;
+  const int pair_row = pair % p.k_tiles2 * 2 * kTile;
   const int row0 = pair_row + static_cast<int>(rank) * kTile;  // this CTA's first key
-  const int hk = blockIdx.y;
-  const int seq = blockIdx.z / p.splits, split = blockIdx.z % p.splits;
+  const int hk = pair / p.k_tiles2 % p.hkv, z = pair / p.k_tiles2 / p.hkv;
+  const int seq = z / p.k_splits, split = z % p.k_splits;
   const int mi = N == 1 ? 0 : seq, bz = N == 1 ? seq : 0, b = p.b0 + seq;
   const int q_len = p.q_len[mi], kv_len = p.kv_len[mi];
   const int q_tiles = (q_len + kTile - 1) / kTile;
   // this split's steps of the walk over (query head of the group, query tile)
-  const int first = split * p.per_split;
-  const int last = min(first + p.per_split, q_tiles * p.group);
+  const int first = split * p.k_per;
+  const int last = min(first + p.k_per, q_tiles * p.group);
   const int steps = pair_row < kv_len ? max(last - first, 0) : 0;
 
   if (steps > 0 && threadIdx.x < 256) {  // row threadIdx.x % 128 of one of the two A tiles of ones
@@ -282,7 +314,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     tbase = open_cta(bars, NBAR, S_READ, OUT_FULL, reinterpret_cast<uint32_t*>(smem + kSmemBar + NBAR * 8), abort_flag);
   const uint32_t lead_bars = mapa_shared(smem_u32(bars), 0);
   auto wait = [&](int bar, uint32_t use, int site) {  // for phase `use` of a barrier
-    return mbar_wait_spin(&bars[bar], use & 1, abort_flag, p.status, VOMNI_DEV_TIMEOUT_BASE + site);
+    return wait_for(&bars[bar], use & 1, abort_flag, p.status, site);
   };
   bool out_ok = steps == 0;
 
@@ -304,6 +336,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const int ahead = min(steps, 2);
       uint32_t bar = arm(START, kTileBytes + ahead * (kHalfTile + kAuxBytes));
       load_resident(&maps.k[mi], bar, smem + kSmemK, row0, hk, bz);
+      pdl_wait();  // the stats come from the launch before
       for (int j = 0; j < ahead; ++j) {
         place(j, h, row);
         load_rows(&maps.q[mi], bar, smem + smem_of(kQr, j), row, h, bz, rank);
@@ -419,17 +452,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     tc_fence_after();
   }
 
-  if (warp >= kControl && out_ok) {
-    const int wg = (warp - kControl) >> 2, quad = warp & 3;
+  // The sums leave TMEM, the pair parts, and only then are the stores issued: parting waits for stores made before it.
+  const int wg = (warp - kControl) >> 2, quad = warp & 3;
+  const int row = row0 + quad * 32 + lane;
+  uint32_t dv_sum[kCols], dk_sum[kCols];
+  clear(dv_sum);
+  clear(dk_sum);
+  if (warp >= kControl && steps > 0 && out_ok) {
     const uint32_t col = tbase + (static_cast<uint32_t>(quad * 32) << 16) + kCols * wg;
-    const int row = row0 + quad * 32 + lane;
-    const bool parts = p.splits > 1;
-    const long long at = (parts ? split * p.part : 0) +
-                         ((static_cast<long long>(b) * p.s_kv + row) * p.hkv + hk) * kD + kCols * wg;
-    store_share(col + kColDv, 1.f, steps > 0, row < kv_len, row < p.s_kv, parts, p.out1, at);
-    store_share(col + kColDk, p.scale, steps > 0, row < kv_len, row < p.s_kv, parts, p.out0, at);
+    tmem_ld32(col + kColDv, dv_sum);
+    tmem_ld_wait(dv_sum);
+    tmem_ld32(col + kColDk, dk_sum);
+    tmem_ld_wait(dk_sum);
+    if (row >= kv_len) {  // rows behind the sequence are zero, whatever was summed there
+      clear(dv_sum);
+      clear(dk_sum);
+    }
   }
   if (steps > 0) close_cta(tbase);
+  if (warp >= kControl && out_ok && row < p.s_kv) {
+    const bool parts = p.k_splits > 1;
+    const long long at = (parts ? split * p.k_part : 0) +
+                         ((static_cast<long long>(b) * p.s_kv + row) * p.hkv + hk) * kD + kCols * wg;
+    store_share(dv_sum, 1.f, parts, p.dv, at);
+    store_share(dk_sum, p.scale, parts, p.dk, at);
+  }
 }
 }  // namespace dkdv
 
@@ -451,37 +498,36 @@ enum Bar : int {
   DP_FULL = S_FULL + kRegions,  // + step % 2
   S_READ = DP_FULL + 2,         // Y's, + step % 2: S of step j is read; V's rows of j (and dO, for the first) are there
   DS_READY = S_READ + 2,        // X's, + step % 3: dS of step j; K's dims of j and K's rows of j + 3 are there
-  OUT_FULL = DS_READY + kRegions,
+  Y_ISSUED = DS_READY + kRegions,  // + step % 2: dP of step j is queued on the tensor pipe
+  OUT_FULL = Y_ISSUED + 2,
   NBAR = OUT_FULL + 1
 };
 static_assert(NBAR * 8 + 8 <= 256, "barriers, TMEM slot and abort flag fit their area");
 
 template <int N>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-    attn_bwd_dq_kernel(const __grid_constant__ Maps<N> maps, const __grid_constant__ Params p) {
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+VOMNI_DEV void body(const Maps<N>& maps, const Params& p, uint8_t* smem, int pair) {
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kSmemBar);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + kSmemBar + NBAR * 8 + 4);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
   const bool leader = rank == 0;
-  const int pair_row = (blockIdx.x >> 1) * 2 * kTile;
+  const int pair_row = pair % p.q_tiles2 * 2 * kTile;
   const int row0 = pair_row + static_cast<int>(rank) * kTile;  // this CTA's first query
-  const int h = blockIdx.y, hk = h / p.group;
-  const int seq = blockIdx.z / p.splits, split = blockIdx.z % p.splits;
+  const int h = pair / p.q_tiles2 % p.hq, hk = h / p.group, z = pair / p.q_tiles2 / p.hq;
+  const int seq = z / p.q_splits, split = z % p.q_splits;
   const int mi = N == 1 ? 0 : seq, bz = N == 1 ? seq : 0, b = p.b0 + seq;
   const int q_len = p.q_len[mi], kv_len = p.kv_len[mi];
-  const int first = split * p.per_split;
-  const int last = min(first + p.per_split, (kv_len + kTile - 1) / kTile);
+  const int first = split * p.q_per;
+  const int last = min(first + p.q_per, (kv_len + kTile - 1) / kTile);
   const int steps = pair_row < q_len ? max(last - first, 0) : 0;
 
   uint32_t tbase = 0;
   if (steps > 0)
-    tbase = open_cta(bars, NBAR, S_READ, OUT_FULL, reinterpret_cast<uint32_t*>(smem + kSmemBar + NBAR * 8), abort_flag);
+    tbase = open_cta(bars, NBAR, S_READ, Y_ISSUED, reinterpret_cast<uint32_t*>(smem + kSmemBar + NBAR * 8), abort_flag);
   const uint32_t lead_bars = mapa_shared(smem_u32(bars), 0);
   auto wait = [&](int bar, uint32_t use, int site) {
-    return mbar_wait_spin(&bars[bar], use & 1, abort_flag, p.status, VOMNI_DEV_TIMEOUT_BASE + site);
+    return site == kSiteScores ? mbar_poll(&bars[bar], use & 1, abort_flag, p.status, VOMNI_DEV_TIMEOUT_BASE + site)
+                               : wait_for(&bars[bar], use & 1, abort_flag, p.status, site);
   };
   bool out_ok = steps == 0;
 
@@ -541,6 +587,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if (!(ok = wait(DS_READY + r, use, kSiteMma))) break;
         tc_fence_after();
         issue_grad(tbase + kColDq, tbase + kColR + r * 128, desc_mn(smem + kSmemKd + r * kHalfTile), j > 0);
+        // dP(j+1), which the score warps wait for next, goes ahead of S(j+3)
+        if (j + 1 < steps && !(ok = wait(Y_ISSUED + ((j + 1) & 1), (j + 1) >> 1, kSiteMma))) break;
         if (j + kRegions < steps) scores(r);
         if (++r == kRegions) {
           r = 0;
@@ -557,6 +605,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         tc_fence_after();
         issue_scores(tbase + kColR + r * 128, a, desc_k(smem + kSmemVr + (j & 1) * kHalfTile));
         tc_commit_pair(&bars[DP_FULL + (j & 1)]);
+        mbar_arrive(&bars[Y_ISSUED + (j & 1)]);
         r = r + 1 == kRegions ? 0 : r + 1;
       }
     }
@@ -567,6 +616,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const long long at = (static_cast<long long>(b) * p.hq + h) * p.rows + row;
     const bool known = row < p.rows;  // the pair's second CTA may lie behind the last tile
     float nlse = -kNoKeys, neg_delta = 0.f;
+    pdl_wait();  // the stats come from the launch before
     if (known) sum_stats(p.stats[at], p.scale_log2, nlse, neg_delta);
     const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2), nlse2 = f2_pack(nlse, nlse);
     bool ok = true;
@@ -609,18 +659,40 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     tc_fence_after();
   }
 
-  if (warp >= kControl && out_ok) {
-    const int wg = (warp - kControl) >> 2, quad = warp & 3;
-    const int row = row0 + quad * 32 + lane;
-    const bool parts = p.splits > 1;
-    const long long at = (parts ? split * p.part : 0) +
-                         ((static_cast<long long>(b) * p.s_q + row) * p.hq + h) * kD + kCols * wg;
-    store_share(tbase + (static_cast<uint32_t>(quad * 32) << 16) + kColDq + kCols * wg, p.scale, steps > 0, row < q_len,
-                row < p.s_q, parts, p.out0, at);
+  const int wg = (warp - kControl) >> 2, quad = warp & 3;
+  const int row = row0 + quad * 32 + lane;
+  uint32_t sum[kCols];
+  clear(sum);
+  if (warp >= kControl && steps > 0 && out_ok) {
+    tmem_ld32(tbase + (static_cast<uint32_t>(quad * 32) << 16) + kColDq + kCols * wg, sum);
+    tmem_ld_wait(sum);
+    if (row >= q_len) clear(sum);
   }
   if (steps > 0) close_cta(tbase);
+  if (warp >= kControl && out_ok && row < p.s_q) {
+    const bool parts = p.q_splits > 1;
+    const long long at = (parts ? split * p.q_part : 0) +
+                         ((static_cast<long long>(b) * p.s_q + row) * p.hq + h) * kD + kCols * wg;
+    store_share(sum, p.scale, parts, p.dq, at);
+  }
 }
 }  // namespace dq
+
+// A CTA pair of either kind: both are in one launch, so that the pairs of one fill the device while the other's last ones
+// run.
+constexpr uint32_t kSmemBytes = dkdv::kSmemBytes > dq::kSmemBytes ? dkdv::kSmemBytes : dq::kSmemBytes;
+template <int N>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    attn_bwd_kernel(const __grid_constant__ Maps<N> maps, const __grid_constant__ Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int pair = blockIdx.x >> 1;
+  if (pair < p.k_pairs)
+    dkdv::body<N>(maps, p, smem, pair);
+  else
+    dq::body<N>(maps, p, smem, pair - p.k_pairs);
+  pdl_wait();  // no CTA ends before the launch that it overlapped
+}
 
 // ================================================================ rows: lse and delta
 struct RowParams {
@@ -638,6 +710,7 @@ struct RowParams {
 
 // One half-warp per row, 8 values a lane. Rows behind a sequence's end (up to the tile's) get no probability.
 __global__ void __launch_bounds__(256) attn_bwd_rows_kernel(const __grid_constant__ RowParams p) {
+  pdl_trigger();
   const long long n = static_cast<long long>(p.b) * p.hq * p.rows;
   const long long i = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) >> 4;
   if (i >= n) return;  // n is a multiple of 128: whole warps leave
@@ -672,57 +745,77 @@ __global__ void __launch_bounds__(256) attn_bwd_rows_kernel(const __grid_constan
   }
 }
 
-// out = bf16(sum over parts), in order.
-__global__ void __launch_bounds__(256) attn_bwd_join_kernel(const float* __restrict__ parts, int n_parts, long long part,
-                                                            __nv_bfloat16* __restrict__ out) {
-  const long long at = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) * 4;
-  if (at >= part) return;  // part is a multiple of 128
-  float4 s = *reinterpret_cast<const float4*>(parts + at);
-  for (int i = 1; i < n_parts; ++i) {
-    const float4 t = *reinterpret_cast<const float4*>(parts + i * part + at);
-    s.x += t.x; s.y += t.y; s.z += t.z; s.w += t.w;
+// out = bf16(sum over parts), in order, of up to three gradients in one launch.
+struct JoinParams {
+  const float* parts[3];
+  __nv_bfloat16* out[3];
+  long long part[3];  // elements, 0 where there is nothing to join
+  int n[3];
+};
+__global__ void __launch_bounds__(256) attn_bwd_join_kernel(const __grid_constant__ JoinParams p) {
+  long long at = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) * 4;
+  int t = 0;
+  while (t < 3 && at >= p.part[t]) at -= p.part[t++];  // every part is a multiple of 128
+  if (t == 3) return;
+  const float* parts = p.parts[t] + at;
+  float4 s = *reinterpret_cast<const float4*>(parts);
+  for (int i = 1; i < p.n[t]; ++i) {
+    const float4 u = *reinterpret_cast<const float4*>(parts + i * p.part[t]);
+    s.x += u.x; s.y += u.y; s.z += u.z; s.w += u.w;
   }
-  *reinterpret_cast<uint2*>(out + at) = make_uint2(pack_bf16x2(s.x, s.y), pack_bf16x2(s.z, s.w));
+  *reinterpret_cast<uint2*>(p.out[t] + at) = make_uint2(pack_bf16x2(s.x, s.y), pack_bf16x2(s.z, s.w));
 }
 
 // ================================================================ host
-// How many CTA pairs share one output tile's walk of `tiles` steps: the count whose waves of pairs take the
-// least time, a pair costing its steps and about two more to start and finish (and half a step more to write
-// and join fp32 parts). 1 where the output tiles alone fill the device.
-int choose_splits(long long outputs, int tiles) {
-  const long long slots = num_sms() / 2 > 0 ? num_sms() / 2 : 1;
-  int best = 1;
-  double best_cost = 0;
-  for (int s = 1; s <= 16 && s <= tiles; ++s) {
-    const int per = (tiles + s - 1) / s;
-    if ((tiles + per - 1) / per != s) continue;  // no empty splits
-    const double cost = static_cast<double>((outputs * s + slots - 1) / slots) * (per + 2 + (s > 1 ? 1 : 0));
-    if (s == 1 || cost < best_cost * 0.97) {
-      best = s;
-      best_cost = cost;
+// How many CTA pairs share the walk of one dK/dV tile and of one dQ tile: the counts for which the launch is estimated to
+// end first. A pair takes 4 units a step (dkdv) or 3 (dq) and about 8 to start and finish; the pairs run on half as many
+// slots as there are SMs, and the last of the longest kind to start overhangs by half of its time on average. Joining
+// fp32 parts costs a launch, about 12 units. 1 and 1 where the tiles alone fill the device.
+constexpr int kMaxSplits = 16;
+bool even_split(int tiles, int s, int& per) {
+  per = (tiles + s - 1) / s;
+  return (tiles + per - 1) / per == s;  // no empty splits
+}
+void choose_splits(long long k_outputs, int k_walk, long long q_outputs, int q_walk, int& k_splits, int& q_splits) {
+  const double slots = num_sms() / 2 > 0 ? num_sms() / 2 : 1;
+  double best = 0;
+  k_splits = q_splits = 1;
+  for (int sk = 1; sk <= kMaxSplits && sk <= k_walk; ++sk) {
+    int k_per, q_per;
+    if (!even_split(k_walk, sk, k_per)) continue;
+    for (int sq = 1; sq <= kMaxSplits && sq <= q_walk; ++sq) {
+      if (!even_split(q_walk, sq, q_per)) continue;
+      const double k_len = 4.0 * k_per + 8, q_len = 3.0 * q_per + 8;
+      const double work = k_outputs * sk * k_len + q_outputs * sq * q_len;
+      const double longest = std::max(k_len, q_len);
+      const double cost = std::max(work / slots + longest / 2, longest) + (sk > 1 || sq > 1 ? 12 : 0);
+      if (best == 0 || cost < best * 0.98) {
+        best = cost;
+        k_splits = sk;
+        q_splits = sq;
+      }
     }
   }
-  return best;
 }
 
 struct Plan {
   int rows;
   int q_splits, q_per, k_splits, k_per;  // splits of the dq walk (key tiles) and of the dkdv walk (query tiles)
-  size_t row_bytes, part_bytes;
+  size_t row_bytes, q_bytes, k_bytes;    // stats; dq's parts; dk's parts, and dv's
+  size_t bytes() const { return row_bytes + q_bytes + 2 * k_bytes; }
 };
 Plan plan_of(int b, int s_q, int s_kv, int hq, int hkv) {
   Plan p;
   const int q_tiles = (s_q + kTile - 1) / kTile, k_tiles = (s_kv + kTile - 1) / kTile;
   p.rows = q_tiles * kTile;
-  p.q_splits = choose_splits(static_cast<long long>(b) * hq * ((q_tiles + 1) / 2), k_tiles);
-  p.q_per = (k_tiles + p.q_splits - 1) / p.q_splits;
   const int walk = q_tiles * (hq / hkv);
-  p.k_splits = choose_splits(static_cast<long long>(b) * hkv * ((k_tiles + 1) / 2), walk);
+  choose_splits(static_cast<long long>(b) * hkv * ((k_tiles + 1) / 2), walk, static_cast<long long>(b) * hq * ((q_tiles + 1) / 2),
+                k_tiles, p.k_splits, p.q_splits);
+  p.q_per = (k_tiles + p.q_splits - 1) / p.q_splits;
   p.k_per = (walk + p.k_splits - 1) / p.k_splits;
   p.row_bytes = align_up(static_cast<size_t>(b) * hq * p.rows * sizeof(uint4), 256);
-  const size_t dq = p.q_splits > 1 ? static_cast<size_t>(p.q_splits) * b * s_q * hq * kD * 4 : 0;
-  const size_t dkv = p.k_splits > 1 ? 2 * static_cast<size_t>(p.k_splits) * b * s_kv * hkv * kD * 4 : 0;
-  p.part_bytes = std::max(dq, dkv);  // the two kernels' parts live one after the other
+  p.q_bytes = p.q_splits > 1 ? static_cast<size_t>(p.q_splits) * b * s_q * hq * kD * 4 : 0;
+  p.k_bytes = p.k_splits > 1 ? static_cast<size_t>(p.k_splits) * b * s_kv * hkv * kD * 4 : 0;
   return p;
 }
 
@@ -745,15 +838,6 @@ int make_maps(CUtensorMap* q, CUtensorMap* k, CUtensorMap* v, CUtensorMap* o, co
   return VOMNI_OK;
 }
 
-int join(const void* parts, int n, long long part, void* out, cudaStream_t st) {
-  const long long blocks = (part / 4 + 255) / 256;
-  if (blocks > 0x7fffffffll) return VOMNI_EBADSHAPE;
-  attn_bwd_join_kernel<<<static_cast<unsigned>(blocks), 256, 0, st>>>(static_cast<const float*>(parts), n, part,
-                                                                      static_cast<__nv_bfloat16*>(out));
-  VOMNI_CUDA_TRY(cudaGetLastError());
-  return VOMNI_OK;
-}
-
 }  // namespace abwd
 }  // namespace vomni
 
@@ -762,26 +846,31 @@ using namespace vomni;
 extern "C" size_t vomni_attention_bwd_workspace_bytes(int b, int s_q, int s_kv, int hq, int hkv, int d) {
   if (abwd::bad_shape(b, s_q, s_kv, hq, hkv, d)) return 0;
   const abwd::Plan p = abwd::plan_of(b, s_q, s_kv, hq, hkv);
-  return p.row_bytes + p.part_bytes;
+  return p.bytes();
 }
 
-// Launches both kernels for batch elements [p.b0, p.b0 + n) with their maps.
+// Launches the pairs of batch elements [p.b0, p.b0 + n) with their maps, as a dependent of the stats' launch.
 template <int N>
-static int launch_pair(const abwd::Maps<N>& maps, abwd::Params p, const abwd::Plan& plan, int n, int dq_or_dkdv,
-                       cudaStream_t st) {
+static int launch_pairs(const abwd::Maps<N>& maps, abwd::Params p, int n, cudaStream_t st) {
   using namespace abwd;
-  if (dq_or_dkdv == 0) {
-    auto kern = dkdv::attn_bwd_dkdv_kernel<N>;
-    int rc = ensure_max_smem(kern, dkdv::kSmemBytes);
-    if (rc) return rc;
-    kern<<<dim3(2 * ((p.s_kv + 255) / 256), p.hkv, n * p.splits), kThreads, dkdv::kSmemBytes, st>>>(maps, p);
-  } else {
-    auto kern = dq::attn_bwd_dq_kernel<N>;
-    int rc = ensure_max_smem(kern, dq::kSmemBytes);
-    if (rc) return rc;
-    kern<<<dim3(2 * ((p.s_q + 255) / 256), p.hq, n * p.splits), kThreads, dq::kSmemBytes, st>>>(maps, p);
-  }
-  VOMNI_CUDA_TRY(cudaGetLastError());
+  const long long k_pairs = static_cast<long long>(p.k_tiles2) * p.hkv * n * p.k_splits;
+  const long long pairs = k_pairs + static_cast<long long>(p.q_tiles2) * p.hq * n * p.q_splits;
+  if (pairs > (1 << 30)) return VOMNI_EBADSHAPE;
+  p.k_pairs = static_cast<int>(k_pairs);
+  auto kern = attn_bwd_kernel<N>;
+  int rc = ensure_max_smem(kern, kSmemBytes);
+  if (rc) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(2 * pairs));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmemBytes;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  VOMNI_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, maps, p));
   return VOMNI_OK;
 }
 
@@ -804,7 +893,7 @@ extern "C" int vomni_attention_bwd(const void* grad_o, const void* q, const void
   if (al & 15) return VOMNI_EALIGN;
   if (reinterpret_cast<uintptr_t>(lse) & 3) return VOMNI_EALIGN;
   const Plan plan = plan_of(b, s_q, s_kv, hq, hkv);
-  if (workspace_bytes < plan.row_bytes + plan.part_bytes) return VOMNI_EWORKSPACE;
+  if (workspace_bytes < plan.bytes()) return VOMNI_EWORKSPACE;
   // strides: (row, head, batch) of q, k, v, grad_o, o in elements, multiples of 8 where the extent is over 1
   long long st4[4][3], so[3];
   for (int t = 0; t < 5; ++t) {
@@ -831,7 +920,18 @@ extern "C" int vomni_attention_bwd(const void* grad_o, const void* q, const void
   p.scale = softmax_scale;
   p.scale_log2 = softmax_scale * kLog2e;
   p.status = device_status_ptr();
-  void* parts = ws + plan.row_bytes;
+  p.k_tiles2 = (s_kv + 2 * kTile - 1) / (2 * kTile);
+  p.q_tiles2 = (s_q + 2 * kTile - 1) / (2 * kTile);
+  p.k_splits = plan.k_splits;
+  p.k_per = plan.k_per;
+  p.q_splits = plan.q_splits;
+  p.q_per = plan.q_per;
+  p.q_part = static_cast<long long>(b) * s_q * hq * kD;
+  p.k_part = static_cast<long long>(b) * s_kv * hkv * kD;
+  uint8_t* parts = ws + plan.row_bytes;
+  p.dq = plan.q_splits > 1 ? parts : dq;
+  p.dk = plan.k_splits > 1 ? parts + plan.q_bytes : dk;
+  p.dv = plan.k_splits > 1 ? parts + plan.q_bytes + plan.k_bytes : dv;
 
   const int chunk = lens ? kMaxSeqs : b;
   auto fill_lens = [&](int b0, int n) {
@@ -864,53 +964,48 @@ extern "C" int vomni_attention_bwd(const void* grad_o, const void* q, const void
     if (blocks > 0x7fffffffll) return VOMNI_EBADSHAPE;
     attn_bwd_rows_kernel<<<static_cast<unsigned>(blocks), 256, 0, st>>>(r);
     VOMNI_CUDA_TRY(cudaGetLastError());
-  }
-  // The maps come after the launches above: encoding one needs the thread's driver context, which a thread that has made no
-  // runtime call yet (autograd's) gets from its first launch.
-  CUtensorMap stats_map;
-  rc = make_tmap_2d_plain(&stats_map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, ws, 8, static_cast<uint64_t>(b) * hq * plan.rows, 16,
-                          8, 64);
-  if (rc) return rc;
-  for (int pass = 0; pass < 2; ++pass) {  // dK and dV, then dQ
-    p.splits = pass == 0 ? plan.k_splits : plan.q_splits;
-    p.per_split = pass == 0 ? plan.k_per : plan.q_per;
-    p.part = static_cast<long long>(b) * (pass == 0 ? s_kv : s_q) * (pass == 0 ? hkv : hq) * kD;
-    const bool split = p.splits > 1;
-    p.out0 = split ? parts : pass == 0 ? dk : dq;
-    p.out1 = pass == 0 ? (split ? static_cast<float*>(parts) + p.splits * p.part : dv) : nullptr;
-    for (int b0 = 0; b0 < b; b0 += chunk) {
-      const int n = std::min(chunk, b - b0);
-      if (static_cast<long long>(n) * p.splits > 65535) return VOMNI_EBADSHAPE;
-      fill_lens(b0, n);
-      if (!lens) {
-        Maps<1> maps;
-        maps.stats = stats_map;
-        const void* const base[4] = {q, k, v, grad_o};
-        rc = make_maps(maps.q, maps.k, maps.v, maps.d_o, base, st4, b, s_q, s_kv, hq, hkv);
-        if (rc) return rc;
-        rc = launch_pair<1>(maps, p, plan, n, pass, st);
-      } else {
-        Maps<kMaxSeqs> maps;
-        maps.stats = stats_map;
-        for (int i = 0; i < n; ++i) {
-          const void* base[4];
-          const void* all[4] = {q, k, v, grad_o};
-          for (int t = 0; t < 4; ++t) base[t] = static_cast<const __nv_bfloat16*>(all[t]) + (b0 + i) * st4[t][2];
-          const void* const fixed[4] = {base[0], base[1], base[2], base[3]};
-          // a length of 0 is never loaded from, but a map has no empty extent
-          rc = make_maps(&maps.q[i], &maps.k[i], &maps.v[i], &maps.d_o[i], fixed, st4, 1, std::max(p.q_len[i], 1),
-                         std::max(p.kv_len[i], 1), hq, hkv);
-          if (rc) return rc;
-        }
-        rc = launch_pair<kMaxSeqs>(maps, p, plan, n, pass, st);
+    // The maps come after a launch: encoding one needs the thread's driver context, which a thread that has made no
+    // runtime call yet (autograd's) gets from its first launch.
+    CUtensorMap stats_map;
+    rc = make_tmap_2d_plain(&stats_map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, ws, 8, static_cast<uint64_t>(b) * hq * plan.rows, 16,
+                            8, 64);
+    if (rc) return rc;
+    const __nv_bfloat16* all[4] = {static_cast<const __nv_bfloat16*>(q), static_cast<const __nv_bfloat16*>(k),
+                                   static_cast<const __nv_bfloat16*>(v), static_cast<const __nv_bfloat16*>(grad_o)};
+    if (!lens) {
+      Maps<1> maps;
+      maps.stats = stats_map;
+      const void* const base[4] = {all[0], all[1], all[2], all[3]};
+      rc = make_maps(maps.q, maps.k, maps.v, maps.d_o, base, st4, b, s_q, s_kv, hq, hkv);
+      if (!rc) rc = launch_pairs<1>(maps, p, n, st);
+    } else {
+      Maps<kMaxSeqs> maps;
+      maps.stats = stats_map;
+      for (int i = 0; i < n && !rc; ++i) {
+        const void* const base[4] = {all[0] + (b0 + i) * st4[0][2], all[1] + (b0 + i) * st4[1][2],
+                                     all[2] + (b0 + i) * st4[2][2], all[3] + (b0 + i) * st4[3][2]};
+        // a length of 0 is never loaded from, but a map has no empty extent
+        rc = make_maps(&maps.q[i], &maps.k[i], &maps.v[i], &maps.d_o[i], base, st4, 1, std::max(p.q_len[i], 1),
+                       std::max(p.kv_len[i], 1), hq, hkv);
       }
-      if (rc) return rc;
+      if (!rc) rc = launch_pairs<kMaxSeqs>(maps, p, n, st);
     }
-    if (split) {
-      rc = join(parts, p.splits, p.part, pass == 0 ? dk : dq, st);
-      if (rc) return rc;
-      if (pass == 0 && (rc = join(p.out1, p.splits, p.part, dv, st))) return rc;
+    if (rc) return rc;
+  }
+  if (plan.q_splits > 1 || plan.k_splits > 1) {
+    JoinParams j = {};
+    const void* from[3] = {p.dq, p.dk, p.dv};
+    void* to[3] = {dq, dk, dv};
+    for (int t = 0; t < 3; ++t) {
+      j.parts[t] = static_cast<const float*>(from[t]);
+      j.out[t] = static_cast<__nv_bfloat16*>(to[t]);
+      j.n[t] = t ? plan.k_splits : plan.q_splits;
+      j.part[t] = j.n[t] > 1 ? (t ? p.k_part : p.q_part) : 0;
     }
+    const long long blocks = ((j.part[0] + j.part[1] + j.part[2]) / 4 + 255) / 256;
+    if (blocks > 0x7fffffffll) return VOMNI_EBADSHAPE;
+    attn_bwd_join_kernel<<<static_cast<unsigned>(blocks), 256, 0, st>>>(j);
+    VOMNI_CUDA_TRY(cudaGetLastError());
   }
   return VOMNI_OK;
 }
