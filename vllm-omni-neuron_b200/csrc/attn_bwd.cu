@@ -83,8 +83,8 @@ struct Params {
 // Device status sites (VOMNI_DEV_TIMEOUT_BASE + site).
 enum Site : int { kSiteProducer = 0x40, kSiteMma = 0x41, kSiteScores = 0x42, kSiteOut = 0x43, kSiteDrain = 0x44 };
 
-// mbar_wait without suspension: the thread polls with test_wait (a suspended thread wakes some hundred clocks late), looking
-// at the abort flag and the clock once in 64 polls.
+// mbar_wait whose thread is suspended for 40 ns at a time at most (without the hint it wakes some hundred clocks late), and
+// looks at the abort flag and the clock once in 64 polls.
 VOMNI_DEV bool mbar_poll(uint64_t* bar, uint32_t parity, volatile int* abort, int* status, int code) {
   const uint32_t addr = smem_u32(bar);
   uint64_t t0 = 0;
@@ -93,7 +93,7 @@ VOMNI_DEV bool mbar_poll(uint64_t* bar, uint32_t parity, volatile int* abort, in
     for (int i = 0; i < 64; ++i) {
       uint32_t ok;
       asm volatile(
-          "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+          "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 40;\n\tselp.u32 %0, 1, 0, p;\n\t}"
           : "=r"(ok)
           : "r"(addr), "r"(parity)
           : "memory");
@@ -110,8 +110,9 @@ VOMNI_DEV bool mbar_poll(uint64_t* bar, uint32_t parity, volatile int* abort, in
   }
 }
 
-// The issuers poll; the others may be suspended, which leaves them the issue slots and power. (32760 tokens, clocks a step:
-// dkdv 2660 with polling score warps, 2610 with suspended ones; dq 2520 and 2790, so its score warps poll.)
+// The issuers poll; the others may be suspended for longer, which leaves them the issue slots. (32760 tokens, clocks a step:
+// dkdv 2590 with polling score warps, 2460 with suspended ones; dq 2320 and 2790, so its score warps poll. Polling with
+// test_wait, which never suspends: 2500 and 2380.)
 VOMNI_DEV bool wait_for(uint64_t* bar, uint32_t parity, volatile int* abort, int* status, int site) {
   const int code = VOMNI_DEV_TIMEOUT_BASE + site;
   return site == kSiteMma ? mbar_poll(bar, parity, abort, status, code) : mbar_wait_spin(bar, parity, abort, status, code);
@@ -443,8 +444,11 @@ VOMNI_DEV void body(const Maps<N>& maps, const Params& p, uint8_t* smem, int pai
       for (int i = 0; i < kCols / 2; ++i) pk[i] = pack_bf16x2(pr[2 * i], pr[2 * i + 1]);
       tmem_st16(col, pk);
 #pragma unroll
-      for (int i = 0; i < kCols; i += 2)
-        pk[i / 2] = pack_bf16x2(pr[i] * __uint_as_float(s[i]), pr[i + 1] * __uint_as_float(s[i + 1]));
+      for (int i = 0; i < kCols; i += 2) {
+        float d0, d1;
+        f2_unpack(f2_mul(f2_pack(pr[i], pr[i + 1]), f2_pack(__uint_as_float(s[i]), __uint_as_float(s[i + 1]))), d0, d1);
+        pk[i / 2] = pack_bf16x2(d0, d1);
+      }
       tmem_st16(col + kDs, pk);
       publish(lead_bars + (PD_READY + (j & 1)) * 8);
     }
@@ -618,7 +622,8 @@ VOMNI_DEV void body(const Maps<N>& maps, const Params& p, uint8_t* smem, int pai
     float nlse = -kNoKeys, neg_delta = 0.f;
     pdl_wait();  // the stats come from the launch before
     if (known) sum_stats(p.stats[at], p.scale_log2, nlse, neg_delta);
-    const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2), nlse2 = f2_pack(nlse, nlse);
+    const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2), nlse2 = f2_pack(nlse, nlse),
+                   delta2 = f2_pack(neg_delta, neg_delta);
     bool ok = true;
     for (int j = 0, r = 0, use = 0; j < steps && ok; ++j) {
       const int valid = kv_len - (first + j) * kTile - kCols * wg;  // this warpgroup's columns that are keys
@@ -646,8 +651,11 @@ VOMNI_DEV void body(const Maps<N>& maps, const Params& p, uint8_t* smem, int pai
       tmem_ld32(col, s);
       tmem_ld_wait(s);
 #pragma unroll
-      for (int i = 0; i < kCols; i += 2)
-        pk[i / 2] = pack_bf16x2(pr[i] * (__uint_as_float(s[i]) + neg_delta), pr[i + 1] * (__uint_as_float(s[i + 1]) + neg_delta));
+      for (int i = 0; i < kCols; i += 2) {
+        float d0, d1;
+        f2_unpack(f2_mul(f2_pack(pr[i], pr[i + 1]), f2_add(f2_pack(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), delta2)), d0, d1);
+        pk[i / 2] = pack_bf16x2(d0, d1);
+      }
       tmem_st16(col, pk);
       publish(lead_bars + (DS_READY + r) * 8);
       if (++r == kRegions) {
