@@ -152,9 +152,10 @@ VOMNI_API int vomni_cm_attention_local(const void* q, const void* k, const void*
  * counts, or NULL): the tokens of each batch element; those behind are neither read nor counted, whatever they hold,
  * and their gradients are 0. A row whose lse is -inf has no probabilities. Given the lse of a whole sequence
  * and a part of its keys, the result is that part's share (the parts' dq add up). Bitwise reproducible (no
- * atomics). workspace: vomni_attention_bwd_workspace_bytes (depends on the current device's size; 0 =
- * unsupported shape), not shared by calls that may overlap. */
-VOMNI_API size_t vomni_attention_bwd_workspace_bytes(int b, int s_q, int s_kv, int hq, int hkv, int d);
+ * atomics). |softmax_scale| in [1e-20, 1e20]. workspace: vomni_attention_bwd_workspace_bytes for the same lengths
+ * (depends on the current device's size; 0 = unsupported shape), not shared by calls that may overlap. */
+VOMNI_API size_t vomni_attention_bwd_workspace_bytes(int b, int s_q, int s_kv, int hq, int hkv, int d, const int* q_lens,
+                                                     const int* kv_lens);
 VOMNI_API int vomni_attention_bwd(const void* grad_o, const void* q, const void* k, const void* v, const void* o,
                                   const float* lse, int b, int s_q, int s_kv, int hq, int hkv, int d,
                                   const long long* strides, const int* q_lens, const int* kv_lens, float softmax_scale,

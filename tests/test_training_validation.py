@@ -124,8 +124,8 @@ def test_c_entries(lib):
     assert bwd(strides=(ctypes.c_longlong * 15)(*([513, 128, 512 * 16] * 5))) == 3
     assert bwd(strides=(ctypes.c_longlong * 15)(*([0, 128, 512 * 16] * 5))) == 3
     assert bwd(ws=64) == 8
-    assert lib.vomni_attention_bwd_workspace_bytes(1, 16, 16, 4, 3, 128) == 0
-    assert lib.vomni_attention_bwd_workspace_bytes(2, 200, 16, 4, 4, 128) >= 2 * 2 * 4 * 256 * 4
+    assert lib.vomni_attention_bwd_workspace_bytes(1, 16, 16, 4, 3, 128, None, None) == 0
+    assert lib.vomni_attention_bwd_workspace_bytes(2, 200, 16, 4, 4, 128, None, None) >= 2 * 2 * 4 * 256 * 4
 
     axes = (ctypes.c_int * 3)(44, 42, 42)
 

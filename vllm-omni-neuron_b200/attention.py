@@ -395,11 +395,11 @@ def attention_bwd(grad_o: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: tor
     strides = (ctypes.c_longlong * 15)(*(n for _, st in src for n in st))
     q, k, v, grad_o, o = (t for t, _ in src)
     lse = _lib.dense(lse if lse.dtype == torch.float32 else lse.float())
-    ints = lambda lens: (ctypes.c_int * b)(*lens) if lens is not None else None
-    ws_bytes = _lib.on_device(dev, _lib.load().vomni_attention_bwd_workspace_bytes, b, sq, skv, hq, hkv, _HEAD_DIM)
+    q_lens, kv_lens = ((ctypes.c_int * b)(*lens) if lens is not None else None for lens in (q_lens, kv_lens))
+    ws_bytes = _lib.on_device(dev, _lib.load().vomni_attention_bwd_workspace_bytes, b, sq, skv, hq, hkv, _HEAD_DIM, q_lens, kv_lens)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
     _lib.launch(dev, "vomni_attention_bwd", grad_o.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
-                lse.data_ptr(), b, sq, skv, hq, hkv, _HEAD_DIM, strides, ints(q_lens), ints(kv_lens), scale, dq.data_ptr(),
+                lse.data_ptr(), b, sq, skv, hq, hkv, _HEAD_DIM, strides, q_lens, kv_lens, scale, dq.data_ptr(),
                 dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), ws_bytes)
     return dq, dk, dv
 

@@ -716,40 +716,55 @@ struct RowParams {
   uint4* stats;
 };
 
-// One half-warp per row, 8 values a lane. Rows behind a sequence's end (up to the tile's) get no probability.
+// A half-warp takes kRowsEach adjacent rows, 8 values a lane and row, all loaded before the first is reduced. Rows behind a
+// sequence's end (up to the tile's) get no probability. HBM-bound: 512 bytes a row (26 us for 8190 x 40 rows at the
+// measured copy rate; 48 us with one row at a time).
+constexpr int kRowsEach = 4;
 __global__ void __launch_bounds__(256) attn_bwd_rows_kernel(const __grid_constant__ RowParams p) {
   pdl_trigger();
   const long long n = static_cast<long long>(p.b) * p.hq * p.rows;
-  const long long i = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) >> 4;
-  if (i >= n) return;  // n is a multiple of 128: whole warps leave
+  const long long i = ((static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) >> 4) * kRowsEach;
+  if (i >= n) return;  // n is a multiple of 128, so whole warps leave
   const int sub = threadIdx.x & 15;
-  const int row = static_cast<int>(i % p.rows);
+  const int row = static_cast<int>(i % p.rows);  // p.rows is a multiple of 128: the rows belong to one head
   const int h = static_cast<int>(i / p.rows % p.hq), seq = static_cast<int>(i / p.rows / p.hq), b = p.b0 + seq;
-  const bool in = row < (p.lens ? p.q_len[seq] : p.q_len[0]);
-  float acc = 0.f;
-  if (in) {
-    const uint4 x = *reinterpret_cast<const uint4*>(p.o + b * p.o_b + h * p.o_h + row * p.o_s + sub * 8);
-    const uint4 y = *reinterpret_cast<const uint4*>(p.d_o + b * p.do_b + h * p.do_h + row * p.do_s + sub * 8);
-    const __nv_bfloat162* a = reinterpret_cast<const __nv_bfloat162*>(&x);
-    const __nv_bfloat162* c = reinterpret_cast<const __nv_bfloat162*>(&y);
+  const int len = p.lens ? p.q_len[seq] : p.q_len[0];
+  const __nv_bfloat16* o = p.o + b * p.o_b + h * p.o_h + sub * 8;
+  const __nv_bfloat16* d = p.d_o + b * p.do_b + h * p.do_h + sub * 8;
+  uint4 x[kRowsEach], y[kRowsEach];
+#pragma unroll
+  for (int r = 0; r < kRowsEach; ++r) {
+    x[r] = y[r] = make_uint4(0, 0, 0, 0);
+    if (row + r < len) {
+      x[r] = *reinterpret_cast<const uint4*>(o + (row + r) * p.o_s);
+      y[r] = *reinterpret_cast<const uint4*>(d + (row + r) * p.do_s);
+    }
+  }
+  const long long bh = static_cast<long long>(b) * p.hq + h;
+  float mine = 0.f;  // lane r of the half keeps row r's sum
+#pragma unroll
+  for (int r = 0; r < kRowsEach; ++r) {
+    const __nv_bfloat162* a = reinterpret_cast<const __nv_bfloat162*>(&x[r]);
+    const __nv_bfloat162* c = reinterpret_cast<const __nv_bfloat162*>(&y[r]);
+    float acc = 0.f;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const float2 f = __bfloat1622float2(a[k]), g = __bfloat1622float2(c[k]);
       acc = fmaf(f.x, g.x, fmaf(f.y, g.y, acc));
     }
-  }
 #pragma unroll
-  for (int s = 8; s > 0; s >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, s);
-  if (sub == 0) {
-    const long long bh = static_cast<long long>(b) * p.hq + h;
-    const float none = p.scale > 0.f ? -kNoKeys : kNoKeys;
-    float l = none;
-    if (in) {
-      const float v = p.lse[(bh * 128 + (row & 127)) * p.groups + (row >> 7)];
+    for (int s = 8; s > 0; s >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, s);
+    if (sub == r) mine = acc;
+  }
+  if (sub < kRowsEach) {
+    const int mr = row + sub;
+    float l = p.scale > 0.f ? -kNoKeys : kNoKeys;
+    if (mr < len) {
+      const float v = p.lse[(bh * 128 + (mr & 127)) * p.groups + (mr >> 7)];
       if (!isinf(v)) l = -v / p.scale;
       if (fabsf(l) > kNoKeys) l = l > 0.f ? kNoKeys : -kNoKeys;
     }
-    p.stats[bh * p.rows + row] = stats_of(l, -acc);
+    p.stats[bh * p.rows + mr] = stats_of(l, -mine);
   }
 }
 
@@ -776,27 +791,36 @@ __global__ void __launch_bounds__(256) attn_bwd_join_kernel(const __grid_constan
 
 // ================================================================ host
 // How many CTA pairs share the walk of one dK/dV tile and of one dQ tile: the counts for which the launch is estimated to
-// end first. A pair takes 4 units a step (dkdv) or 3 (dq) and about 8 to start and finish; the pairs run on half as many
-// slots as there are SMs, and the last of the longest kind to start overhangs by half of its time on average. Joining
-// fp32 parts costs a launch, about 12 units. 1 and 1 where the tiles alone fill the device.
+// end first, in microseconds as measured at 1.7 GHz. A pair takes 1.5 us a step (dkdv) or 1.3 (dq) and 4 to start, fill and
+// end; the pairs run on half as many slots as there are SMs, dK/dV first. Joining fp32 parts costs a launch and their
+// traffic. 1 and 1 where the tiles alone fill the device (cross-attention of 8190 x 512 x 40 heads: 438 us with the 4
+// dkdv splits of a rule that looked at that kind alone, 372 without).
 constexpr int kMaxSplits = 16;
+struct Work {
+  long long k_outputs = 0, q_outputs = 0;  // tiles of 256 rows that have something to walk
+  int k_walk = 0, q_walk = 0;              // steps of the longest walk
+  long long k_steps = 0, q_steps = 0;      // of all walks
+  double k_bytes = 0, q_bytes = 0;         // of one part of dk and dv, of dq
+};
 bool even_split(int tiles, int s, int& per) {
   per = (tiles + s - 1) / s;
   return (tiles + per - 1) / per == s;  // no empty splits
 }
-void choose_splits(long long k_outputs, int k_walk, long long q_outputs, int q_walk, int& k_splits, int& q_splits) {
+void choose_splits(const Work& w, int& k_splits, int& q_splits) {
   const double slots = num_sms() / 2 > 0 ? num_sms() / 2 : 1;
-  double best = 0;
   k_splits = q_splits = 1;
-  for (int sk = 1; sk <= kMaxSplits && sk <= k_walk; ++sk) {
+  if (w.k_outputs + w.q_outputs > 16 * slots && w.k_outputs > slots) return;  // splits gain nothing there
+  const double k_step = 1.5, q_step = 1.3, fixed = 4;
+  double best = 0;
+  for (int sk = 1; sk <= kMaxSplits && sk <= w.k_walk; ++sk) {
     int k_per, q_per;
-    if (!even_split(k_walk, sk, k_per)) continue;
-    for (int sq = 1; sq <= kMaxSplits && sq <= q_walk; ++sq) {
-      if (!even_split(q_walk, sq, q_per)) continue;
-      const double k_len = 4.0 * k_per + 8, q_len = 3.0 * q_per + 8;
-      const double work = k_outputs * sk * k_len + q_outputs * sq * q_len;
-      const double longest = std::max(k_len, q_len);
-      const double cost = std::max(work / slots + longest / 2, longest) + (sk > 1 || sq > 1 ? 12 : 0);
+    if (!even_split(w.k_walk, sk, k_per)) continue;
+    for (int sq = 1; sq <= kMaxSplits && sq <= w.q_walk; ++sq) {
+      if (!even_split(w.q_walk, sq, q_per)) continue;
+      const double k_len = k_step * k_per + fixed, q_len = q_step * q_per + fixed;
+      const double work = k_step * w.k_steps + q_step * w.q_steps + fixed * (w.k_outputs * sk + w.q_outputs * sq);
+      double cost = std::max(work / slots + q_len / 2, std::max(k_len, q_len));
+      if (sk > 1 || sq > 1) cost += 3 + 2e-6 / 6.5 * ((sk > 1 ? sk * w.k_bytes : 0) + (sq > 1 ? sq * w.q_bytes : 0));
       if (best == 0 || cost < best * 0.98) {
         best = cost;
         k_splits = sk;
@@ -812,15 +836,28 @@ struct Plan {
   size_t row_bytes, q_bytes, k_bytes;    // stats; dq's parts; dk's parts, and dv's
   size_t bytes() const { return row_bytes + q_bytes + 2 * k_bytes; }
 };
-Plan plan_of(int b, int s_q, int s_kv, int hq, int hkv) {
+// q_lens, kv_lens: null for whole rows.
+Plan plan_of(int b, int s_q, int s_kv, int hq, int hkv, const int* q_lens, const int* kv_lens) {
   Plan p;
-  const int q_tiles = (s_q + kTile - 1) / kTile, k_tiles = (s_kv + kTile - 1) / kTile;
-  p.rows = q_tiles * kTile;
-  const int walk = q_tiles * (hq / hkv);
-  choose_splits(static_cast<long long>(b) * hkv * ((k_tiles + 1) / 2), walk, static_cast<long long>(b) * hq * ((q_tiles + 1) / 2),
-                k_tiles, p.k_splits, p.q_splits);
-  p.q_per = (k_tiles + p.q_splits - 1) / p.q_splits;
-  p.k_per = (walk + p.k_splits - 1) / p.k_splits;
+  Work w;
+  const int group = hq / hkv, n = q_lens || kv_lens ? b : 1, times = n == 1 ? b : 1;
+  for (int i = 0; i < n; ++i) {
+    const long long qt = ((q_lens ? q_lens[i] : s_q) + kTile - 1) / kTile, kt = ((kv_lens ? kv_lens[i] : s_kv) + kTile - 1) / kTile;
+    if (qt == 0 || kt == 0) continue;
+    const long long k_out = times * hkv * ((kt + 1) / 2), q_out = times * hq * ((qt + 1) / 2);
+    w.k_outputs += k_out;
+    w.q_outputs += q_out;
+    w.k_steps += k_out * qt * group;
+    w.q_steps += q_out * kt;
+    w.k_walk = std::max<int>(w.k_walk, static_cast<int>(qt * group));
+    w.q_walk = std::max<int>(w.q_walk, static_cast<int>(kt));
+  }
+  w.k_bytes = 8.0 * b * s_kv * hkv * kD;
+  w.q_bytes = 4.0 * b * s_q * hq * kD;
+  p.rows = (s_q + kTile - 1) / kTile * kTile;
+  choose_splits(w, p.k_splits, p.q_splits);
+  p.q_per = std::max(1, (w.q_walk + p.q_splits - 1) / p.q_splits);
+  p.k_per = std::max(1, (w.k_walk + p.k_splits - 1) / p.k_splits);
   p.row_bytes = align_up(static_cast<size_t>(b) * hq * p.rows * sizeof(uint4), 256);
   p.q_bytes = p.q_splits > 1 ? static_cast<size_t>(p.q_splits) * b * s_q * hq * kD * 4 : 0;
   p.k_bytes = p.k_splits > 1 ? static_cast<size_t>(p.k_splits) * b * s_kv * hkv * kD * 4 : 0;
@@ -851,10 +888,16 @@ int make_maps(CUtensorMap* q, CUtensorMap* k, CUtensorMap* v, CUtensorMap* o, co
 
 using namespace vomni;
 
-extern "C" size_t vomni_attention_bwd_workspace_bytes(int b, int s_q, int s_kv, int hq, int hkv, int d) {
-  if (abwd::bad_shape(b, s_q, s_kv, hq, hkv, d)) return 0;
-  const abwd::Plan p = abwd::plan_of(b, s_q, s_kv, hq, hkv);
-  return p.bytes();
+static bool bad_lens(int b, int s_q, int s_kv, const int* q_lens, const int* kv_lens) {
+  for (int i = 0; i < b; ++i)
+    if ((q_lens && (q_lens[i] < 0 || q_lens[i] > s_q)) || (kv_lens && (kv_lens[i] < 0 || kv_lens[i] > s_kv))) return true;
+  return false;
+}
+
+extern "C" size_t vomni_attention_bwd_workspace_bytes(int b, int s_q, int s_kv, int hq, int hkv, int d, const int* q_lens,
+                                                      const int* kv_lens) {
+  if (abwd::bad_shape(b, s_q, s_kv, hq, hkv, d) || bad_lens(b, s_q, s_kv, q_lens, kv_lens)) return 0;
+  return abwd::plan_of(b, s_q, s_kv, hq, hkv, q_lens, kv_lens).bytes();
 }
 
 // Launches the pairs of batch elements [p.b0, p.b0 + n) with their maps, as a dependent of the stats' launch.
@@ -891,16 +934,14 @@ extern "C" int vomni_attention_bwd(const void* grad_o, const void* q, const void
   if (!grad_o || !q || !k || !v || !o || !lse || !strides || !dq || !dk || !dv || !workspace) return VOMNI_EINVAL;
   if (!(std::fabs(softmax_scale) >= 1e-20f && std::fabs(softmax_scale) <= 1e20f)) return VOMNI_EINVAL;
   if (bad_shape(b, s_q, s_kv, hq, hkv, d)) return VOMNI_EBADSHAPE;
-  for (int i = 0; i < b; ++i)
-    if ((q_lens && (q_lens[i] < 0 || q_lens[i] > s_q)) || (kv_lens && (kv_lens[i] < 0 || kv_lens[i] > s_kv)))
-      return VOMNI_EBADSHAPE;
+  if (bad_lens(b, s_q, s_kv, q_lens, kv_lens)) return VOMNI_EBADSHAPE;
   const uintptr_t al = reinterpret_cast<uintptr_t>(grad_o) | reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) |
                        reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(o) | reinterpret_cast<uintptr_t>(dq) |
                        reinterpret_cast<uintptr_t>(dk) | reinterpret_cast<uintptr_t>(dv) |
                        reinterpret_cast<uintptr_t>(workspace);
   if (al & 15) return VOMNI_EALIGN;
   if (reinterpret_cast<uintptr_t>(lse) & 3) return VOMNI_EALIGN;
-  const Plan plan = plan_of(b, s_q, s_kv, hq, hkv);
+  const Plan plan = plan_of(b, s_q, s_kv, hq, hkv, q_lens, kv_lens);
   if (workspace_bytes < plan.bytes()) return VOMNI_EWORKSPACE;
   // strides: (row, head, batch) of q, k, v, grad_o, o in elements, multiples of 8 where the extent is over 1
   long long st4[4][3], so[3];
@@ -968,7 +1009,7 @@ extern "C" int vomni_attention_bwd(const void* grad_o, const void* q, const void
     r.b0 = b0;
     r.scale = softmax_scale;
     r.stats = const_cast<uint4*>(p.stats);
-    const long long blocks = (static_cast<long long>(n) * hq * plan.rows * 16 + 255) / 256;
+    const long long blocks = (static_cast<long long>(n) * hq * plan.rows / kRowsEach * 16 + 255) / 256;
     if (blocks > 0x7fffffffll) return VOMNI_EBADSHAPE;
     attn_bwd_rows_kernel<<<static_cast<unsigned>(blocks), 256, 0, st>>>(r);
     VOMNI_CUDA_TRY(cudaGetLastError());

@@ -570,41 +570,44 @@ struct SumParams {
   float *dgate, *dpost_w, *dmul, *dadd;
 };
 
-// 32 columns x 8 lanes a CTA; blockIdx.y: A, M or D. Sums each modulation row's parts in the order
-// lane, lane + 8, ..., then the 8 lanes in order, and forms the outputs; those shared by the
-// modulation rows are added over them in order.
-__global__ void __launch_bounds__(256) sandwich_sum_kernel(const SumParams p) {
-  __shared__ float red[8][32];
+// 32 columns x 32 lanes a CTA; blockIdx.y: A, M or D. Sums each modulation row's parts in the order lane, lane + 32, ...,
+// then the 32 lanes as a tree, and forms the outputs; those shared by the modulation rows are added over them in order.
+// (With 8 lanes it took 13 us for 334 parts of 1536 columns, more than the kernel before it.)
+__global__ void __launch_bounds__(1024) sandwich_sum_kernel(const __grid_constant__ SumParams p) {
+  __shared__ float red[32][33];
   const int col = blockIdx.x * 32 + threadIdx.x, q = blockIdx.y;
   const bool in = col < p.H;
-  float shared_out = 0.f, dw = 0.f;
   float* out = q == 0 ? p.dgate : q == 1 ? p.dmul : p.dadd;
   const bool per = p.per & (q == 0 ? kPerGate : q == 1 ? kPerMul : kPerAdd);
   if (!out && !(q == 0 && p.dpost_w)) return;
+  float shared_out = 0.f, dw = 0.f;
+  const int mine = blockIdx.x * 32 + threadIdx.y;  // the column whose lanes this warp adds
   for (int mod = 0; mod < p.n_mod; ++mod) {
     float s = 0.f;
-    if (in)
-      for (int l = threadIdx.y; l < p.lanes; l += 8)
-        s += p.parts[((static_cast<long long>(mod) * p.lanes + l) * 3 + q) * p.H + col];
+    if (in) {
+      const float* at = p.parts + (static_cast<long long>(mod) * p.lanes * 3 + q) * p.H + col;
+#pragma unroll 4
+      for (int l = threadIdx.y; l < p.lanes; l += 32) s += at[static_cast<long long>(l) * 3 * p.H];
+    }
     red[threadIdx.y][threadIdx.x] = s;
     __syncthreads();
-    if (threadIdx.y == 0 && in) {
-      float t = 0.f;
+    float t = red[threadIdx.x][threadIdx.y];
 #pragma unroll
-      for (int l = 0; l < 8; ++l) t += red[l][threadIdx.x];
-      if (q == 0 && p.dpost_w) dw = fmaf(t, p.gate ? p.gate[mod * p.gate_step + col] : 1.f, dw);
-      if (q == 0 && p.post_w) t *= p.post_w[col];
+    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+    if (threadIdx.x == 0 && mine < p.H) {
+      if (q == 0 && p.dpost_w) dw = fmaf(t, p.gate ? p.gate[mod * p.gate_step + mine] : 1.f, dw);
+      if (q == 0 && p.post_w) t *= p.post_w[mine];
       if (per) {
-        if (out) out[static_cast<long long>(mod) * p.H + col] = t;
+        if (out) out[static_cast<long long>(mod) * p.H + mine] = t;
       } else {
         shared_out += t;
       }
     }
     __syncthreads();
   }
-  if (threadIdx.y == 0 && in) {
-    if (out && !per) out[col] = shared_out;
-    if (q == 0 && p.dpost_w) p.dpost_w[col] = dw;
+  if (threadIdx.x == 0 && mine < p.H) {
+    if (out && !per) out[mine] = shared_out;
+    if (q == 0 && p.dpost_w) p.dpost_w[mine] = dw;
   }
 }
 
@@ -810,7 +813,7 @@ extern "C" int vomni_sandwich_norm_bwd(const void* grad_residual_out, const void
   s.dpost_w = dpost_weight;
   s.dmul = dmul;
   s.dadd = dadd;
-  sandwich_sum_kernel<<<dim3((h + 31) / 32, 3), dim3(32, 8), 0, st>>>(s);
+  sandwich_sum_kernel<<<dim3((h + 31) / 32, 3), dim3(32, 32), 0, st>>>(s);
   VOMNI_CUDA_TRY(cudaGetLastError());
   return VOMNI_OK;
 }
