@@ -161,6 +161,32 @@ def test_more_sequences_than_one_launch_holds(pkg, dev):
     _check(got, *want)
 
 
+@pytest.mark.parametrize("sq,skv,hq,hkv,q_lens,kv_lens", [
+    (7700, 200, 22, 11, None, None),  # 31 tiles of 256 queries a head: several a CTA pair, the last group short
+    (8190, 512, 40, 40, None, None),
+    (5000, 250, 20, 20, [5000, 1300, 0], [250, 100, 250]),  # walks of two steps, of one, of none
+])
+def test_short_walks(pkg, dev, sq, skv, hq, hkv, q_lens, kv_lens):
+    """Many queries, few keys: a pair takes several query tiles one after the other."""
+    b = len(q_lens) if q_lens else 1
+    q, k, v, go = _inputs(dev, b, sq, skv, hq, hkv, 22)
+    sc = 1 / math.sqrt(128)
+    o = torch.zeros(b, hq, sq, 128, dtype=torch.bfloat16, device=dev)
+    lse = torch.full((b, hq, sq), -math.inf, device=dev, dtype=torch.float64)
+    g = hq // hkv
+    for h in range(hkv):  # the reference head by head
+        oo, ll = _forward(q[:, :, h * g:(h + 1) * g], k[:, :, h:h + 1], v[:, :, h:h + 1], sc, q_lens, kv_lens)
+        o[:, h * g:(h + 1) * g], lse[:, h * g:(h + 1) * g] = oo.to(torch.bfloat16), ll
+    got = pkg.attention_bwd(go, q, k, v, o, _lse_layout(lse), q_lens=q_lens, kv_lens=kv_lens)
+    torch.cuda.synchronize()
+    assert _status() == 0
+    for h in range(hkv):
+        part = [t[:, :, h * g:(h + 1) * g] if i == 0 else t[:, :, h:h + 1] for i, t in enumerate(got)]
+        want, bound = _grads(q[:, :, h * g:(h + 1) * g], k[:, :, h:h + 1], v[:, :, h:h + 1], o[:, h * g:(h + 1) * g],
+                             lse[:, h * g:(h + 1) * g].float(), go[:, h * g:(h + 1) * g], sc, q_lens, kv_lens)
+        _check([t.contiguous() for t in part], want, bound, f"head {h}")
+
+
 def test_rows_without_probabilities(pkg, dev):
     q, k, v, go = _inputs(dev, 1, 150, 150, 1, 1, 13)
     sc = 1 / math.sqrt(128)

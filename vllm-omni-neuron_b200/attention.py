@@ -387,17 +387,16 @@ def attention_bwd(grad_o: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: tor
     dev = _lib.one_device(grad_o, q, k, v, o, lse)
     scale = 1.0 / math.sqrt(_HEAD_DIM) if softmax_scale is None else float(softmax_scale)
     empty = not (b and sq and skv and hq)
-    make = torch.zeros if empty else torch.empty
-    dq, dk, dv = (make(t.shape, dtype=torch.bfloat16, device=q.device) for t in (q, k, v))
     if empty:
-        return dq, dk, dv
+        return tuple(t.new_zeros(t.shape) for t in (q, k, v))
+    dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
     src = (_any_strides(q), _any_strides(k), _any_strides(v), _any_strides(grad_o, True), _any_strides(o, True))
     strides = (ctypes.c_longlong * 15)(*(n for _, st in src for n in st))
     q, k, v, grad_o, o = (t for t, _ in src)
     lse = _lib.dense(lse if lse.dtype == torch.float32 else lse.float())
     q_lens, kv_lens = ((ctypes.c_int * b)(*lens) if lens is not None else None for lens in (q_lens, kv_lens))
     ws_bytes = _lib.on_device(dev, _lib.load().vomni_attention_bwd_workspace_bytes, b, sq, skv, hq, hkv, _HEAD_DIM, q_lens, kv_lens)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+    ws = q.new_empty(ws_bytes, dtype=torch.uint8)
     _lib.launch(dev, "vomni_attention_bwd", grad_o.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
                 lse.data_ptr(), b, sq, skv, hq, hkv, _HEAD_DIM, strides, q_lens, kv_lens, scale, dq.data_ptr(),
                 dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), ws_bytes)

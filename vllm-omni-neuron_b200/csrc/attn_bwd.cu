@@ -81,7 +81,7 @@ struct Params {
 };
 
 // Device status sites (VOMNI_DEV_TIMEOUT_BASE + site).
-enum Site : int { kSiteProducer = 0x40, kSiteMma = 0x41, kSiteScores = 0x42, kSiteOut = 0x43, kSiteDrain = 0x44 };
+enum Site : int { kSiteProducer = 0x10, kSiteMma = 0x11, kSiteScores = 0x12, kSiteOut = 0x13, kSiteDrain = 0x14 };
 
 // mbar_wait whose thread is suspended for 40 ns at a time at most (without the hint it wakes some hundred clocks late), and
 // looks at the abort flag and the clock once in 64 polls.

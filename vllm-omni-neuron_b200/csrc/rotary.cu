@@ -17,6 +17,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <type_traits>
 
@@ -227,6 +228,39 @@ int check_tensor(const void* x, const void* y, int heads, long long row_stride, 
   return VOMNI_OK;
 }
 
+// The pairs' axes and frequencies. A thread keeps the last ones it formed: a model asks for the same every time, and the
+// powers take some microseconds.
+struct Frequencies {
+  int d = 0, n_axes = 0, dims[kMaxAxes] = {};
+  double theta = 0.0;
+  unsigned char axis[kMaxDim / 2];
+  double turns[kMaxDim / 2];
+};
+int frequencies(Params& p, int n_axes, const int* dims, int d, double theta) {
+  static thread_local Frequencies f;
+  bool same = f.d == d && f.n_axes == n_axes && f.theta == theta;
+  for (int a = 0; same && a < n_axes; ++a) same = f.dims[a] == dims[a];
+  if (!same) {
+    f.d = 0;  // until it is whole
+    int pair = 0;
+    for (int a = 0; a < n_axes; ++a) {
+      if (dims[a] <= 0 || dims[a] % 2 || pair + dims[a] / 2 > d / 2) return VOMNI_EBADSHAPE;
+      for (int i = 0; i < dims[a] / 2; ++i, ++pair) {
+        f.axis[pair] = static_cast<unsigned char>(a);
+        f.turns[pair] = std::pow(theta, -2.0 * i / dims[a]) / 6.283185307179586476925286766559;
+      }
+      f.dims[a] = dims[a];
+    }
+    if (pair != d / 2) return VOMNI_EBADSHAPE;
+    f.n_axes = n_axes;
+    f.theta = theta;
+    f.d = d;
+  }
+  std::copy(f.axis, f.axis + d / 2, p.axis);
+  std::copy(f.turns, f.turns + d / 2, p.turns);
+  return VOMNI_OK;
+}
+
 }  // namespace rotary
 }  // namespace vomni
 
@@ -250,16 +284,9 @@ extern "C" int vomni_rotary_axes(const void* q, void* q_out, int q_heads, long l
   if (rc) return rc;
   if (q_heads + k_heads == 0) return VOMNI_EBADSHAPE;
   if (reinterpret_cast<uintptr_t>(positions) & (pos_type == 1 ? 7 : 3)) return VOMNI_EALIGN;
-  rotary::Params p = {};
-  int pair = 0;
-  for (int a = 0; a < n_axes; ++a) {
-    if (axes_dims[a] <= 0 || axes_dims[a] % 2 || pair + axes_dims[a] / 2 > d / 2) return VOMNI_EBADSHAPE;
-    for (int i = 0; i < axes_dims[a] / 2; ++i, ++pair) {
-      p.axis[pair] = static_cast<unsigned char>(a);
-      p.turns[pair] = std::pow(theta, -2.0 * i / axes_dims[a]) / 6.283185307179586476925286766559;
-    }
-  }
-  if (pair != d / 2) return VOMNI_EBADSHAPE;
+  rotary::Params p;
+  rc = rotary::frequencies(p, n_axes, axes_dims, d, theta);
+  if (rc) return rc;
   rc = require_sm100();
   if (rc) return rc;
   p.t[0] = {q, q_out, q_heads, q_row_stride, q_batch_stride};

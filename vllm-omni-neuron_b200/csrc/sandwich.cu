@@ -175,7 +175,7 @@ VOMNI_DEV void normalise(Vals<R, C>& x, int kind, const bool (&in)[C / 8], const
 // A CTA's rows come R at a time (adjacent rows: one bulk copy per tensor) through a ring of `slots` slots; one thread
 // issues the copies, slots - 1 groups ahead.
 constexpr int kMaxSlots = 4;
-constexpr int kSiteRowWait = 0x48, kSiteRowDrain = 0x49;
+constexpr int kSiteRowWait = 0x18, kSiteRowDrain = 0x19;
 
 struct Ring {
   uint4* mem;  // [slots][tensors][R * H / 8]

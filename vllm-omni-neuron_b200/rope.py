@@ -121,11 +121,11 @@ def _rotary(q, k, positions, axes_dims, theta, pairing, inverse):
     outs, args, keep = [], [], []
     for t in (q, k):
         if t is None or t.numel() == 0:
-            outs.append(None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device))
+            outs.append(None if t is None else t.new_empty(t.shape))
             args += (None, None, 0, 0, 0)
             continue
         src, row, batch = _rotary_source(t)
-        out = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+        out = t.new_empty(t.shape)
         keep.append(src)
         outs.append(out)
         args += (src.data_ptr(), out.data_ptr(), t.shape[2], row, batch)

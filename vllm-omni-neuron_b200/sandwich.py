@@ -99,8 +99,8 @@ def _forward(x, residual, gate, mul, add, post_weight, eps, post_norm, norm_type
     dev = _lib.one_device(x, residual, gate, mul, add, post_weight)
     x = None if x is None else _rows("x", x, residual.shape)
     residual = _rows("residual", residual, residual.shape)
-    res_out = None if x is None else torch.empty_like(residual)
-    out = torch.empty_like(residual)
+    res_out = None if x is None else residual.new_empty(residual.shape)
+    out = residual.new_empty(residual.shape)
     if rows:
         _lib.launch(dev, "vomni_sandwich_norm", _ptr(x), residual.data_ptr(), _ptr(v["gate"]), _ptr(v["post_weight"]), _ptr(v["mul"]),
                     _ptr(v["add"]), rows, hidden, per_mod, bits, eps, _NORMS[post_norm], _NORMS[norm_type], _ptr(res_out),
@@ -117,13 +117,13 @@ def _backward(grad_res, grad_out, x, residual_out, gate, mul, add, post_weight, 
     grad_out = None if grad_out is None else _rows("grad_out", grad_out, shape)
     x = None if x is None else _rows("x", x, shape)
     residual_out = _rows("residual_out", residual_out, shape)
-    dx = None if x is None else torch.empty_like(x)
-    dres = torch.empty_like(residual_out)
-    make = torch.empty if rows else torch.zeros
-    sums = {n: make(t.shape, dtype=torch.float32, device=residual_out.device) if t is not None and need[n] else None for n, t in vectors.items()}
+    dx = None if x is None else x.new_empty(shape)
+    dres = residual_out.new_empty(shape)
+    make = residual_out.new_empty if rows else residual_out.new_zeros
+    sums = {n: make(t.shape, dtype=torch.float32) if t is not None and need[n] else None for n, t in vectors.items()}
     if rows:
         ws_bytes = _lib.on_device(dev, _lib.load().vomni_sandwich_norm_workspace_bytes, rows, hidden, per_mod)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=residual_out.device)
+        ws = residual_out.new_empty(ws_bytes, dtype=torch.uint8)
         _lib.launch(dev, "vomni_sandwich_norm_bwd", _ptr(grad_res), _ptr(grad_out), _ptr(x), residual_out.data_ptr(), _ptr(v["gate"]),
                     _ptr(v["post_weight"]), _ptr(v["mul"]), rows, hidden, per_mod, bits, eps, _NORMS[post_norm], _NORMS[norm_type],
                     _ptr(dx), dres.data_ptr(), _ptr(sums["gate"]), _ptr(sums["post_weight"]), _ptr(sums["mul"]), _ptr(sums["add"]),
