@@ -18,6 +18,11 @@ output shapes and dtypes, so a traced or compiled caller sees one opaque node pe
 ``b200omni::row_mx_qkv_proj``          FP8 QKV projection (+ across-heads norm, rotate-half RoPE)
 ``b200omni::row_mx_mlp``               FP8 FFN leaf
 ``b200omni::cfg_combine``              CFG combine of two gathered branch outputs
+``b200omni::attention_fwd``            attention with its log-sum-exp (``attention_fwd``); differentiable
+``b200omni::attention_bwd``            its gradients
+``b200omni::rotary_axes``              rotary positions with several axes; differentiable
+``b200omni::sandwich_norm``            norms around a block with its gate and residual; differentiable
+``b200omni::sandwich_norm_bwd``        its gradients
 =====================================  =====================================================
 
 Importing this module registers the operators once; the package imports it.
@@ -30,6 +35,8 @@ import math
 import torch
 
 from .adaln import adaln_modulate as _adaln
+from .attention import attention_bwd as _attention_bwd
+from .attention import attention_fwd as _attention_fwd
 from .attention import ring_attention_const_max_fwd as _ring_fwd
 from .block import cross_attention as _cross
 from .cfg import cfg_combine as _cfg_combine
@@ -37,6 +44,9 @@ from .ffn import row_mx_mlp as _row_mx_mlp
 from .ffn import wan_mlp as _wan_mlp
 from .oproj import wan_o_proj as _wan_o_proj
 from .qkv import row_mx_qkv_proj as _qkv
+from .rope import rotary_axes as _rotary_axes
+from .sandwich import sandwich_norm as _sandwich_norm
+from .sandwich import sandwich_norm_bwd as _sandwich_norm_bwd
 
 NS = "b200omni"
 
@@ -207,3 +217,144 @@ def cfg_combine(positive: torch.Tensor, negative: torch.Tensor, true_cfg_scale: 
 @cfg_combine.register_fake
 def _(positive, negative, true_cfg_scale):
     return torch.empty_like(positive)
+
+
+# ---------------------------------------------------------------- training: attention
+
+
+def _of_call(ctx, grads):
+    """The gradients of the arguments that the call gave (arguments left at their defaults take none)."""
+    return tuple(grads[: len(ctx.needs_input_grad)])
+
+
+@torch.library.custom_op(f"{NS}::attention_fwd", mutates_args=())
+def attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, softmax_scale: float | None = None,
+                  q_lens: list[int] | None = None, kv_lens: list[int] | None = None) -> list[torch.Tensor]:
+    """``[o, lse]`` of :func:`attention_fwd`; differentiable through ``o``."""
+    return list(_attention_fwd(q, k, v, softmax_scale, q_lens=q_lens, kv_lens=kv_lens))
+
+
+@attention_fwd.register_fake
+def _(q, k, v, softmax_scale=None, q_lens=None, kv_lens=None):
+    b, s, h, d = q.shape
+    return [q.new_empty((b, h, s, d), dtype=torch.bfloat16), q.new_empty((b, h, 128, (s + 127) // 128), dtype=torch.float32)]
+
+
+@torch.library.custom_op(f"{NS}::attention_bwd", mutates_args=())
+def attention_bwd(grad_o: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, lse: torch.Tensor,
+                  softmax_scale: float | None = None, q_lens: list[int] | None = None,
+                  kv_lens: list[int] | None = None) -> list[torch.Tensor]:
+    """``[dq, dk, dv]`` of :func:`attention_bwd`."""
+    return list(_attention_bwd(grad_o, q, k, v, o, lse, softmax_scale, q_lens=q_lens, kv_lens=kv_lens))
+
+
+@attention_bwd.register_fake
+def _(grad_o, q, k, v, o, lse, softmax_scale=None, q_lens=None, kv_lens=None):
+    return [t.new_empty(tuple(t.shape), dtype=torch.bfloat16) for t in (q, k, v)]
+
+
+def _attention_setup(ctx, inputs, output):
+    q, k, v, scale, q_lens, kv_lens = inputs
+    ctx.save_for_backward(q, k, v, *output)
+    ctx.rest = (scale, q_lens, kv_lens)
+
+
+def _attention_grad(ctx, grads):
+    if grads[0] is None:
+        return _of_call(ctx, (None,) * 6)
+    q, k, v, o, lse = ctx.saved_tensors
+    return _of_call(ctx, (*torch.ops.b200omni.attention_bwd(grads[0], q, k, v, o, lse, *ctx.rest), None, None, None))
+
+
+attention_fwd.register_autograd(_attention_grad, setup_context=_attention_setup)
+
+
+# ---------------------------------------------------------------- training: rotary positions
+
+
+@torch.library.custom_op(f"{NS}::rotary_axes", mutates_args=())
+def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, axes_dims: list[int], theta: float = 10000.0,
+                pairing: str = "interleaved", inverse: bool = False) -> list[torch.Tensor]:
+    """``[q', k']`` (``[q']`` without ``k``) of :func:`rotary_axes`."""
+    out = _rotary_axes(q, k, positions, axes_dims, theta=theta, pairing=pairing, inverse=inverse)
+    return [out] if k is None else list(out)
+
+
+@rotary_axes.register_fake
+def _(q, k, positions, axes_dims, theta=10000.0, pairing="interleaved", inverse=False):
+    return [t.new_empty(tuple(t.shape)) for t in (q, k) if t is not None]
+
+
+def _rotary_setup(ctx, inputs, output):
+    _, k, positions, axes_dims, theta, pairing, inverse = inputs
+    ctx.save_for_backward(positions)
+    ctx.rest = (axes_dims, theta, pairing, not inverse)
+    ctx.two = k is not None
+
+
+def _rotary_grad(ctx, grads):
+    (positions,) = ctx.saved_tensors
+    first = grads[0] if grads[0] is not None else grads[1]
+    both = ctx.two and grads[0] is not None and grads[1] is not None
+    out = torch.ops.b200omni.rotary_axes(first, grads[1] if both else None, positions, *ctx.rest)
+    dq = out[0] if grads[0] is not None else None
+    dk = out[-1] if ctx.two and grads[1] is not None else None
+    return _of_call(ctx, (dq, dk, None, None, None, None, None))
+
+
+rotary_axes.register_autograd(_rotary_grad, setup_context=_rotary_setup)
+
+
+# ---------------------------------------------------------------- training: norms around a block
+
+
+@torch.library.custom_op(f"{NS}::sandwich_norm", mutates_args=())
+def sandwich_norm(x: torch.Tensor | None, residual: torch.Tensor, gate: torch.Tensor | None, mul: torch.Tensor | None,
+                  add: torch.Tensor | None, eps: float, post_norm: str = "rms_norm", post_weight: torch.Tensor | None = None,
+                  norm_type: str = "layer_norm") -> list[torch.Tensor]:
+    """``[residual_out, out]`` of :func:`sandwich_norm` (``[out]`` without ``x``, whose residual_out is ``residual``)."""
+    res, out = _sandwich_norm(x, residual, gate, mul, add, eps=eps, post_norm=post_norm, post_weight=post_weight, norm_type=norm_type)
+    return [out] if x is None else [res, out]
+
+
+@sandwich_norm.register_fake
+def _(x, residual, gate, mul, add, eps, post_norm="rms_norm", post_weight=None, norm_type="layer_norm"):
+    return [residual.new_empty(tuple(residual.shape)) for _ in range(1 if x is None else 2)]
+
+
+@torch.library.custom_op(f"{NS}::sandwich_norm_bwd", mutates_args=())
+def sandwich_norm_bwd(grad_residual_out: torch.Tensor | None, grad_out: torch.Tensor | None, x: torch.Tensor | None,
+                      residual_out: torch.Tensor, gate: torch.Tensor | None, mul: torch.Tensor | None, add: torch.Tensor | None,
+                      eps: float, post_norm: str = "rms_norm", post_weight: torch.Tensor | None = None,
+                      norm_type: str = "layer_norm") -> list[torch.Tensor]:
+    """The gradients of :func:`sandwich_norm_bwd` of the tensors that are given, in the order x, residual, gate, mul, add,
+    post_weight."""
+    g = _sandwich_norm_bwd(grad_residual_out, grad_out, x, residual_out, gate, mul, add, eps=eps, post_norm=post_norm,
+                           post_weight=post_weight, norm_type=norm_type)
+    return [t for t in g if t is not None]
+
+
+@sandwich_norm_bwd.register_fake
+def _(grad_residual_out, grad_out, x, residual_out, gate, mul, add, eps, post_norm="rms_norm", post_weight=None,
+      norm_type="layer_norm"):
+    return [t.new_empty(tuple(t.shape)) for t in (x, residual_out, gate, mul, add, post_weight) if t is not None]
+
+
+def _sandwich_setup(ctx, inputs, output):
+    x, residual, gate, mul, add, eps, post_norm, post_weight, norm_type = inputs
+    ctx.save_for_backward(x, residual if x is None else output[0], gate, mul, add, post_weight)
+    ctx.rest = (eps, post_norm, norm_type)
+
+
+def _sandwich_grad(ctx, grads):
+    x, res, gate, mul, add, post_weight = ctx.saved_tensors
+    eps, post_norm, norm_type = ctx.rest
+    grad_res, grad_out = (None, grads[0]) if x is None else grads
+    if grad_res is None and grad_out is None:
+        return _of_call(ctx, (None,) * 9)
+    out = iter(torch.ops.b200omni.sandwich_norm_bwd(grad_res, grad_out, x, res, gate, mul, add, eps, post_norm, post_weight, norm_type))
+    dx, dres, dgate, dmul, dadd, dw = (next(out) if t is not None else None for t in (x, res, gate, mul, add, post_weight))
+    return _of_call(ctx, (dx, dres, dgate, dmul, dadd, None, None, dw, None))
+
+
+sandwich_norm.register_autograd(_sandwich_grad, setup_context=_sandwich_setup)
