@@ -46,6 +46,13 @@ def test_attention(pkg):
         bwd(kv_lens=[-1, 3])
     with pytest.raises(TypeError):  # a device tensor of lengths would need a synchronisation
         bwd(kv_lens=torch.tensor([3, 4]))
+    for bad in (0.0, float("nan"), float("inf")):
+        with pytest.raises(ValueError):
+            pkg.attention_bwd(o, q, q, q, o, lse, bad)
+        with pytest.raises(ValueError):
+            pkg.attention_fwd(q, q, q, bad)
+    with pytest.raises(ValueError):  # the softmax bound is a norm: positive scales only
+        pkg.wan_attention(q, q, q, -0.1)
     with pytest.raises(RuntimeError):
         pkg.attention_fwd(q, q, q)
     with pytest.raises(RuntimeError):
@@ -103,6 +110,12 @@ def test_sandwich(pkg):
     for bad in (_bf(2, 8, 12), _bf(1, 8200), _bf(64)):
         with pytest.raises(ValueError):
             pkg.sandwich_norm(bad, bad, eps=1e-6)
+    for eps in (0.0, -1e-6, float("nan"), float("inf")):
+        with pytest.raises(ValueError):
+            pkg.sandwich_norm(x, x, eps=eps)
+    many = _bf(70000, 1, 8)
+    with pytest.raises(ValueError):
+        pkg.sandwich_norm(many, many, torch.zeros(70000, 1, 8), eps=1e-6)
     with pytest.raises(ValueError):
         pkg.sandwich_norm_bwd(None, None, x, x, eps=1e-6)
 
@@ -112,12 +125,12 @@ def test_c_entries(lib):
     p, odd = ctypes.c_void_p(256), ctypes.c_void_p(258)
     ok = (ctypes.c_longlong * 15)(*([512, 128, 512 * 16] * 5))
 
-    def bwd(b=2, sq=16, skv=16, hq=4, hkv=4, d=128, strides=ok, ql=None, kl=None, ws=1 << 40, dq=p, q=p):
+    def bwd(b=2, sq=16, skv=16, hq=4, hkv=4, d=128, strides=ok, ql=None, kl=None, ws=1 << 40, dq=p, q=p, scale=0.1):
         ints = lambda v: (ctypes.c_int * len(v))(*v) if v else None
-        return lib.vomni_attention_bwd(p, q, p, p, p, p, b, sq, skv, hq, hkv, d, strides, ints(ql), ints(kl), 0.1, dq, p, p, p, ws,
+        return lib.vomni_attention_bwd(p, q, p, p, p, p, b, sq, skv, hq, hkv, d, strides, ints(ql), ints(kl), scale, dq, p, p, p, ws,
                                        None)
 
-    assert bwd(dq=None) == 1
+    assert bwd(dq=None) == 1 and bwd(scale=0.0) == 1 and bwd(scale=float("nan")) == 1 and bwd(scale=1e30) == 1
     assert bwd(d=64) == 2 and bwd(hkv=3) == 2 and bwd(sq=0) == 2 and bwd(b=5000) == 2
     assert bwd(ql=[17, 1]) == 2 and bwd(kl=[-1, 1]) == 2
     assert bwd(q=odd) == 3
@@ -144,6 +157,7 @@ def test_c_entries(lib):
 
     assert norm(res=None) == 1 and norm(r=None) == 1 and norm(bits=8) == 1 and norm(post=3) == 1 and norm(kind=-1) == 1
     assert norm(x=None, gate=p) == 1
+    assert norm(rows=70000, per=1) == 2
     assert norm(h=12) == 2 and norm(h=8200) == 2 and norm(rows=0) == 2 and norm(per=3) == 2
     assert norm(x=odd) == 3
 

@@ -285,6 +285,13 @@ def _lens(name: str, lens, b: int, s: int):
     return lens
 
 
+def _training_scale(softmax_scale, signed: bool = False) -> float:
+    scale = 1.0 / math.sqrt(_HEAD_DIM) if softmax_scale is None else float(softmax_scale)
+    if not 1e-20 <= (abs(scale) if signed else scale) <= 1e20:  # the forward's softmax bound needs a positive one
+        raise ValueError(f"softmax_scale must be {'nonzero' if signed else 'positive'} and finite (1e-20 to 1e20), got {scale}")
+    return scale
+
+
 def _check_training(q, k, v, q_lens, kv_lens):
     for name, t in (("q", q), ("k", k), ("v", v)):
         if t.dim() != 4:
@@ -330,12 +337,15 @@ def attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, softmax_sca
     ``q [b, s_q, hq, 128]``, ``k, v [b, s_kv, hkv, 128]`` token-major bf16, ``hq % hkv == 0`` (query head ``h`` reads key head
     ``h // (hq // hkv)``). ``lse[.., r, g]`` belongs to token ``128 g + r``, as in :func:`ring_attention_const_max_fwd`.
     ``q_lens`` / ``kv_lens``: tokens of each batch element (host ints); rows behind them are not read, and their output
-    is 0 with an lse of -inf, as is that of rows without keys. ``softmax_scale`` defaults to ``1 / sqrt(128)``.
+    is 0 with an lse of -inf, as is that of rows without keys. ``softmax_scale`` (positive) defaults to ``1 / sqrt(128)``.
+    Like every forward here it sums under the bound ``softmax_scale * |q_i| * max_j |k_j|``: a row whose largest score lies
+    more than about 87 below that bound has no representable probabilities.
     """
     b, sq, skv, hq, hkv, q_lens, kv_lens = _check_training(q, k, v, q_lens, kv_lens)
+    scale = _training_scale(softmax_scale)
     dev = _lib.one_device(q, k, v)
-    scale = 1.0 / math.sqrt(_HEAD_DIM) if softmax_scale is None else float(softmax_scale)
     device = q.device
+    q, k, v = (t if t.data_ptr() % 16 == 0 else t.clone() for t in (q, k, v))
     with torch.cuda.device(dev):
         if hkv != hq:
             k, v = (t.repeat_interleave(hq // hkv, dim=2) for t in (k, v))
@@ -384,8 +394,8 @@ def attention_bwd(grad_o: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: tor
             raise ValueError(f"{name} must be [{b}, {hq}, {sq}, {_HEAD_DIM}], got {tuple(t.shape)}")
     if not lse.is_floating_point() or lse.shape != (b, hq, 128, -(-sq // 128)):
         raise ValueError(f"lse must be [{b}, {hq}, 128, {-(-sq // 128)}], got {lse.dtype} {tuple(lse.shape)}")
+    scale = _training_scale(softmax_scale, signed=True)
     dev = _lib.one_device(grad_o, q, k, v, o, lse)
-    scale = 1.0 / math.sqrt(_HEAD_DIM) if softmax_scale is None else float(softmax_scale)
     empty = not (b and sq and skv and hq)
     if empty:
         return tuple(t.new_zeros(t.shape) for t in (q, k, v))
@@ -423,5 +433,5 @@ def wan_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, softmax_sca
                   kv_lens=None) -> torch.Tensor:
     """Differentiable attention ``[b, hq, s_q, 128]`` of one device's ``q [b, s_q, hq, 128]``, ``k, v [b, s_kv, hkv, 128]``;
     the arguments are those of :func:`attention_fwd`, the gradients those of :func:`attention_bwd`."""
-    q_lens, kv_lens = (tuple(n) if isinstance(n, (list, tuple)) else n for n in (q_lens, kv_lens))
+    q_lens, kv_lens = (n if n is None or isinstance(n, torch.Tensor) else tuple(int(i) for i in n) for n in (q_lens, kv_lens))
     return _WanAttention.apply(q, k, v, softmax_scale, q_lens, kv_lens)

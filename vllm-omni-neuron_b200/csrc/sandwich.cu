@@ -705,7 +705,7 @@ int launch(Params p, long long n_mod, const Shape& s, cudaStream_t st) {
 
 int check(long long rows, int h, long long rows_per_mod, int post, int norm, float eps) {
   if (rows <= 0 || rows > 0x7fffffffLL || h <= 0 || h > kMaxH || h % 8) return VOMNI_EBADSHAPE;
-  if (rows_per_mod <= 0 || rows % rows_per_mod) return VOMNI_EBADSHAPE;
+  if (rows_per_mod <= 0 || rows % rows_per_mod || rows / rows_per_mod > 65535) return VOMNI_EBADSHAPE;
   if (post < 0 || post > 2 || norm < 0 || norm > 2) return VOMNI_EINVAL;
   if (!(eps > 0.f && eps <= 3.0e38f)) return VOMNI_EINVAL;  // rows behind the last one are zero: eps keeps them finite
   return VOMNI_OK;
@@ -751,7 +751,6 @@ extern "C" int vomni_sandwich_norm(const void* x, const void* residual, const fl
   if (misaligned(x, residual, residual_out, out) || misaligned(gate, post_weight, mul, add)) return VOMNI_EALIGN;
   rc = require_sm100();
   if (rc) return rc;
-  if (rows / rows_per_mod > 65535) return VOMNI_EBADSHAPE;
   Params p = {};
   fill(p, x, residual, gate, post_weight, mul, add, rows, h, rows_per_mod, per_mod, eps, post_norm, norm_type);
   p.out0 = static_cast<__nv_bfloat16*>(residual_out);
@@ -781,7 +780,6 @@ extern "C" int vomni_sandwich_norm_bwd(const void* grad_residual_out, const void
   int rc = check(rows, h, rows_per_mod, post_norm, norm_type, eps);
   if (rc) return rc;
   const long long n_mod = rows / rows_per_mod;
-  if (n_mod > 65535) return VOMNI_EBADSHAPE;
   if (workspace_bytes < vomni_sandwich_norm_workspace_bytes(rows, h, rows_per_mod)) return VOMNI_EWORKSPACE;
   if (misaligned(x, residual_out, grad_residual_out, grad_out) || misaligned(gate, post_weight, mul, workspace) ||
       misaligned(dx, dresidual))

@@ -23,6 +23,7 @@ from . import _lib
 from .adaln import _NORMS
 
 _MAX_HIDDEN = 8192
+_MAX_BATCH = 65535
 _PER = {"gate": 1, "mul": 2, "add": 4}  # VOMNI_PER_*
 
 
@@ -86,6 +87,8 @@ def _plan(x, residual, vectors, eps, post_norm, norm_type):
     for name, v in vectors.items():
         dense[name], per = _vector(name, v, batch, hidden)
         bits |= _PER[name] if per else 0
+    if bits and batch > _MAX_BATCH:
+        raise ValueError(f"per-batch vectors of more than {_MAX_BATCH} batch elements are unsupported, got {batch}")
     return hidden, rows, rows // batch if bits and batch else rows, bits, dense
 
 
