@@ -57,7 +57,7 @@ struct Params {
 // Eight adjacent values as they come from memory, and as floats.
 template <typename T>
 struct Io {  // 16-bit types
-  static constexpr int kAhead = 3;  // heads whose values a thread has in flight
+  static constexpr int kAhead = 4;  // heads whose values a thread has in flight
   using Raw = uint4;
   static VOMNI_DEV Raw load8(const T* p) { return __ldcs(reinterpret_cast<const uint4*>(p)); }
   static VOMNI_DEV void unpack(const Raw& w, float (&v)[8]) {
@@ -110,11 +110,12 @@ struct Io<float> {
 // one thread, into shared memory; then thread t works on pair group t % (d / 16) of heads t / (d / 16), ...; d / 16 need not
 // divide kThreads: the threads past the last whole head idle. A thread has kAhead heads' values in flight, the first of them
 // while the table is made. HBM-bound: every value is read and written once.
-// Measured, 32760 tokens of 80 heads of 128 in bf16 (1.34 GB): 253 us, 5.3 TB/s, 0.81 of the measured copy. With every
-// thread forming the eight angles it uses (32 times over at 80 heads) 351 us; 256 threads 259 us, 64 threads 259 us;
-// first loads after the table 281 us.
+// Measured, 32760 tokens of 80 heads of 128 in bf16 (1.34 GB): 212 us, 6.3 TB/s, 0.97 of the measured copy. With every
+// thread forming the eight angles it uses (32 times over at 80 heads) 351 us; first loads after the table 281 us instead of
+// 267; sixteen adjacent values a thread and the table by pairs, which filled the L1's data pipe with bank conflicts and half
+// used lines (83 % of its wavefronts), 253 us.
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 7) rotary_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kThreads, 6) rotary_kernel(const __grid_constant__ Params p) {
   __shared__ __align__(16) float2 table[kThreads];  // [per][d / 2] (cosine, sine)
   const int groups = p.d / (2 * kGroup), pairs = p.d / 2;
   const int lanes = kThreads / groups;  // heads in flight
@@ -126,9 +127,9 @@ __global__ void __launch_bounds__(kThreads, 7) rotary_kernel(const __grid_consta
   const long long b0 = token0 / p.s;
   const int s0 = static_cast<int>(token0 - b0 * p.s);
 
-  // values of the group: interleaved 16 consecutive ones, rotate-half 8 of each half of the head
-  const int o1 = p.half ? g * kGroup : g * 2 * kGroup;
-  const int o2 = p.half ? o1 + p.d / 2 : o1 + kGroup;
+  // values of the group: 8 of each half of the head, so that neighbouring threads load neighbouring 16 bytes. They are pairs
+  // 8 g .. 8 g + 7 (rotate-half), or 4 g .. 4 g + 3 and the same behind the middle (interleaved).
+  const int o1 = g * 8, o2 = o1 + p.d / 2;
   const int all = p.t[0].heads + p.t[1].heads, step = p.head_blocks * lanes;
   int k = lane < lanes ? 0 : count, h = share * lanes + lane;  // token of the CTA, head over both tensors
   constexpr int kAhead = Io<T>::kAhead;
@@ -175,7 +176,10 @@ __global__ void __launch_bounds__(kThreads, 7) rotary_kernel(const __grid_consta
     t -= rint(t);
     float sn, c;
     sincospif(2.f * static_cast<float>(t), &sn, &c);
-    table[threadIdx.x] = make_float2(c, sn * p.sign);
+    // the four float4 (two pairs each) that a group reads lie `groups` apart: a quarter-warp reads 128 adjacent bytes
+    const int behind = !p.half && pair >= pairs / 2, q = behind ? pair - pairs / 2 : pair;
+    const int owner = p.half ? q / 8 : q / 4, i = p.half ? q % 8 / 2 : q % 4 / 2 + 2 * behind;
+    table[tk * pairs + (i * groups + owner) * 2 + (pair & 1)] = make_float2(c, sn * p.sign);
   }
   __syncthreads();
 
@@ -186,10 +190,10 @@ __global__ void __launch_bounds__(kThreads, 7) rotary_kernel(const __grid_consta
       float a[8], b[8], c[kGroup], sn[kGroup];
       Io<T>::unpack(ra[u], a);
       Io<T>::unpack(rb[u], b);
-      const float4* cs = reinterpret_cast<const float4*>(table + tok[u] * pairs + g * kGroup);
+      const float4* cs = reinterpret_cast<const float4*>(table + tok[u] * pairs) + g;
 #pragma unroll
       for (int i = 0; i < kGroup / 2; ++i) {
-        const float4 w = cs[i];
+        const float4 w = cs[i * groups];
         c[2 * i] = w.x; sn[2 * i] = w.y; c[2 * i + 1] = w.z; sn[2 * i + 1] = w.w;
       }
       if (p.half) {
