@@ -523,9 +523,11 @@ __global__ void __launch_bounds__(kMaxThreads, 1) sandwich_kernel(const __grid_c
     else
       forward_rows<R, NV, false>(p, w, in, buf, turn, load, store);
   });
-  if constexpr (kBackward)
+  if constexpr (kBackward) {
+    pdl_trigger();  // the sums' launch may get ready while the last rows end
     store_sums<C>(p.parts + (static_cast<long long>(blockIdx.y) * gridDim.x + blockIdx.x) * 3 * p.H + c, p.H, stride, in, sum_a,
                   sum_m, sum_d);
+  }
 }
 
 // Short rows (H <= 256): a row per warp, four warps a CTA, straight from global memory.
@@ -557,8 +559,10 @@ __global__ void __launch_bounds__(128) sandwich_warp_kernel(const __grid_constan
     else
       forward_rows<1, 1, true>(p, w, in, nullptr, turn, load, store);
   }
-  if constexpr (kBackward)
+  if constexpr (kBackward) {
+    pdl_trigger();
     store_sums<8>(p.parts + (static_cast<long long>(blockIdx.y) * lanes + lane) * 3 * p.H + c, p.H, 0, in, sum_a, sum_m, sum_d);
+  }
 }
 
 struct SumParams {
@@ -579,6 +583,7 @@ __global__ void __launch_bounds__(1024) sandwich_sum_kernel(const __grid_constan
   const bool in = col < p.H;
   float* out = q == 0 ? p.dgate : q == 1 ? p.dmul : p.dadd;
   const bool per = p.per & (q == 0 ? kPerGate : q == 1 ? kPerMul : kPerAdd);
+  pdl_wait();  // launched as a dependent of the rows' kernel
   if (!out && !(q == 0 && p.dpost_w)) return;
   float shared_out = 0.f, dw = 0.f;
   const int mine = blockIdx.x * 32 + threadIdx.y;  // the column whose lanes this warp adds
@@ -811,7 +816,15 @@ extern "C" int vomni_sandwich_norm_bwd(const void* grad_residual_out, const void
   s.dpost_w = dpost_weight;
   s.dmul = dmul;
   s.dadd = dadd;
-  sandwich_sum_kernel<<<dim3((h + 31) / 32, 3), dim3(32, 32), 0, st>>>(s);
-  VOMNI_CUDA_TRY(cudaGetLastError());
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((h + 31) / 32, 3);
+  cfg.blockDim = dim3(32, 32);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  VOMNI_CUDA_TRY(cudaLaunchKernelEx(&cfg, sandwich_sum_kernel, s));
   return VOMNI_OK;
 }
