@@ -178,6 +178,14 @@ VOMNI_API int vomni_adaln_modulate(const void* hidden, const void* residual, con
                                    int norm_type, int quant, int ocp, int packed, void* out, void* out_scale,
                                    void* residual_out, vomni_stream_t stream);
 
+/* The same where lse was used too: grad_lse (or NULL: 0) is its gradient, in its layout; that of a row whose lse is -inf is
+ * ignored. */
+VOMNI_API int vomni_attention_bwd_lse(const void* grad_o, const float* grad_lse, const void* q, const void* k, const void* v,
+                                      const void* o, const float* lse, int b, int s_q, int s_kv, int hq, int hkv, int d,
+                                      const long long* strides, const int* q_lens, const int* kv_lens, float softmax_scale,
+                                      void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes,
+                                      vomni_stream_t stream);
+
 /* ------------------------------------------------------------------ norms around a block
  * The gated residual of adaln_modulate with a norm before it as well as after, and its gradients:
  *   y = post(x) * post_weight;  r = residual + gate * y -> residual_out = bf16(r);

@@ -90,6 +90,11 @@ SIGNATURES = {
         [P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, ctypes.POINTER(c_longlong), ctypes.POINTER(c_int),
          ctypes.POINTER(c_int), c_float, P, P, P, P, c_size_t, P],
     ),
+    "vomni_attention_bwd_lse": (
+        c_int,
+        [P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, ctypes.POINTER(c_longlong), ctypes.POINTER(c_int),
+         ctypes.POINTER(c_int), c_float, P, P, P, P, c_size_t, P],
+    ),
     "vomni_rotary_axes": (
         c_int,
         [P, P, c_int, c_longlong, c_longlong, P, P, c_int, c_longlong, c_longlong, c_int, c_int, c_int, P, c_int, c_int,

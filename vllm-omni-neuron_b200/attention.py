@@ -376,15 +376,16 @@ def _any_strides(t: torch.Tensor, head_major: bool = False):
 
 
 def attention_bwd(grad_o: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, lse: torch.Tensor,
-                  softmax_scale: float | None = None, *, q_lens=None, kv_lens=None):
+                  softmax_scale: float | None = None, *, q_lens=None, kv_lens=None, grad_lse: torch.Tensor | None = None):
     """``(dq, dk, dv)``, dense bf16 in the shapes of ``q, k, v``, of the attention whose output and log-sum-exp are ``o``, ``lse``.
 
     ``o`` / ``grad_o [b, hq, s_q, 128]`` bf16 (any strides) and ``lse`` as :func:`attention_fwd` or
-    ``ring_attention_const_max_fwd(training=True)`` return them; the other arguments as in :func:`attention_fwd`. The
+    ``ring_attention_const_max_fwd(training=True)`` return them, ``grad_lse`` (None: 0) the gradient of ``lse`` where that was
+    used too, as when parts are merged by it; the other arguments as in :func:`attention_fwd`. The
     probabilities are recomputed as ``exp(softmax_scale q k^T - lse)``, so with the ``lse`` and ``o`` of a whole sequence
     and a part of its keys the result is that part's share of the gradients (for a context-parallel ring: the parts'
     ``dq`` add up). Rows behind ``q_lens`` / ``kv_lens`` are not read and get zero gradients; a row whose lse is -inf
-    contributes nothing. The same call gives the same bits (no atomics).
+    has probabilities 0 and no ``grad_lse``. The same call gives the same bits (no atomics).
     """
     b, sq, skv, hq, hkv, q_lens, kv_lens = _check_training(q, k, v, q_lens, kv_lens)
     for name, t in (("grad_o", grad_o), ("o", o)):
@@ -394,8 +395,10 @@ def attention_bwd(grad_o: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: tor
             raise ValueError(f"{name} must be [{b}, {hq}, {sq}, {_HEAD_DIM}], got {tuple(t.shape)}")
     if not lse.is_floating_point() or lse.shape != (b, hq, 128, -(-sq // 128)):
         raise ValueError(f"lse must be [{b}, {hq}, 128, {-(-sq // 128)}], got {lse.dtype} {tuple(lse.shape)}")
+    if grad_lse is not None and (not grad_lse.is_floating_point() or grad_lse.shape != lse.shape):
+        raise ValueError(f"grad_lse must be {list(lse.shape)} like lse, got {grad_lse.dtype} {tuple(grad_lse.shape)}")
     scale = _training_scale(softmax_scale, signed=True)
-    dev = _lib.one_device(grad_o, q, k, v, o, lse)
+    dev = _lib.one_device(grad_o, q, k, v, o, lse, grad_lse)
     empty = not (b and sq and skv and hq)
     if empty:
         return tuple(t.new_zeros(t.shape) for t in (q, k, v))
@@ -403,13 +406,13 @@ def attention_bwd(grad_o: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: tor
     src = (_any_strides(q), _any_strides(k), _any_strides(v), _any_strides(grad_o, True), _any_strides(o, True))
     strides = (ctypes.c_longlong * 15)(*(n for _, st in src for n in st))
     q, k, v, grad_o, o = (t for t, _ in src)
-    lse = _lib.dense(lse if lse.dtype == torch.float32 else lse.float())
+    lse, grad_lse = (t if t is None else _lib.dense(t if t.dtype == torch.float32 else t.float()) for t in (lse, grad_lse))
     q_lens, kv_lens = ((ctypes.c_int * b)(*lens) if lens is not None else None for lens in (q_lens, kv_lens))
     ws_bytes = _lib.on_device(dev, _lib.load().vomni_attention_bwd_workspace_bytes, b, sq, skv, hq, hkv, _HEAD_DIM, q_lens, kv_lens)
     ws = q.new_empty(ws_bytes, dtype=torch.uint8)
-    _lib.launch(dev, "vomni_attention_bwd", grad_o.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
-                lse.data_ptr(), b, sq, skv, hq, hkv, _HEAD_DIM, strides, q_lens, kv_lens, scale, dq.data_ptr(),
-                dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), ws_bytes)
+    _lib.launch(dev, "vomni_attention_bwd_lse", grad_o.data_ptr(), None if grad_lse is None else grad_lse.data_ptr(), q.data_ptr(),
+                k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), b, sq, skv, hq, hkv, _HEAD_DIM, strides, q_lens, kv_lens,
+                scale, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), ws_bytes)
     return dq, dk, dv
 
 

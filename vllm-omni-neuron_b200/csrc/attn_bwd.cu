@@ -1,6 +1,6 @@
 // Attention's backward pass for sm_100a, which recomputes the probabilities from the forward's log-sum-exp:
 //     P = exp(scale Q K^T - lse)            dV = P^T dO
-//     dS = P (dO V^T - delta)               delta = rowsum(dO O)
+//     dS = P (dO V^T - delta)               delta = rowsum(dO O) - dlse, as the derivative of lse is P
 //     dQ = scale dS K                       dK = scale dS^T Q
 // The forward's lse is the one of ring_attention_const_max_fwd(training=True)
 // (vllm_omni_neuron/kernels/nkilib/experimental/attention/ring_attention_const_max_fwd.py:1062-1065), so the gradients
@@ -709,7 +709,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 struct RowParams {
   const __nv_bfloat16* o;
   const __nv_bfloat16* d_o;
-  const float* lse;  // [b, hq, 128, ceil(s_q / 128)]
+  const float* lse;   // [b, hq, 128, ceil(s_q / 128)]
+  const float* dlse;  // the same, or null (0)
   long long o_s, o_h, o_b, do_s, do_h, do_b;  // strides in elements
   int b, hq, s_q, rows, groups;
   int lens;  // q_len per batch element (b <= kMaxSeqs), else q_len[0]
@@ -763,8 +764,14 @@ __global__ void __launch_bounds__(256) attn_bwd_rows_kernel(const __grid_constan
     const int mr = row + sub;
     float l = p.scale > 0.f ? -kNoKeys : kNoKeys;
     if (mr < len) {
-      const float v = p.lse[(bh * 128 + (mr & 127)) * p.groups + (mr >> 7)];
-      if (!isinf(v)) l = -v / p.scale;
+      const long long at = (bh * 128 + (mr & 127)) * p.groups + (mr >> 7);
+      const float v = p.lse[at];
+      if (isinf(v)) {
+        mine = 0.f;  // no probabilities, whatever dlse holds
+      } else {
+        l = -v / p.scale;
+        if (p.dlse) mine -= p.dlse[at];
+      }
       if (fabsf(l) > kNoKeys) l = l > 0.f ? kNoKeys : -kNoKeys;
     }
     p.stats[bh * p.rows + mr] = stats_of(l, -mine);
@@ -928,11 +935,11 @@ static int launch_pairs(const abwd::Maps<N>& maps, abwd::Params p, int n, cudaSt
   return VOMNI_OK;
 }
 
-extern "C" int vomni_attention_bwd(const void* grad_o, const void* q, const void* k, const void* v, const void* o,
-                                   const float* lse, int b, int s_q, int s_kv, int hq, int hkv, int d,
-                                   const long long* strides, const int* q_lens, const int* kv_lens, float softmax_scale,
-                                   void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes,
-                                   vomni_stream_t stream) {
+extern "C" int vomni_attention_bwd_lse(const void* grad_o, const float* grad_lse, const void* q, const void* k, const void* v,
+                                       const void* o, const float* lse, int b, int s_q, int s_kv, int hq, int hkv, int d,
+                                       const long long* strides, const int* q_lens, const int* kv_lens, float softmax_scale,
+                                       void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes,
+                                       vomni_stream_t stream) {
   using namespace abwd;
   if (!grad_o || !q || !k || !v || !o || !lse || !strides || !dq || !dk || !dv || !workspace) return VOMNI_EINVAL;
   if (!(std::fabs(softmax_scale) >= 1e-20f && std::fabs(softmax_scale) <= 1e20f)) return VOMNI_EINVAL;
@@ -943,7 +950,7 @@ extern "C" int vomni_attention_bwd(const void* grad_o, const void* q, const void
                        reinterpret_cast<uintptr_t>(dk) | reinterpret_cast<uintptr_t>(dv) |
                        reinterpret_cast<uintptr_t>(workspace);
   if (al & 15) return VOMNI_EALIGN;
-  if (reinterpret_cast<uintptr_t>(lse) & 3) return VOMNI_EALIGN;
+  if ((reinterpret_cast<uintptr_t>(lse) | reinterpret_cast<uintptr_t>(grad_lse)) & 3) return VOMNI_EALIGN;
   const Plan plan = plan_of(b, s_q, s_kv, hq, hkv, q_lens, kv_lens);
   if (workspace_bytes < plan.bytes()) return VOMNI_EWORKSPACE;
   // strides: (row, head, batch) of q, k, v, grad_o, o in elements, multiples of 8 where the extent is over 1
@@ -1000,6 +1007,7 @@ extern "C" int vomni_attention_bwd(const void* grad_o, const void* q, const void
     r.o = static_cast<const __nv_bfloat16*>(o);
     r.d_o = static_cast<const __nv_bfloat16*>(grad_o);
     r.lse = lse;
+    r.dlse = grad_lse;
     r.o_s = so[0]; r.o_h = so[1]; r.o_b = so[2];
     r.do_s = st4[3][0]; r.do_h = st4[3][1]; r.do_b = st4[3][2];
     r.b = n;
@@ -1060,4 +1068,13 @@ extern "C" int vomni_attention_bwd(const void* grad_o, const void* q, const void
     VOMNI_CUDA_TRY(cudaGetLastError());
   }
   return VOMNI_OK;
+}
+
+extern "C" int vomni_attention_bwd(const void* grad_o, const void* q, const void* k, const void* v, const void* o,
+                                   const float* lse, int b, int s_q, int s_kv, int hq, int hkv, int d,
+                                   const long long* strides, const int* q_lens, const int* kv_lens, float softmax_scale,
+                                   void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes,
+                                   vomni_stream_t stream) {
+  return vomni_attention_bwd_lse(grad_o, nullptr, q, k, v, o, lse, b, s_q, s_kv, hq, hkv, d, strides, q_lens, kv_lens,
+                                 softmax_scale, dq, dk, dv, workspace, workspace_bytes, stream);
 }

@@ -230,7 +230,7 @@ def _of_call(ctx, grads):
 @torch.library.custom_op(f"{NS}::attention_fwd", mutates_args=())
 def attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, softmax_scale: float | None = None,
                   q_lens: list[int] | None = None, kv_lens: list[int] | None = None) -> list[torch.Tensor]:
-    """``[o, lse]`` of :func:`attention_fwd`; differentiable through ``o``."""
+    """``[o, lse]`` of :func:`attention_fwd`; differentiable through both."""
     return list(_attention_fwd(q, k, v, softmax_scale, q_lens=q_lens, kv_lens=kv_lens))
 
 
@@ -243,13 +243,13 @@ def _(q, k, v, softmax_scale=None, q_lens=None, kv_lens=None):
 @torch.library.custom_op(f"{NS}::attention_bwd", mutates_args=())
 def attention_bwd(grad_o: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, lse: torch.Tensor,
                   softmax_scale: float | None = None, q_lens: list[int] | None = None,
-                  kv_lens: list[int] | None = None) -> list[torch.Tensor]:
+                  kv_lens: list[int] | None = None, grad_lse: torch.Tensor | None = None) -> list[torch.Tensor]:
     """``[dq, dk, dv]`` of :func:`attention_bwd`."""
-    return list(_attention_bwd(grad_o, q, k, v, o, lse, softmax_scale, q_lens=q_lens, kv_lens=kv_lens))
+    return list(_attention_bwd(grad_o, q, k, v, o, lse, softmax_scale, q_lens=q_lens, kv_lens=kv_lens, grad_lse=grad_lse))
 
 
 @attention_bwd.register_fake
-def _(grad_o, q, k, v, o, lse, softmax_scale=None, q_lens=None, kv_lens=None):
+def _(grad_o, q, k, v, o, lse, softmax_scale=None, q_lens=None, kv_lens=None, grad_lse=None):
     return [t.new_empty(tuple(t.shape), dtype=torch.bfloat16) for t in (q, k, v)]
 
 
@@ -257,13 +257,17 @@ def _attention_setup(ctx, inputs, output):
     q, k, v, scale, q_lens, kv_lens = inputs
     ctx.save_for_backward(q, k, v, *output)
     ctx.rest = (scale, q_lens, kv_lens)
+    ctx.set_materialize_grads(False)
 
 
 def _attention_grad(ctx, grads):
-    if grads[0] is None:
+    grad_o, grad_lse = grads
+    if grad_o is None and grad_lse is None:
         return _of_call(ctx, (None,) * 6)
     q, k, v, o, lse = ctx.saved_tensors
-    return _of_call(ctx, (*torch.ops.b200omni.attention_bwd(grads[0], q, k, v, o, lse, *ctx.rest), None, None, None))
+    if grad_o is None:
+        grad_o = torch.zeros_like(o)
+    return _of_call(ctx, (*torch.ops.b200omni.attention_bwd(grad_o, q, k, v, o, lse, *ctx.rest, grad_lse), None, None, None))
 
 
 attention_fwd.register_autograd(_attention_grad, setup_context=_attention_setup)
