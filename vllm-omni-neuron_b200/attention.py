@@ -294,15 +294,15 @@ def _training_scale(softmax_scale, signed: bool = False) -> float:
 
 def _check_training(q, k, v, q_lens, kv_lens):
     for name, t in (("q", q), ("k", k), ("v", v)):
-        if t.dim() != 4:
+        if len(t.shape) != 4:
             raise ValueError(f"{name} must be token-major [b, s, heads, {_HEAD_DIM}], got {tuple(t.shape)}")
-        if t.dtype != torch.bfloat16:
+        if t.dtype is not torch.bfloat16:
             raise TypeError(f"{name} must be bfloat16, got {t.dtype}")
     b, sq, hq, d = q.shape
-    skv, hkv = k.shape[1:3]
+    kb, skv, hkv, kd = k.shape
     if d != _HEAD_DIM:
         raise ValueError(f"head_dim must be {_HEAD_DIM}, got {d}")
-    if k.shape != v.shape or k.shape[0] != b or k.shape[3] != d:
+    if k.shape != v.shape or kb != b or kd != d:
         raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must be [{b}, s_kv, heads, {d}]")
     if hkv == 0 or hq % hkv:
         raise ValueError(f"query heads ({hq}) must be a multiple of key heads ({hkv})")
@@ -362,13 +362,17 @@ def attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, softmax_sca
         return o, lse
 
 
+_Strides = ctypes.c_longlong * 15  # (token, head, batch) of q, k, v, grad_o, o
+
+
 def _any_strides(t: torch.Tensor, head_major: bool = False):
     """(tensor, its token, head and batch strides): ``t`` as it is where TMA can address its strides (d dense, the others
     positive multiples of 8), else a copy. ``head_major``: ``t`` is ``[b, heads, s, d]``."""
-    st, sh = t.stride(), t.shape
-    ok = st[3] == 1 and t.data_ptr() % 16 == 0
-    for i in range(3):
-        ok = ok and (sh[i] == 1 or (st[i] > 0 and st[i] % 8 == 0))
+    st = t.stride()
+    ok = t.data_ptr() % 16 == 0
+    if ok and not t.is_contiguous():
+        sh = t.shape
+        ok = st[3] == 1 and all(sh[i] == 1 or (st[i] > 0 and st[i] % 8 == 0) for i in range(3))
     if not ok:
         t = _lib.dense(t)
         st = t.stride()
@@ -389,7 +393,7 @@ def attention_bwd(grad_o: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: tor
     """
     b, sq, skv, hq, hkv, q_lens, kv_lens = _check_training(q, k, v, q_lens, kv_lens)
     for name, t in (("grad_o", grad_o), ("o", o)):
-        if t.dtype != torch.bfloat16:
+        if t.dtype is not torch.bfloat16:
             raise TypeError(f"{name} must be bfloat16, got {t.dtype}")
         if t.shape != (b, hq, sq, _HEAD_DIM):
             raise ValueError(f"{name} must be [{b}, {hq}, {sq}, {_HEAD_DIM}], got {tuple(t.shape)}")
@@ -402,14 +406,22 @@ def attention_bwd(grad_o: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: tor
     empty = not (b and sq and skv and hq)
     if empty:
         return tuple(t.new_zeros(t.shape) for t in (q, k, v))
-    dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
-    src = (_any_strides(q), _any_strides(k), _any_strides(v), _any_strides(grad_o, True), _any_strides(o, True))
-    strides = (ctypes.c_longlong * 15)(*(n for _, st in src for n in st))
-    q, k, v, grad_o, o = (t for t, _ in src)
-    lse, grad_lse = (t if t is None else _lib.dense(t if t.dtype == torch.float32 else t.float()) for t in (lse, grad_lse))
-    q_lens, kv_lens = ((ctypes.c_int * b)(*lens) if lens is not None else None for lens in (q_lens, kv_lens))
+    dq, dk, dv = _lib.empty(q), _lib.empty(k), _lib.empty(v)
+    q, q_st = _any_strides(q)
+    k, k_st = _any_strides(k)
+    v, v_st = _any_strides(v)
+    grad_o, go_st = _any_strides(grad_o, True)
+    o, o_st = _any_strides(o, True)
+    strides = _Strides(*q_st, *k_st, *v_st, *go_st, *o_st)
+    lse = _lib.dense(lse.float())
+    if grad_lse is not None:
+        grad_lse = _lib.dense(grad_lse.float())
+    if q_lens is not None:
+        q_lens = (ctypes.c_int * b)(*q_lens)
+    if kv_lens is not None:
+        kv_lens = (ctypes.c_int * b)(*kv_lens)
     ws_bytes = _lib.on_device(dev, _lib.load().vomni_attention_bwd_workspace_bytes, b, sq, skv, hq, hkv, _HEAD_DIM, q_lens, kv_lens)
-    ws = q.new_empty(ws_bytes, dtype=torch.uint8)
+    ws = _lib.workspace(ws_bytes, q.device)
     _lib.launch(dev, "vomni_attention_bwd_lse", grad_o.data_ptr(), None if grad_lse is None else grad_lse.data_ptr(), q.data_ptr(),
                 k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), b, sq, skv, hq, hkv, _HEAD_DIM, strides, q_lens, kv_lens,
                 scale, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), ws_bytes)

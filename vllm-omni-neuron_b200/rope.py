@@ -107,6 +107,8 @@ def _rotary_source(t: torch.Tensor):
     """(tensor, row stride, batch stride) as the kernel reads it: heads dense inside a token, strides of 16 bytes
     (column slices of a fused projection pass as they are); anything else is copied."""
     b, s, h, d = t.shape
+    if t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t, h * d, s * h * d
     sb, ss, sh, sd = t.stride()
     row, batch = ss if s > 1 else h * d, sb if b > 1 else s * h * d
     unit = 16 // t.element_size()
@@ -117,24 +119,29 @@ def _rotary_source(t: torch.Tensor):
 
 
 def _rotary(q, k, positions, axes_dims, theta, pairing, inverse):
-    b, s, _, d = q.shape
-    outs, args, keep = [], [], []
-    for t in (q, k):
-        if t is None or t.numel() == 0:
-            outs.append(None if t is None else t.new_empty(t.shape))
-            args += (None, None, 0, 0, 0)
-            continue
-        src, row, batch = _rotary_source(t)
-        out = t.new_empty(t.shape)
-        keep.append(src)
-        outs.append(out)
-        args += (src.data_ptr(), out.data_ptr(), t.shape[2], row, batch)
-    if keep:
-        pos = positions if positions.is_contiguous() else positions.contiguous()
-        axes = (ctypes.c_int * len(axes_dims))(*axes_dims)
-        _lib.launch(q.get_device(), "vomni_rotary_axes", *args, b, s, d, pos.data_ptr(), _POSITION_DTYPES[pos.dtype],
-                    int(pos.dim() == 3), len(axes_dims), axes, theta, pairing, int(inverse), _ROTARY_DTYPES[q.dtype])
-    return outs
+    b, s, hq, d = q.shape
+    q_out = k_out = None
+    q_args = k_args = (None, None, 0, 0, 0)
+    if q.numel():
+        q, row, batch = _rotary_source(q)
+        q_out = _lib.empty(q)
+        q_args = (q.data_ptr(), q_out.data_ptr(), hq, row, batch)
+    if k is not None and k.numel():
+        k, row, batch = _rotary_source(k)
+        k_out = _lib.empty(k)
+        k_args = (k.data_ptr(), k_out.data_ptr(), k.shape[2], row, batch)
+    if q_out is not None or k_out is not None:
+        if not positions.is_contiguous():
+            positions = positions.contiguous()
+        n = len(axes_dims)
+        _lib.launch(q.get_device(), "vomni_rotary_axes", *q_args, *k_args, b, s, d, positions.data_ptr(),
+                    _POSITION_DTYPES[positions.dtype], int(positions.dim() == 3), n, (ctypes.c_int * n)(*axes_dims), theta, pairing,
+                    int(inverse), _ROTARY_DTYPES[q.dtype])
+    if q_out is None:
+        q_out = q.new_empty(q.shape)
+    if k_out is None and k is not None:
+        k_out = k.new_empty(k.shape)
+    return q_out, k_out
 
 
 class _RotaryAxes(torch.autograd.Function):
@@ -143,7 +150,7 @@ class _RotaryAxes(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(positions)
         ctx.rest = (axes_dims, theta, pairing, inverse)
-        return tuple(_rotary(q, k, positions, axes_dims, theta, pairing, inverse))
+        return _rotary(q, k, positions, axes_dims, theta, pairing, inverse)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -179,26 +186,26 @@ def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor
     """
     if pairing not in _PAIRINGS:
         raise ValueError(f"unknown pairing {pairing!r}")
-    axes_dims = tuple(int(n) for n in axes_dims)
-    for name, t in (("q", q), ("k", k)):
-        if t is None and name == "k":
-            continue
-        if t.dim() != 4:
+    axes_dims = tuple(map(int, axes_dims))
+    for name, t in (("q", q),) if k is None else (("q", q), ("k", k)):
+        if len(t.shape) != 4:
             raise ValueError(f"{name} must be token-major [b, s, heads, d], got {tuple(t.shape)}")
         if t.dtype not in _ROTARY_DTYPES:
             raise TypeError(f"{name} must be bfloat16, float16 or float32, got {t.dtype}")
     b, s, _, d = q.shape
-    if k is not None and (k.shape[0], k.shape[1], k.shape[3]) != (b, s, d):
-        raise ValueError(f"k {tuple(k.shape)} must match q {tuple(q.shape)} but for the heads")
-    if k is not None and k.dtype != q.dtype:
-        raise TypeError(f"q and k must have one dtype, got {q.dtype} and {k.dtype}")
+    if k is not None:
+        kb, ks, _, kd = k.shape
+        if kb != b or ks != s or kd != d:
+            raise ValueError(f"k {tuple(k.shape)} must match q {tuple(q.shape)} but for the heads")
+        if k.dtype is not q.dtype:
+            raise TypeError(f"q and k must have one dtype, got {q.dtype} and {k.dtype}")
     if d % 16 or not 0 < d <= 256:
         raise ValueError(f"head dim {d} unsupported (needs d % 16 == 0 and d <= 256)")
-    if not 1 <= len(axes_dims) <= 4 or any(n <= 0 or n % 2 for n in axes_dims) or sum(axes_dims) != d:
+    if not 1 <= len(axes_dims) <= 4 or min(axes_dims) <= 0 or sum(axes_dims) != d or [n for n in axes_dims if n % 2]:
         raise ValueError(f"axes_dims {axes_dims} must be 1 to 4 even counts that sum to the head dim {d}")
     if positions.dtype not in _POSITION_DTYPES:
         raise TypeError(f"positions must be int32, int64 or float32, got {positions.dtype}")
-    if positions.shape != (s, len(axes_dims)) and positions.shape != (b, s, len(axes_dims)):
+    if positions.shape not in ((s, len(axes_dims)), (b, s, len(axes_dims))):
         raise ValueError(f"positions must be [{s}, {len(axes_dims)}] or [{b}, {s}, {len(axes_dims)}], got {tuple(positions.shape)}")
     if not (theta > 0 and theta < float("inf")):
         raise ValueError(f"theta must be positive and finite, got {theta}")
@@ -208,4 +215,4 @@ def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor
         out = _RotaryAxes.apply(*args)
     else:
         out = _rotary(*args)
-    return out[0] if k is None else tuple(out)
+    return out[0] if k is None else out

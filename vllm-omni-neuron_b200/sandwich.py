@@ -24,7 +24,7 @@ from .adaln import _NORMS
 
 _MAX_HIDDEN = 8192
 _MAX_BATCH = 65535
-_PER = {"gate": 1, "mul": 2, "add": 4}  # VOMNI_PER_*
+_PER_GATE, _PER_MUL, _PER_ADD = 1, 2, 4  # VOMNI_PER_*
 
 
 class SandwichGrads(NamedTuple):
@@ -39,100 +39,112 @@ class SandwichGrads(NamedTuple):
 
 
 def _rows(name: str, t: torch.Tensor, shape) -> torch.Tensor:
-    if t.dtype != torch.bfloat16:
+    if t.dtype is not torch.bfloat16:
         raise TypeError(f"{name} must be bfloat16, got {t.dtype}")
     if t.shape != shape:
         raise ValueError(f"{name} shape {tuple(t.shape)} must be {tuple(shape)}")
     return _lib.dense(t)
 
 
-def _vector(name: str, v: torch.Tensor | None, batch: int, hidden: int):
-    """(fp32 dense rows or None, whether one per batch element)."""
-    if v is None:
-        return None, False
-    if v.dtype not in (torch.float32, torch.bfloat16, torch.float16):
-        raise TypeError(f"{name} must be float32, bfloat16 or float16, got {v.dtype}")
+def _vector(name: str, v: torch.Tensor, batch: int, hidden: int) -> torch.Tensor:
+    """``v`` checked, as dense fp32."""
     shape = v.shape
     if len(shape) == 3 and name != "post_weight":
         if shape != (batch, 1, hidden):
             raise ValueError(f"per-batch {name} must be [{batch}, 1, {hidden}], got {tuple(shape)}")
-        per = True
     elif shape != (hidden,) and shape != (1, hidden):
         raise ValueError(f"{name} must be {'' if name == 'post_weight' else f'[{batch}, 1, {hidden}] or '}[{hidden}], got {tuple(shape)}")
-    else:
-        per = False
-    return _lib.dense(v if v.dtype == torch.float32 else v.float()), per
+    if v.dtype is not torch.float32:
+        if v.dtype not in (torch.bfloat16, torch.float16):
+            raise TypeError(f"{name} must be float32, bfloat16 or float16, got {v.dtype}")
+        v = v.float()
+    return _lib.dense(v)
 
 
-def _plan(x, residual, vectors, eps, post_norm, norm_type):
-    """Checked (hidden, rows, rows_per_mod, per bits, fp32 vectors) of a call."""
+def _plan(x, residual, gate, mul, add, post_weight, eps, post_norm, norm_type):
+    """Checked ``(hidden, rows, rows_per_mod, per bits, post kind, norm kind, the vectors in fp32)`` of a call."""
     if not 0 < eps < float("inf"):
         raise ValueError(f"eps must be positive and finite, got {eps}")
     if post_norm not in _NORMS:
         raise ValueError(f"unsupported post_norm {post_norm!r}")
     if norm_type not in _NORMS:
         raise ValueError(f"unsupported norm_type {norm_type!r}")
-    if residual.dim() < 2:
+    shape = residual.shape
+    if len(shape) < 2:
         raise ValueError("residual must have at least 2 dims")
-    hidden = residual.shape[-1]
+    hidden = shape[-1]
     if not 0 < hidden <= _MAX_HIDDEN or hidden % 8:
         raise ValueError(f"hidden dim {hidden} unsupported (needs H <= {_MAX_HIDDEN} and H % 8 == 0)")
     if x is None:
-        for name in ("gate", "post_weight"):
-            if vectors[name] is not None:
+        for name, v in (("gate", gate), ("post_weight", post_weight)):
+            if v is not None:
                 raise ValueError(f"{name} requires x (it scales the sub-layer output)")
-    batch = residual.shape[0] if residual.dim() == 3 else 1
+    batch = shape[0] if len(shape) == 3 else 1
     rows = residual.numel() // hidden
-    dense, bits = {}, 0
-    for name, v in vectors.items():
-        dense[name], per = _vector(name, v, batch, hidden)
-        bits |= _PER[name] if per else 0
+    bits = 0
+    if gate is not None:
+        gate = _vector("gate", gate, batch, hidden)
+        bits = _PER_GATE if gate.dim() == 3 else 0
+    if mul is not None:
+        mul = _vector("mul", mul, batch, hidden)
+        bits |= _PER_MUL if mul.dim() == 3 else 0
+    if add is not None:
+        add = _vector("add", add, batch, hidden)
+        bits |= _PER_ADD if add.dim() == 3 else 0
+    if post_weight is not None:
+        post_weight = _vector("post_weight", post_weight, batch, hidden)
     if bits and batch > _MAX_BATCH:
         raise ValueError(f"per-batch vectors of more than {_MAX_BATCH} batch elements are unsupported, got {batch}")
-    return hidden, rows, rows // batch if bits and batch else rows, bits, dense
+    per_mod = rows // batch if bits and batch else rows
+    return hidden, rows, per_mod, bits, _NORMS[post_norm], _NORMS[norm_type], gate, mul, add, post_weight
 
 
 def _ptr(t):
-    return t.data_ptr() if t is not None else None
+    return None if t is None else t.data_ptr()
 
 
 def _forward(x, residual, gate, mul, add, post_weight, eps, post_norm, norm_type):
-    hidden, rows, per_mod, bits, v = _plan(
-        x, residual, {"gate": gate, "mul": mul, "add": add, "post_weight": post_weight}, eps, post_norm, norm_type)
+    hidden, rows, per_mod, bits, post, norm, gate, mul, add, post_weight = _plan(x, residual, gate, mul, add, post_weight, eps,
+                                                                                 post_norm, norm_type)
     dev = _lib.one_device(x, residual, gate, mul, add, post_weight)
-    x = None if x is None else _rows("x", x, residual.shape)
+    if x is not None:
+        x = _rows("x", x, residual.shape)
     residual = _rows("residual", residual, residual.shape)
-    res_out = None if x is None else residual.new_empty(residual.shape)
-    out = residual.new_empty(residual.shape)
+    res_out = None if x is None else torch.empty_like(residual)
+    out = torch.empty_like(residual)
     if rows:
-        _lib.launch(dev, "vomni_sandwich_norm", _ptr(x), residual.data_ptr(), _ptr(v["gate"]), _ptr(v["post_weight"]), _ptr(v["mul"]),
-                    _ptr(v["add"]), rows, hidden, per_mod, bits, eps, _NORMS[post_norm], _NORMS[norm_type], _ptr(res_out),
-                    out.data_ptr())
+        _lib.launch(dev, "vomni_sandwich_norm", _ptr(x), residual.data_ptr(), _ptr(gate), _ptr(post_weight), _ptr(mul), _ptr(add), rows,
+                    hidden, per_mod, bits, eps, post, norm, _ptr(res_out), out.data_ptr())
     return res_out, out
 
 
 def _backward(grad_res, grad_out, x, residual_out, gate, mul, add, post_weight, eps, post_norm, norm_type, need):
-    vectors = {"gate": gate, "mul": mul, "add": add, "post_weight": post_weight}
-    hidden, rows, per_mod, bits, v = _plan(x, residual_out, vectors, eps, post_norm, norm_type)
-    dev = _lib.one_device(grad_res, grad_out, x, residual_out, *vectors.values())
+    """``need``: whether gate's, mul's, add's and post_weight's gradients are asked for."""
+    given = (gate, mul, add, post_weight)
+    hidden, rows, per_mod, bits, post, norm, *vectors = _plan(x, residual_out, *given, eps, post_norm, norm_type)
+    dev = _lib.one_device(grad_res, grad_out, x, residual_out, *vectors)
     shape = residual_out.shape
-    grad_res = None if grad_res is None else _rows("grad_residual_out", grad_res, shape)
-    grad_out = None if grad_out is None else _rows("grad_out", grad_out, shape)
-    x = None if x is None else _rows("x", x, shape)
+    if grad_res is not None:
+        grad_res = _rows("grad_residual_out", grad_res, shape)
+    if grad_out is not None:
+        grad_out = _rows("grad_out", grad_out, shape)
+    dx = None
+    if x is not None:
+        x = _rows("x", x, shape)
+        dx = torch.empty_like(x)
     residual_out = _rows("residual_out", residual_out, shape)
-    dx = None if x is None else x.new_empty(shape)
-    dres = residual_out.new_empty(shape)
-    make = residual_out.new_empty if rows else residual_out.new_zeros
-    sums = {n: make(t.shape, dtype=torch.float32) if t is not None and need[n] else None for n, t in vectors.items()}
+    dres = torch.empty_like(residual_out)
+    make = torch.empty_like if rows else torch.zeros_like
+    sums = [make(v) if v is not None and n else None for v, n in zip(vectors, need)]  # fp32 and dense, as the vectors now are
     if rows:
         ws_bytes = _lib.on_device(dev, _lib.load().vomni_sandwich_norm_workspace_bytes, rows, hidden, per_mod)
-        ws = residual_out.new_empty(ws_bytes, dtype=torch.uint8)
-        _lib.launch(dev, "vomni_sandwich_norm_bwd", _ptr(grad_res), _ptr(grad_out), _ptr(x), residual_out.data_ptr(), _ptr(v["gate"]),
-                    _ptr(v["post_weight"]), _ptr(v["mul"]), rows, hidden, per_mod, bits, eps, _NORMS[post_norm], _NORMS[norm_type],
-                    _ptr(dx), dres.data_ptr(), _ptr(sums["gate"]), _ptr(sums["post_weight"]), _ptr(sums["mul"]), _ptr(sums["add"]),
-                    ws.data_ptr(), ws_bytes)
-    done = {n: t if t is None or vectors[n].dtype == torch.float32 else t.to(vectors[n].dtype) for n, t in sums.items()}
-    return SandwichGrads(dx, dres, done["gate"], done["mul"], done["add"], done["post_weight"])
+        ws = _lib.workspace(ws_bytes, residual_out.device)
+        gate, mul, _, post_weight = vectors
+        dgate, dmul, dadd, dw = map(_ptr, sums)
+        _lib.launch(dev, "vomni_sandwich_norm_bwd", _ptr(grad_res), _ptr(grad_out), _ptr(x), residual_out.data_ptr(), _ptr(gate),
+                    _ptr(post_weight), _ptr(mul), rows, hidden, per_mod, bits, eps, post, norm, _ptr(dx), dres.data_ptr(), dgate, dw,
+                    dmul, dadd, ws.data_ptr(), ws_bytes)
+    return SandwichGrads(dx, dres, *(t if t is None or t.dtype is g.dtype else t.to(g.dtype) for t, g in zip(sums, given)))
 
 
 class _SandwichNorm(torch.autograd.Function):
@@ -151,10 +163,9 @@ class _SandwichNorm(torch.autograd.Function):
         grad_res, grad_out = (None, grads[0]) if x is None else grads
         if grad_res is None and grad_out is None:
             return (None,) * 9
-        names = ("x", "residual", "gate", "mul", "add", "post_weight")
-        need = dict(zip(names, ctx.needs_input_grad))
-        g = _backward(grad_res, grad_out, x, res, gate, mul, add, post_weight, *ctx.kinds, need)
-        return tuple(getattr(g, n) if need[n] else None for n in names) + (None, None, None)
+        need = ctx.needs_input_grad[:6]
+        grads = _backward(grad_res, grad_out, x, res, gate, mul, add, post_weight, *ctx.kinds, need[2:])
+        return tuple(g if n else None for g, n in zip(grads, need)) + (None, None, None)
 
 
 def sandwich_norm(
@@ -206,6 +217,5 @@ def sandwich_norm_bwd(
     the ``residual_out`` it returned (``residual`` itself where ``x`` is None)."""
     if grad_residual_out is None and grad_out is None:
         raise ValueError("at least one of grad_residual_out and grad_out is needed")
-    need = dict.fromkeys(("gate", "mul", "add", "post_weight"), True)
     return _backward(grad_residual_out, grad_out, x, residual_out, gate, mul, add, post_weight, float(eps), post_norm, norm_type,
-                     need)
+                     (True,) * 4)
