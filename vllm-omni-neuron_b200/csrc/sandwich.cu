@@ -18,7 +18,7 @@
 // time through a ring in shared memory; a thread owns chunks of 8 adjacent columns of all of them. The kernels are persistent, so
 // that in the backward pass a thread's column sums stay in its registers over all rows of its CTA; the CTAs' sums
 // go to a workspace and are added in a fixed order by a second kernel (no atomics: the same call gives the same bits).
-// Measured, 32760 x 5120: forward 225 us (0.91 of the measured copy rate), backward 380 us (0.81).
+// Measured, 32760 x 5120: forward 225 us (0.91 of the measured copy rate), backward 356 us (0.86).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -85,9 +85,9 @@ VOMNI_DEV float warp_fold(float (&v)[N]) {
 // Sums N values over the threads that share a row (or a few rows): one warp (kWarpRow), or the whole CTA through
 // shared memory. Every thread ends with the same sums, added in an order that only the CTA's size sets. `turn`
 // alternates between two buffers: a buffer is written again only after a barrier that follows its last read. Entries
-// of warps that the CTA does not have are zero from the start.
-template <int N, bool kWarpRow>
-VOMNI_DEV void row_sum(float (&v)[N], float (*buf)[kBuf], int& turn) {
+// of warps that the CTA does not have are zero from the start. Returns whether any thread said `bad` (kVote).
+template <int N, bool kWarpRow, bool kVote = false>
+VOMNI_DEV bool row_sum(float (&v)[N], float (*buf)[kBuf], int& turn, bool bad = false) {
   constexpr int kGroup = 32 / N;
   const int lane = threadIdx.x & 31;
   float s = warp_fold<N>(v);
@@ -95,7 +95,10 @@ VOMNI_DEV void row_sum(float (&v)[N], float (*buf)[kBuf], int& turn) {
     float* b = buf[turn];
     turn ^= 1;
     if (lane % kGroup == 0) b[lane / kGroup * 32 + (threadIdx.x >> 5)] = s;
-    __syncthreads();
+    if (kVote)
+      bad = __syncthreads_or(bad);
+    else
+      __syncthreads();
     b += lane * N;  // value lane / kGroup, N of its 32 warps
     if constexpr (N == 8) {
       const float4 x = reinterpret_cast<const float4*>(b)[0], y = reinterpret_cast<const float4*>(b)[1];
@@ -114,6 +117,7 @@ VOMNI_DEV void row_sum(float (&v)[N], float (*buf)[kBuf], int& turn) {
   }
 #pragma unroll
   for (int i = 0; i < N; ++i) v[i] = __shfl_sync(0xffffffffu, s, i * kGroup);
+  return bad;
 }
 
 // The values of R rows that a thread owns (C of each) as fp32 pairs: the packed arithmetic halves the instructions,
@@ -127,6 +131,16 @@ VOMNI_DEV float halves_sum(uint64_t v) {
   float a, b;
   f2_unpack(v, a, b);
   return a + b;
+}
+
+template <int NV>
+VOMNI_DEV void centre(uint64_t (&v)[NV * 4], float mean, const bool (&in)[NV]) {
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const uint64_t neg = both(in[j] ? -mean : 0.f);
+#pragma unroll
+    for (int i = 4 * j; i < 4 * j + 4; ++i) v[i] = f2_add(v[i], neg);
+  }
 }
 
 // x -> its normalised values. Two passes (mean, then squared deviations) in fp32. Columns behind
@@ -318,12 +332,7 @@ VOMNI_DEV void backward_rows(const Params& p, const Vecs<NV * 8>& w, const bool 
   const int kind[2] = {kNorm != kAsked ? kNorm : has_out ? p.norm : kNone, kPost != kAsked ? kPost : has_x ? p.post : kNone};
   auto centred = [&](int q, int r, uint64_t (&v)[P]) {
     load(q ? 0 : 1, r, v);
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const uint64_t neg = both(in[j] ? -mean[2 * r + q] : 0.f);
-#pragma unroll
-      for (int i = 4 * j; i < 4 * j + 4; ++i) v[i] = f2_add(v[i], neg);
-    }
+    centre<NV>(v, mean[2 * r + q], in);
   };
   auto hat = [&](int q, int r, uint64_t (&v)[P]) {
     centred(q, r, v);
@@ -530,6 +539,267 @@ __global__ void __launch_bounds__(kMaxThreads, 1) sandwich_kernel(const __grid_c
   }
 }
 
+// ---------------------------------------------------------------- long calls' backward pass
+// The backward pass of calls with a branch and both gradients over many rows: R rows at a time, like backward_rows, but the
+// statistics of the next R rows are summed along with this group's gradients, so that a group costs two barriers (the
+// second also frees its slots) instead of five. For that x and residual_out of the next group are there a group early: they have
+// three slots, the gradients two. One CTA of 10 warps an SM has nothing else to
+// issue around a barrier: 32760 x 5120 356 us instead of 383 with sandwich_kernel, 0.86 of the measured copy rate. Several CTAs an SM
+// hide that by themselves (32760 x 1536: 125 us with either). One row at a time, where each row takes the two
+// barriers, it is slower (16384 x 8192: 481 us instead of 397).
+template <int R, int NV, int kMaxThreads, bool kFull, int kPost, int kNorm>
+__global__ void __launch_bounds__(kMaxThreads, 1) sandwich_bwd_kernel(const __grid_constant__ Params p) {
+  constexpr int C = NV * 8, P = C / 2;
+  constexpr bool kMeans = kPost == kLayer || kNorm == kLayer, kSquares = kPost != kNone || kNorm != kNone;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ __align__(8) uint64_t full[5];  // rows' slots, gradients' slots
+  __shared__ int abort_flag;
+  __shared__ __align__(16) float buf[2][kBuf];
+  for (int i = threadIdx.x; i < 2 * kBuf; i += blockDim.x) buf[i / kBuf][i % kBuf] = 0.f;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 5; ++i) mbar_init(&full[i], 1);
+    abort_flag = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+  const int c = threadIdx.x * 8, stride = blockDim.x * 8, pitch = p.H >> 3, chunks = R * pitch;
+  const long long begin = static_cast<long long>(blockIdx.y) * p.rows_per_mod, end = begin + p.rows_per_mod;
+  const long long first = begin + static_cast<long long>(blockIdx.x) * R, step = static_cast<long long>(gridDim.x) * R;
+  uint4* const mem = reinterpret_cast<uint4*>(smem);  // [3][x, residual_out][chunks], [2][d_res, d_out][chunks]
+  auto rows_slot = [&](int s) { return mem + s * 2 * chunks; };
+  auto grads_slot = [&](int s) { return mem + (6 + s * 2) * chunks; };
+  auto issue = [&](const __nv_bfloat16* a, const __nv_bfloat16* b, long long row, uint4* dst, uint64_t* bar) {
+    if (row >= end) return;
+    const uint32_t bytes = static_cast<uint32_t>(min(static_cast<long long>(R), end - row)) * p.H * 2u;
+    mbar_expect_tx(bar, 2 * bytes);
+    bulk_g2s(dst, a + row * p.H, bytes, bar);
+    bulk_g2s(dst + chunks, b + row * p.H, bytes, bar);
+  };
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < 3; ++s) {
+      issue(p.x, p.residual, first + s * step, rows_slot(s), &full[s]);
+      if (s < 2) issue(p.d_res, p.d_out, first + s * step, grads_slot(s), &full[3 + s]);
+    }
+  }
+  bool in[NV];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) in[j] = kFull || c + j * stride < p.H;
+  Vecs<C> w;
+  load_vecs<C>(p, blockIdx.y, c, stride, in, w);
+  uint64_t sum_a[P] = {}, sum_m[P] = {}, sum_d[P] = {};
+  int turn = 0;
+  bool ok = true;
+  auto wait = [&](int bar, uint32_t use) {
+    ok = mbar_wait(&full[bar], use & 1, &abort_flag, p.status, VOMNI_DEV_TIMEOUT_BASE + kSiteRowWait) && ok;
+  };
+  auto clear_missing = [&](uint4* slot, long long row) {  // zeros in place of rows behind the last (a thread reads only its chunks)
+    if (R == 1 || end - row >= R) return;
+    for (int t = 0; t < 2; ++t)
+      for (int r = static_cast<int>(end - row); r < R; ++r)
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+          if (in[j]) slot[t * chunks + r * pitch + threadIdx.x + j * blockDim.x] = make_uint4(0, 0, 0, 0);
+  };
+  auto load = [&](const uint4* slot, int t, int r, uint64_t (&v)[P]) {
+    const uint4* s = slot + t * chunks + r * pitch + threadIdx.x;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      uint4 u = make_uint4(0, 0, 0, 0);
+      if (in[j]) u = s[j * blockDim.x];
+      unpack_pairs(u, &v[4 * j]);
+    }
+  };
+  // Partial sums of a group's statistics; of row r: 2 r residual_out's, 2 r + 1 x's.
+  constexpr int kKind[2] = {kNorm, kPost};
+  auto sums_of = [&](const uint4* slot, float* s) {
+#pragma unroll
+    for (int i = 0; i < 2 * R; ++i) {
+      s[i] = 0.f;
+      if (kKind[i & 1] != kLayer) continue;
+      uint64_t v[P];
+      load(slot, i & 1 ? 0 : 1, i >> 1, v);
+      uint64_t t = v[0];
+#pragma unroll
+      for (int k = 1; k < P; ++k) t = f2_add(t, v[k]);
+      s[i] = halves_sum(t);
+    }
+  };
+  auto squares_of = [&](const uint4* slot, const float (&mean)[2 * R], float* s) {
+#pragma unroll
+    for (int i = 0; i < 2 * R; ++i) {
+      s[i] = 0.f;
+      if (kKind[i & 1] == kNone) continue;
+      uint64_t v[P];
+      load(slot, i & 1 ? 0 : 1, i >> 1, v);
+      if (kKind[i & 1] == kLayer) centre<NV>(v, mean[i], in);
+      uint64_t t = f2_mul(v[0], v[0]);
+#pragma unroll
+      for (int k = 1; k < P; ++k) t = f2_fma(v[k], v[k], t);
+      s[i] = halves_sum(t);
+    }
+  };
+  float mean[2 * R] = {}, rstd[2 * R], next_mean[2 * R] = {};
+  auto deviations = [&](const float* s) {
+#pragma unroll
+    for (int i = 0; i < 2 * R; ++i) rstd[i] = kKind[i & 1] == kNone ? 1.f : rsqrtf(s[i] * p.inv_h + p.eps);
+  };
+  auto hat = [&](const uint4* slot, int i, uint64_t (&v)[P]) {  // normalised row i >> 1 of residual_out or x
+    load(slot, i & 1 ? 0 : 1, i >> 1, v);
+    if (kKind[i & 1] == kLayer) centre<NV>(v, mean[i], in);
+    if (kKind[i & 1] != kNone) {
+#pragma unroll
+      for (int k = 0; k < P; ++k) v[k] = f2_mul(v[k], both(rstd[i]));
+    }
+  };
+  auto pair_sums = [&](const uint64_t (&g)[P], const uint64_t (&h)[P], float* s) {
+    uint64_t t = g[0], u = f2_mul(g[0], h[0]);
+#pragma unroll
+    for (int k = 1; k < P; ++k) {
+      t = f2_add(t, g[k]);
+      u = f2_fma(g[k], h[k], u);
+    }
+    s[0] = halves_sum(t);
+    s[1] = halves_sum(u);
+  };
+  auto behind = [&](int i, uint64_t (&g)[P], const uint64_t (&h)[P], const float* s) {
+    const float k = rstd[i];
+    const uint64_t c1 = both(-k * (s[1] * p.inv_h)), k2 = both(k);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const uint64_t c0 = both(in[j] && kKind[i & 1] == kLayer ? -k * (s[0] * p.inv_h) : 0.f);
+#pragma unroll
+      for (int q = 4 * j; q < 4 * j + 4; ++q) g[q] = f2_fma(g[q], k2, f2_fma(h[q], c1, c0));
+    }
+  };
+  {  // the first group's statistics
+    wait(0, 0);
+    clear_missing(rows_slot(0), first);
+    float s[2 * R];
+    if (kMeans) {
+      sums_of(rows_slot(0), s);
+      row_sum<2 * R, false>(s, buf, turn);
+#pragma unroll
+      for (int i = 0; i < 2 * R; ++i) mean[i] = s[i] * p.inv_h;
+    }
+    if (kSquares) {
+      squares_of(rows_slot(0), mean, s);
+      row_sum<2 * R, false>(s, buf, turn);
+    }
+    deviations(s);
+  }
+  long long row = first;
+  int slot = 0, next = 1, gslot = 0;  // slots of this group's rows, the next one's and this group's gradients
+  uint32_t use = 0, next_use = 0, guse = 0;
+  for (; row < end; row += step) {
+    const bool more = row + step < end;
+    const uint4 *xr = rows_slot(slot), *xn = rows_slot(next), *g = grads_slot(gslot);
+    wait(3 + gslot, guse);
+    clear_missing(grads_slot(gslot), row);
+    if (more) {
+      wait(next, next_use);
+      clear_missing(rows_slot(next), row + step);
+    }
+    auto store = [&](__nv_bfloat16* out, int r, const uint64_t (&v)[P]) {
+      out += (row + r) * p.H + c;
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+        if (in[j] && (R == 1 || row + r < end)) __stcs(reinterpret_cast<uint4*>(out + j * stride), pack_pairs(&v[4 * j]));
+    };
+    uint64_t d[R][P], h[R][P], v[P];
+    float s[4 * R] = {};  // this group's sums, the next one's
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      hat(xr, 2 * r, h[r]);
+      load(g, 1, r, d[r]);
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        sum_m[i] = f2_fma(d[r][i], h[r][i], sum_m[i]);
+        sum_d[i] = f2_add(sum_d[i], d[r][i]);
+        d[r][i] = f2_mul(d[r][i], w.mul[i]);
+      }
+      if (kNorm != kNone) pair_sums(d[r], h[r], &s[2 * r]);
+    }
+    if constexpr (kMeans) {
+      if (more) sums_of(xn, s + 2 * R);
+      row_sum<4 * R, false>(s, buf, turn);
+#pragma unroll
+      for (int i = 0; i < 2 * R; ++i) next_mean[i] = s[2 * R + i] * p.inv_h;
+    } else if constexpr (kNorm != kNone) {
+      float t[2 * R];
+#pragma unroll
+      for (int i = 0; i < 2 * R; ++i) t[i] = s[i];
+      row_sum<2 * R, false>(t, buf, turn);
+#pragma unroll
+      for (int i = 0; i < 2 * R; ++i) s[i] = t[i];
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (kNorm != kNone) behind(2 * r, d[r], h[r], &s[2 * r]);
+      load(g, 0, r, v);
+#pragma unroll
+      for (int i = 0; i < P; ++i) d[r][i] = f2_add(d[r][i], v[i]);
+      store(p.out1, r, d[r]);
+      hat(xr, 2 * r + 1, h[r]);
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        sum_a[i] = f2_fma(d[r][i], h[r][i], sum_a[i]);
+        d[r][i] = f2_mul(d[r][i], w.gw[i]);
+      }
+      s[2 * r] = s[2 * r + 1] = 0.f;
+      if (kPost != kNone) pair_sums(d[r], h[r], &s[2 * r]);
+    }
+    bool bad;
+    if constexpr (kSquares) {
+      if (more) squares_of(xn, next_mean, s + 2 * R);
+      bad = row_sum<4 * R, false, true>(s, buf, turn, !ok);
+    } else {
+      bad = __syncthreads_or(!ok);
+    }
+    if (bad) break;
+    if (threadIdx.x == 0) {  // every thread has read this group's slots
+      fence_proxy_async_smem();
+      issue(p.d_res, p.d_out, row + 2 * step, grads_slot(gslot), &full[3 + gslot]);
+      issue(p.x, p.residual, row + 3 * step, rows_slot(slot), &full[slot]);
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (kPost != kNone) behind(2 * r + 1, d[r], h[r], &s[2 * r]);
+      store(p.out0, r, d[r]);
+    }
+#pragma unroll
+    for (int i = 0; i < 2 * R; ++i) mean[i] = next_mean[i];
+    deviations(s + 2 * R);
+    slot = next;
+    use = next_use;
+    if (++next == 3) {
+      next = 0;
+      ++next_use;
+    }
+    if (++gslot == 2) {
+      gslot = 0;
+      ++guse;
+    }
+  }
+  if (abort_flag && threadIdx.x == 0) {  // copies still in flight into this CTA's memory: of groups from `row` on
+    int ignored = 0;
+    for (int i = 0; i < 3 && row + i * step < end; ++i) {
+      mbar_wait(&full[slot], use & 1, &ignored, p.status, VOMNI_DEV_TIMEOUT_BASE + kSiteRowDrain);
+      if (i < 2) mbar_wait(&full[3 + gslot], guse & 1, &ignored, p.status, VOMNI_DEV_TIMEOUT_BASE + kSiteRowDrain);
+      if (++slot == 3) {
+        slot = 0;
+        ++use;
+      }
+      if (++gslot == 2) {
+        gslot = 0;
+        ++guse;
+      }
+    }
+  }
+  pdl_trigger();  // the sums' launch may get ready while the last rows end
+  store_sums<C>(p.parts + (static_cast<long long>(blockIdx.y) * gridDim.x + blockIdx.x) * 3 * p.H + c, p.H, stride, in, sum_a,
+                sum_m, sum_d);
+}
+
 // Short rows (H <= 256): a row per warp, four warps a CTA, straight from global memory.
 template <bool kBackward>
 __global__ void __launch_bounds__(128) sandwich_warp_kernel(const __grid_constant__ Params p) {
@@ -655,34 +925,43 @@ Shape shape_of(long long rows_per_mod, long long n_mod, int h, int tensors, bool
 
 typedef void (*Kernel)(Params);
 
-// The backward kernels that know their norms at compile time (430 us instead of 574 at 32760 x 5120): those of a call
-// with a branch and both gradients.
-template <int R, int NV, int kMaxThreads, bool kFull>
+bool all_given(const Params& p) { return p.x && p.d_res && p.d_out; }
+
+// The backward kernels that know their norms at compile time (430 us instead of 574 at 32760 x 5120 when both were the same
+// kernel): those of a call with a branch and both gradients. Two rows at a time: sandwich_bwd_kernel; one: sandwich_kernel.
+template <int R, bool kFull, int kPost, int kNorm>
+Kernel backward_kind() {
+  if constexpr (R == 2)
+    return sandwich_bwd_kernel<2, 2, 320, kFull, kPost, kNorm>;
+  else
+    return sandwich_kernel<1, 2, 512, kFull, true, kPost, kNorm, true>;
+}
+template <int R, bool kFull>
 Kernel backward_of(const Params& p) {
-  if (!p.x || !p.d_res || !p.d_out) return sandwich_kernel<R, NV, kMaxThreads, kFull, true>;
   switch (p.post * 3 + p.norm) {
-    case 0: return sandwich_kernel<R, NV, kMaxThreads, kFull, true, 0, 0, true>;
-    case 1: return sandwich_kernel<R, NV, kMaxThreads, kFull, true, 0, 1, true>;
-    case 2: return sandwich_kernel<R, NV, kMaxThreads, kFull, true, 0, 2, true>;
-    case 3: return sandwich_kernel<R, NV, kMaxThreads, kFull, true, 1, 0, true>;
-    case 4: return sandwich_kernel<R, NV, kMaxThreads, kFull, true, 1, 1, true>;
-    case 5: return sandwich_kernel<R, NV, kMaxThreads, kFull, true, 1, 2, true>;
-    case 6: return sandwich_kernel<R, NV, kMaxThreads, kFull, true, 2, 0, true>;
-    case 7: return sandwich_kernel<R, NV, kMaxThreads, kFull, true, 2, 1, true>;
-    default: return sandwich_kernel<R, NV, kMaxThreads, kFull, true, 2, 2, true>;
+    case 0: return backward_kind<R, kFull, 0, 0>();
+    case 1: return backward_kind<R, kFull, 0, 1>();
+    case 2: return backward_kind<R, kFull, 0, 2>();
+    case 3: return backward_kind<R, kFull, 1, 0>();
+    case 4: return backward_kind<R, kFull, 1, 1>();
+    case 5: return backward_kind<R, kFull, 1, 2>();
+    case 6: return backward_kind<R, kFull, 2, 0>();
+    case 7: return backward_kind<R, kFull, 2, 1>();
+    default: return backward_kind<R, kFull, 2, 2>();
   }
 }
 
 // Rows at a time and chunks a thread. The reductions cost a warp the same for one value a thread as for many and all
 // warps wait for each other in them, so more of both is better while registers and shared memory last. Measured at
-// 32760 x 5120: forward 393 / 299 / 228 us with 1 / 2 / 4 rows of one chunk; backward 402 us with two rows of one
-// chunk (640 threads), 381 us with two rows of two (320), 624 us with one row of two, 740 us with one row of four.
+// 32760 x 5120: forward 393 / 299 / 228 us with 1 / 2 / 4 rows of one chunk; backward (sandwich_kernel) 402 us with two rows
+// of one chunk (640 threads), 383 us with two rows of two (320), 624 us with one row of two, 740 us with one row of four.
 template <bool kBackward>
 Kernel kernel_of(const Params& p, const Shape& s) {
   const bool full = s.threads * s.nv * 8 == p.H;
   if constexpr (kBackward) {
-    if (s.rows == 2) return full ? backward_of<2, 2, 320, true>(p) : backward_of<2, 2, 320, false>(p);
-    if (s.nv == 2) return backward_of<1, 2, 512, false>(p);
+    const bool all = all_given(p);
+    if (s.rows == 2) return !all ? sandwich_kernel<2, 2, 320, false, true> : full ? backward_of<2, true>(p) : backward_of<2, false>(p);
+    if (s.nv == 2) return all ? backward_of<1, false>(p) : sandwich_kernel<1, 2, 512, false, true>;
     return sandwich_kernel<1, 1, 640, false, true>;
   } else {
     if (s.rows == 4) return full ? sandwich_kernel<4, 1, 640, true, false> : sandwich_kernel<4, 1, 640, false, false>;
@@ -699,10 +978,13 @@ int launch(Params p, long long n_mod, const Shape& s, cudaStream_t st) {
   if (s.warp_row) {
     sandwich_warp_kernel<kBackward><<<grid, dim3(32, 4), 0, st>>>(p);
   } else {
+    // sandwich_bwd_kernel: three slots of two tensors and two of the others (at most 200 KB an SM for the CTAs that
+    // shape_of counts: per_sm <= 5120 / H)
+    const size_t smem = kBackward && s.rows == 2 && all_given(p) ? static_cast<size_t>(10) * s.rows * p.H * 2 : s.smem;
     const Kernel kern = kernel_of<kBackward>(p, s);
-    int rc = ensure_max_smem(kern, static_cast<int>(s.smem));
+    int rc = ensure_max_smem(kern, static_cast<int>(smem));
     if (rc) return rc;
-    kern<<<grid, s.threads, s.smem, st>>>(p);
+    kern<<<grid, s.threads, smem, st>>>(p);
   }
   VOMNI_CUDA_TRY(cudaGetLastError());
   return VOMNI_OK;
