@@ -82,39 +82,44 @@ VOMNI_DEV float warp_fold(float (&v)[N]) {
   return v[0];
 }
 
-// Sums N values over the threads that share a row (or a few rows): one warp (kWarpRow), or the whole CTA through
+// Sums N values over the threads that share a row (or a few rows): kLanes lanes of a warp, or (0) the whole CTA through
 // shared memory. Every thread ends with the same sums, added in an order that only the CTA's size sets. `turn`
 // alternates between two buffers: a buffer is written again only after a barrier that follows its last read. Entries
 // of warps that the CTA does not have are zero from the start. Returns whether any thread said `bad` (kVote).
-template <int N, bool kWarpRow, bool kVote = false>
+template <int N, int kLanes, bool kVote = false>
 VOMNI_DEV bool row_sum(float (&v)[N], float (*buf)[kBuf], int& turn, bool bad = false) {
+  if constexpr (kLanes > 0) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int o = kLanes / 2; o > 0; o /= 2) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+    return bad;
+  }
   constexpr int kGroup = 32 / N;
   const int lane = threadIdx.x & 31;
   float s = warp_fold<N>(v);
-  if (!kWarpRow) {
-    float* b = buf[turn];
-    turn ^= 1;
-    if (lane % kGroup == 0) b[lane / kGroup * 32 + (threadIdx.x >> 5)] = s;
-    if (kVote)
-      bad = __syncthreads_or(bad);
-    else
-      __syncthreads();
-    b += lane * N;  // value lane / kGroup, N of its 32 warps
-    if constexpr (N == 8) {
-      const float4 x = reinterpret_cast<const float4*>(b)[0], y = reinterpret_cast<const float4*>(b)[1];
-      s = ((x.x + x.y) + (x.z + x.w)) + ((y.x + y.y) + (y.z + y.w));
-    } else if constexpr (N == 4) {
-      const float4 x = *reinterpret_cast<const float4*>(b);
-      s = (x.x + x.y) + (x.z + x.w);
-    } else if constexpr (N == 2) {
-      const float2 x = *reinterpret_cast<const float2*>(b);
-      s = x.x + x.y;
-    } else {
-      s = b[0];
-    }
-#pragma unroll
-    for (int o = kGroup / 2; o > 0; o /= 2) s += __shfl_xor_sync(0xffffffffu, s, o);
+  float* b = buf[turn];
+  turn ^= 1;
+  if (lane % kGroup == 0) b[lane / kGroup * 32 + (threadIdx.x >> 5)] = s;
+  if (kVote)
+    bad = __syncthreads_or(bad);
+  else
+    __syncthreads();
+  b += lane * N;  // value lane / kGroup, N of its 32 warps
+  if constexpr (N == 8) {
+    const float4 x = reinterpret_cast<const float4*>(b)[0], y = reinterpret_cast<const float4*>(b)[1];
+    s = ((x.x + x.y) + (x.z + x.w)) + ((y.x + y.y) + (y.z + y.w));
+  } else if constexpr (N == 4) {
+    const float4 x = *reinterpret_cast<const float4*>(b);
+    s = (x.x + x.y) + (x.z + x.w);
+  } else if constexpr (N == 2) {
+    const float2 x = *reinterpret_cast<const float2*>(b);
+    s = x.x + x.y;
+  } else {
+    s = b[0];
   }
+#pragma unroll
+  for (int o = kGroup / 2; o > 0; o /= 2) s += __shfl_xor_sync(0xffffffffu, s, o);
 #pragma unroll
   for (int i = 0; i < N; ++i) v[i] = __shfl_sync(0xffffffffu, s, i * kGroup);
   return bad;
@@ -145,7 +150,7 @@ VOMNI_DEV void centre(uint64_t (&v)[NV * 4], float mean, const bool (&in)[NV]) {
 
 // x -> its normalised values. Two passes (mean, then squared deviations) in fp32. Columns behind
 // the row's end (whole chunks: in[j] false) hold zeros before and after.
-template <int R, int C, bool kWarpRow>
+template <int R, int C, int kLanes>
 VOMNI_DEV void normalise(Vals<R, C>& x, int kind, const bool (&in)[C / 8], const Params& p, float (*buf)[kBuf],
                          int& turn) {
   if (kind == kNone) return;
@@ -158,7 +163,7 @@ VOMNI_DEV void normalise(Vals<R, C>& x, int kind, const bool (&in)[C / 8], const
       for (int i = 1; i < C / 2; ++i) t = f2_add(t, x.v[r][i]);
       s[r] = halves_sum(t);
     }
-    row_sum<R, kWarpRow>(s, buf, turn);
+    row_sum<R, kLanes>(s, buf, turn);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
 #pragma unroll
@@ -176,7 +181,7 @@ VOMNI_DEV void normalise(Vals<R, C>& x, int kind, const bool (&in)[C / 8], const
     for (int i = 1; i < C / 2; ++i) t = f2_fma(x.v[r][i], x.v[r][i], t);
     s[r] = halves_sum(t);
   }
-  row_sum<R, kWarpRow>(s, buf, turn);
+  row_sum<R, kLanes>(s, buf, turn);
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const uint64_t rstd = both(rsqrtf(s[r] * p.inv_h + p.eps));
@@ -289,7 +294,7 @@ VOMNI_DEV void load_vecs(const Params& p, long long mod, int c, int stride, cons
 
 // One group of R rows, forward. load(t, r, v): the thread's values of row r of tensor t (0 x, 1 residual; zero behind the
 // row's end); store(t, r, v): to output t.
-template <int R, int NV, bool kWarpRow, typename Load, typename Store>
+template <int R, int NV, int kLanes, typename Load, typename Store>
 VOMNI_DEV void forward_rows(const Params& p, const Vecs<NV * 8>& w, const bool (&in)[NV], float (*buf)[kBuf], int& turn,
                             Load&& load, Store&& store) {
   constexpr int C = NV * 8;
@@ -297,7 +302,7 @@ VOMNI_DEV void forward_rows(const Params& p, const Vecs<NV * 8>& w, const bool (
 #pragma unroll
   for (int r = 0; r < R; ++r) load(p.x ? 0 : 1, r, x.v[r]);
   if (p.x) {
-    normalise<R, C, kWarpRow>(x, p.post, in, p, buf, turn);
+    normalise<R, C, kLanes>(x, p.post, in, p, buf, turn);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       uint64_t res[C / 2];
@@ -307,7 +312,7 @@ VOMNI_DEV void forward_rows(const Params& p, const Vecs<NV * 8>& w, const bool (
       store(0, r, x.v[r]);
     }
   }
-  normalise<R, C, kWarpRow>(x, p.norm, in, p, buf, turn);
+  normalise<R, C, kLanes>(x, p.norm, in, p, buf, turn);
 #pragma unroll
   for (int r = 0; r < R; ++r) {
 #pragma unroll
@@ -321,7 +326,7 @@ VOMNI_DEV void forward_rows(const Params& p, const Vecs<NV * 8>& w, const bool (
 // slot again for each of their statistics instead of being kept: the accumulators and vectors leave registers for two
 // tensors of values.
 // kPost, kNorm: the kinds, or kAsked to go by the call's; kAll: x, d_res and d_out are all there.
-template <int R, int NV, bool kWarpRow, int kPost, int kNorm, bool kAll, typename Load, typename Store>
+template <int R, int NV, int kLanes, int kPost, int kNorm, bool kAll, typename Load, typename Store>
 VOMNI_DEV void backward_rows(const Params& p, const Vecs<NV * 8>& w, const bool (&in)[NV], float (*buf)[kBuf], int& turn,
                              uint64_t (&sum_a)[NV * 4], uint64_t (&sum_m)[NV * 4], uint64_t (&sum_d)[NV * 4], Load&& load,
                              Store&& store) {
@@ -353,7 +358,7 @@ VOMNI_DEV void backward_rows(const Params& p, const Vecs<NV * 8>& w, const bool 
         for (int i = 1; i < P; ++i) t = f2_add(t, v[i]);
         s[2 * r + q] = halves_sum(t);
       }
-    row_sum<2 * R, kWarpRow>(s, buf, turn);
+    row_sum<2 * R, kLanes>(s, buf, turn);
 #pragma unroll
     for (int i = 0; i < 2 * R; ++i) mean[i] = s[i] * p.inv_h;
   }
@@ -371,7 +376,7 @@ VOMNI_DEV void backward_rows(const Params& p, const Vecs<NV * 8>& w, const bool 
         for (int i = 1; i < P; ++i) t = f2_fma(v[i], v[i], t);
         s[2 * r + q] = halves_sum(t);
       }
-    row_sum<2 * R, kWarpRow>(s, buf, turn);
+    row_sum<2 * R, kLanes>(s, buf, turn);
   }
 #pragma unroll
   for (int i = 0; i < 2 * R; ++i) rstd[i] = kind[i & 1] == kNone ? 1.f : rsqrtf(s[i] * p.inv_h + p.eps);
@@ -413,7 +418,7 @@ VOMNI_DEV void backward_rows(const Params& p, const Vecs<NV * 8>& w, const bool 
       pair_sums(r, d[r], h[r]);
     }
     if (kind[0] != kNone) {
-      row_sum<2 * R, kWarpRow>(s, buf, turn);
+      row_sum<2 * R, kLanes>(s, buf, turn);
 #pragma unroll
       for (int r = 0; r < R; ++r) behind(0, r, d[r], h[r]);
     }
@@ -438,7 +443,7 @@ VOMNI_DEV void backward_rows(const Params& p, const Vecs<NV * 8>& w, const bool 
     pair_sums(r, d[r], h[r]);
   }
   if (!has_x) return;
-  if (kind[1] != kNone) row_sum<2 * R, kWarpRow>(s, buf, turn);
+  if (kind[1] != kNone) row_sum<2 * R, kLanes>(s, buf, turn);
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     if (kind[1] != kNone) behind(1, r, d[r], h[r]);
@@ -463,7 +468,7 @@ VOMNI_DEV uint4 pack_pairs(const uint64_t* v) {
 }
 
 template <int C>
-VOMNI_DEV void store_sums(float* part, int H, int stride, const bool (&in)[C / 8], const uint64_t (&a)[C / 2],
+VOMNI_DEV void store_sums(float* part, int pitch, int stride, const bool (&in)[C / 8], const uint64_t (&a)[C / 2],
                           const uint64_t (&m)[C / 2], const uint64_t (&d)[C / 2]) {
 #pragma unroll
   for (int q = 0; q < 3; ++q) {
@@ -471,7 +476,7 @@ VOMNI_DEV void store_sums(float* part, int H, int stride, const bool (&in)[C / 8
 #pragma unroll
     for (int j = 0; j < C / 8; ++j) {
       if (!in[j]) continue;
-      ulonglong2* at = reinterpret_cast<ulonglong2*>(part + static_cast<size_t>(q) * H + j * stride);
+      ulonglong2* at = reinterpret_cast<ulonglong2*>(part + static_cast<size_t>(q) * pitch + j * stride);
       at[0] = make_ulonglong2(s[4 * j], s[4 * j + 1]);
       at[1] = make_ulonglong2(s[4 * j + 2], s[4 * j + 3]);
     }
@@ -528,9 +533,9 @@ __global__ void __launch_bounds__(kMaxThreads, 1) sandwich_kernel(const __grid_c
         if (in[j] && (R == 1 || r < rows)) __stcs(reinterpret_cast<uint4*>(out + j * stride), pack_pairs(&x[4 * j]));
     };
     if constexpr (kBackward)
-      backward_rows<R, NV, false, kPost, kNorm, kAll>(p, w, in, buf, turn, sum_a, sum_m, sum_d, load, store);
+      backward_rows<R, NV, 0, kPost, kNorm, kAll>(p, w, in, buf, turn, sum_a, sum_m, sum_d, load, store);
     else
-      forward_rows<R, NV, false>(p, w, in, buf, turn, load, store);
+      forward_rows<R, NV, 0>(p, w, in, buf, turn, load, store);
   });
   if constexpr (kBackward) {
     pdl_trigger();  // the sums' launch may get ready while the last rows end
@@ -677,13 +682,13 @@ __global__ void __launch_bounds__(kMaxThreads, 1) sandwich_bwd_kernel(const __gr
     float s[2 * R];
     if (kMeans) {
       sums_of(rows_slot(0), s);
-      row_sum<2 * R, false>(s, buf, turn);
+      row_sum<2 * R, 0>(s, buf, turn);
 #pragma unroll
       for (int i = 0; i < 2 * R; ++i) mean[i] = s[i] * p.inv_h;
     }
     if (kSquares) {
       squares_of(rows_slot(0), mean, s);
-      row_sum<2 * R, false>(s, buf, turn);
+      row_sum<2 * R, 0>(s, buf, turn);
     }
     deviations(s);
   }
@@ -721,14 +726,14 @@ __global__ void __launch_bounds__(kMaxThreads, 1) sandwich_bwd_kernel(const __gr
     }
     if constexpr (kMeans) {
       if (more) sums_of(xn, s + 2 * R);
-      row_sum<4 * R, false>(s, buf, turn);
+      row_sum<4 * R, 0>(s, buf, turn);
 #pragma unroll
       for (int i = 0; i < 2 * R; ++i) next_mean[i] = s[2 * R + i] * p.inv_h;
     } else if constexpr (kNorm != kNone) {
       float t[2 * R];
 #pragma unroll
       for (int i = 0; i < 2 * R; ++i) t[i] = s[i];
-      row_sum<2 * R, false>(t, buf, turn);
+      row_sum<2 * R, 0>(t, buf, turn);
 #pragma unroll
       for (int i = 0; i < 2 * R; ++i) s[i] = t[i];
     }
@@ -751,7 +756,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) sandwich_bwd_kernel(const __gr
     bool bad;
     if constexpr (kSquares) {
       if (more) squares_of(xn, next_mean, s + 2 * R);
-      bad = row_sum<4 * R, false, true>(s, buf, turn, !ok);
+      bad = row_sum<4 * R, 0, true>(s, buf, turn, !ok);
     } else {
       bad = __syncthreads_or(!ok);
     }
@@ -800,38 +805,63 @@ __global__ void __launch_bounds__(kMaxThreads, 1) sandwich_bwd_kernel(const __gr
                 sum_m, sum_d);
 }
 
-// Short rows (H <= 256): a row per warp, four warps a CTA, straight from global memory.
-template <bool kBackward>
-__global__ void __launch_bounds__(128) sandwich_warp_kernel(const __grid_constant__ Params p) {
-  const int c = threadIdx.x * 8;
+// Short rows (H <= 256): kLanes lanes a row, 32 / kLanes rows a warp, straight from global memory, the next rows' loads
+// under way meanwhile. The column sums are added in the CTA, in order: a part per warp left the sums' kernel thousands to add.
+// Backward (with 6 us of two launches): 200000 x 128 68 us instead of 172 with a row and a part a warp and no loads ahead, 98280 x 256
+// 68 instead of 102, 20000 x 64 14 instead of 41.
+constexpr int kRowWarps = 8;
+template <bool kBackward, int kLanes>
+__global__ void __launch_bounds__(32 * kRowWarps) sandwich_warp_kernel(const __grid_constant__ Params p) {
+  constexpr int kRows = 32 / kLanes;  // of a warp
+  const int sub = threadIdx.x / kLanes, c = threadIdx.x % kLanes * 8;
   const bool in[1] = {c < p.H};
   const long long end = (static_cast<long long>(blockIdx.y) + 1) * p.rows_per_mod;
-  const int lanes = gridDim.x * blockDim.y, lane = blockIdx.x * blockDim.y + threadIdx.y;
   Vecs<8> w;
   load_vecs<8>(p, blockIdx.y, c, 0, in, w);
   uint64_t sum_a[4] = {}, sum_m[4] = {}, sum_d[4] = {};
   int turn = 0;
-  const __nv_bfloat16* src[4] = {p.x, p.residual, p.d_res, p.d_out};
-  for (long long row = static_cast<long long>(blockIdx.y) * p.rows_per_mod + lane; row < end; row += lanes) {
-    const long long at = row * p.H + c;
-    uint4 raw[4];
+  const __nv_bfloat16* src[4] = {p.x, (kBackward && !p.d_out) ? nullptr : p.residual, p.d_res, p.d_out};
+  constexpr int kTensors = kBackward ? 4 : 2;
+  uint4 next[kTensors];
+  auto fetch = [&](long long row) {  // zeros for rows behind the last
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      raw[t] = make_uint4(0, 0, 0, 0);
-      if (in[0] && src[t]) raw[t] = __ldcs(reinterpret_cast<const uint4*>(src[t] + at));
+    for (int t = 0; t < kTensors; ++t) {
+      next[t] = make_uint4(0, 0, 0, 0);
+      if (in[0] && row < end && src[t]) next[t] = __ldcs(reinterpret_cast<const uint4*>(src[t] + row * p.H + c));
     }
+  };
+  const int step = static_cast<int>(gridDim.x) * kRowWarps * kRows;
+  long long first = static_cast<long long>(blockIdx.y) * p.rows_per_mod + (blockIdx.x * kRowWarps + threadIdx.y) * kRows;  // the warp's
+  fetch(first + sub);
+  for (; first < end; first += step) {
+    const long long row = first + sub;
+    uint4 raw[kTensors];
+#pragma unroll
+    for (int t = 0; t < kTensors; ++t) raw[t] = next[t];
+    fetch(row + step);
     auto load = [&](int t, int, uint64_t (&x)[4]) { unpack_pairs(raw[t], x); };
     auto store = [&](int t, int, const uint64_t (&x)[4]) {
-      if (in[0]) __stcs(reinterpret_cast<uint4*>((t ? p.out1 : p.out0) + at), pack_pairs(x));
+      if (in[0] && row < end) __stcs(reinterpret_cast<uint4*>((t ? p.out1 : p.out0) + row * p.H + c), pack_pairs(x));
     };
     if constexpr (kBackward)
-      backward_rows<1, 1, true, kAsked, kAsked, false>(p, w, in, nullptr, turn, sum_a, sum_m, sum_d, load, store);
+      backward_rows<1, 1, kLanes, kAsked, kAsked, false>(p, w, in, nullptr, turn, sum_a, sum_m, sum_d, load, store);
     else
-      forward_rows<1, 1, true>(p, w, in, nullptr, turn, load, store);
+      forward_rows<1, 1, kLanes>(p, w, in, nullptr, turn, load, store);
   }
   if constexpr (kBackward) {
     pdl_trigger();
-    store_sums<8>(p.parts + (static_cast<long long>(blockIdx.y) * lanes + lane) * 3 * p.H + c, p.H, 0, in, sum_a, sum_m, sum_d);
+    __shared__ __align__(16) float red[kRowWarps * kRows][3][8 * kLanes];
+    const bool every[1] = {true};
+    store_sums<8>(&red[threadIdx.y * kRows + sub][0][0] + c, 8 * kLanes, 0, every, sum_a, sum_m, sum_d);
+    __syncthreads();
+    float* part = p.parts + (static_cast<long long>(blockIdx.y) * gridDim.x + blockIdx.x) * 3 * p.H;
+    for (int i = threadIdx.y * 32 + threadIdx.x; i < 3 * p.H; i += 32 * kRowWarps) {
+      const int q = i / p.H, col = i - q * p.H;
+      float t = red[0][q][col];
+#pragma unroll
+      for (int k = 1; k < kRowWarps * kRows; ++k) t += red[k][q][col];
+      part[i] = t;
+    }
   }
 }
 
@@ -886,11 +916,11 @@ __global__ void __launch_bounds__(1024) sandwich_sum_kernel(const __grid_constan
   }
 }
 
-// How a call is laid out: a row per warp, or R rows at a time per CTA with NV chunks a thread.
+// How a call is laid out: a row or more per warp, or R rows at a time per CTA with NV chunks a thread.
 struct Shape {
-  bool warp_row;
+  int row_lanes;  // of a row that is part of a warp, else 0
   int nv, rows, threads;  // rows: R
-  int lanes;              // CTAs (x warps) that share a modulation row's tokens
+  int lanes;              // CTAs that share a modulation row's tokens
   unsigned blocks;        // gridDim.x
   int slots;
   size_t smem;
@@ -898,11 +928,13 @@ struct Shape {
 Shape shape_of(long long rows_per_mod, long long n_mod, int h, int tensors, bool backward) {
   Shape s = {};
   const int chunks = h / 8;
-  s.warp_row = chunks <= 32;
-  if (s.warp_row) {
-    const long long need = (rows_per_mod + 3) / 4, cap = (static_cast<long long>(num_sms()) * 8 + n_mod - 1) / n_mod;
+  s.row_lanes = chunks <= 8 ? 8 : chunks <= 16 ? 16 : chunks <= 32 ? 32 : 0;
+  if (s.row_lanes) {
+    const int rows = kRowWarps * 32 / s.row_lanes;  // of a CTA at a time; two or four CTAs fit an SM
+    const long long need = (rows_per_mod + rows - 1) / rows;
+    const long long cap = (static_cast<long long>(num_sms()) * (backward ? 2 : 4) + n_mod - 1) / n_mod;
     s.blocks = static_cast<unsigned>(need < cap ? need : cap);
-    s.lanes = static_cast<int>(s.blocks) * 4;
+    s.lanes = static_cast<int>(s.blocks);
     return s;
   }
   // Few rows: one at a time, so that they spread over the device. Else a thread of the backward pass takes two chunks
@@ -975,8 +1007,11 @@ int launch(Params p, long long n_mod, const Shape& s, cudaStream_t st) {
   p.slots = s.slots;
   p.status = device_status_ptr();
   const dim3 grid(s.blocks, static_cast<unsigned>(n_mod));
-  if (s.warp_row) {
-    sandwich_warp_kernel<kBackward><<<grid, dim3(32, 4), 0, st>>>(p);
+  if (s.row_lanes) {
+    const Kernel kern = s.row_lanes == 8    ? sandwich_warp_kernel<kBackward, 8>
+                        : s.row_lanes == 16 ? sandwich_warp_kernel<kBackward, 16>
+                                            : sandwich_warp_kernel<kBackward, 32>;
+    kern<<<grid, dim3(32, kRowWarps), 0, st>>>(p);
   } else {
     // sandwich_bwd_kernel: three slots of two tensors and two of the others (at most 200 KB an SM for the CTAs that
     // shape_of counts: per_sm <= 5120 / H)
