@@ -496,8 +496,10 @@ __global__ void __launch_bounds__(kMaxThreads, 1) sandwich_kernel(const __grid_c
   int turn = 0;
   const int c = threadIdx.x * 8, stride = blockDim.x * 8;
   bool in[NV];
+  // Of two chunks the first is always there (shape_of: threads <= H / 8 then). Not in the backward pass of one row at a time,
+  // which spills without the predicates: 16384 x 8192 430 us instead of 399, forward 223 instead of 238.
 #pragma unroll
-  for (int j = 0; j < NV; ++j) in[j] = kFull || c + j * stride < p.H;
+  for (int j = 0; j < NV; ++j) in[j] = kFull || (NV > 1 && j == 0 && !kBackward) || c + j * stride < p.H;
   const __nv_bfloat16* src[4] = {p.x, (kBackward && !p.d_out) ? nullptr : p.residual, p.d_res, p.d_out};
   int at[4], tensors = 0;
 #pragma unroll
@@ -587,8 +589,9 @@ __global__ void __launch_bounds__(kMaxThreads, 1) sandwich_bwd_kernel(const __gr
     }
   }
   bool in[NV];
+  // of two chunks the first is always there (shape_of: threads <= H / 8 then): 16384 x 5000 195 us instead of 227
 #pragma unroll
-  for (int j = 0; j < NV; ++j) in[j] = kFull || c + j * stride < p.H;
+  for (int j = 0; j < NV; ++j) in[j] = kFull || (NV > 1 && j == 0) || c + j * stride < p.H;
   Vecs<C> w;
   load_vecs<C>(p, blockIdx.y, c, stride, in, w);
   uint64_t sum_a[P] = {}, sum_m[P] = {}, sum_d[P] = {};
