@@ -7,6 +7,7 @@ is missing or the device is not an sm_100 part, calls raise instead of computing
 from __future__ import annotations
 
 import ctypes
+import functools
 import threading
 from pathlib import Path
 
@@ -194,6 +195,12 @@ def launch(index: int, name: str, *args) -> None:
 def empty(t):
     """An uninitialised dense tensor of ``t``'s shape, dtype and device (``empty_like`` takes half of ``new_empty``'s time)."""
     return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
+@functools.lru_cache(maxsize=256)
+def workspace_bytes(index: int, name: str, *sizes) -> int:
+    """The workspace that entry point ``name`` asks for, on device ``index``: a function of the sizes (and the device's) alone."""
+    return on_device(index, getattr(load(), f"{name}_workspace_bytes"), *sizes)
 
 
 def workspace(n: int, device) -> torch.Tensor:

@@ -416,11 +416,11 @@ def attention_bwd(grad_o: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: tor
     lse = _lib.dense(lse.float())
     if grad_lse is not None:
         grad_lse = _lib.dense(grad_lse.float())
-    if q_lens is not None:
-        q_lens = (ctypes.c_int * b)(*q_lens)
-    if kv_lens is not None:
-        kv_lens = (ctypes.c_int * b)(*kv_lens)
-    ws_bytes = _lib.on_device(dev, _lib.load().vomni_attention_bwd_workspace_bytes, b, sq, skv, hq, hkv, _HEAD_DIM, q_lens, kv_lens)
+    if q_lens is None and kv_lens is None:
+        ws_bytes = _lib.workspace_bytes(dev, "vomni_attention_bwd", b, sq, skv, hq, hkv, _HEAD_DIM, None, None)
+    else:
+        q_lens, kv_lens = (n if n is None else (ctypes.c_int * b)(*n) for n in (q_lens, kv_lens))
+        ws_bytes = _lib.on_device(dev, _lib.load().vomni_attention_bwd_workspace_bytes, b, sq, skv, hq, hkv, _HEAD_DIM, q_lens, kv_lens)
     ws = _lib.workspace(ws_bytes, q.device)
     _lib.launch(dev, "vomni_attention_bwd_lse", grad_o.data_ptr(), None if grad_lse is None else grad_lse.data_ptr(), q.data_ptr(),
                 k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), b, sq, skv, hq, hkv, _HEAD_DIM, strides, q_lens, kv_lens,

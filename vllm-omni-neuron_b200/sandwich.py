@@ -137,7 +137,7 @@ def _backward(grad_res, grad_out, x, residual_out, gate, mul, add, post_weight, 
     make = torch.empty_like if rows else torch.zeros_like
     sums = [make(v) if v is not None and n else None for v, n in zip(vectors, need)]  # fp32 and dense, as the vectors now are
     if rows:
-        ws_bytes = _lib.on_device(dev, _lib.load().vomni_sandwich_norm_workspace_bytes, rows, hidden, per_mod)
+        ws_bytes = _lib.workspace_bytes(dev, "vomni_sandwich_norm", rows, hidden, per_mod)
         ws = _lib.workspace(ws_bytes, residual_out.device)
         gate, mul, _, post_weight = vectors
         dgate, dmul, dadd, dw = map(_ptr, sums)
