@@ -32,6 +32,14 @@ def test_short_rows(pkg, dev, lead, h):
         _check_backward(pkg, st, _check_forward(pkg, st, post, norm), post, norm)
 
 
+@pytest.mark.parametrize("per", [("gate", "mul", "add"), ("gate",), ("mul",), ("add",)])
+@pytest.mark.parametrize("lead,h", [((8, 3), 264), ((9, 2), 128), ((64, 1), 1536), ((65, 7), 72), ((333, 1), 2048), ((1000, 2), 264)])
+def test_many_modulation_rows(pkg, dev, lead, h, per):
+    """Up to one modulation row per token; the shared vectors' gradients are sums over all of them."""
+    st = _make(dev, lead, h, h + lead[0], per=per)
+    _check_backward(pkg, st, _check_forward(pkg, st, "rms_norm", "layer_norm"), "rms_norm", "layer_norm")
+
+
 @pytest.mark.parametrize("missing", ["grad_r", "grad_out", "x"])
 def test_parts_of_a_call(pkg, dev, missing):
     st = _make(dev, (3, 1001), 1536, 7, branch=missing != "x")

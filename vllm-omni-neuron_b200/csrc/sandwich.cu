@@ -869,13 +869,36 @@ __global__ void __launch_bounds__(32 * kRowWarps) sandwich_warp_kernel(const __g
 }
 
 struct SumParams {
-  const float* parts;  // [n_mod][lanes][3][H]
+  float* parts;  // [n_mod][lanes][3][H]
   const float* gate;
   const float* post_w;
   long long gate_step;
   int H, lanes, n_mod, per;  // per: kPer* flags
+  int mods;                  // modulation rows of a range
   float *dgate, *dpost_w, *dmul, *dadd;
 };
+
+// What the sum over all modulation rows gives: the shared vectors' gradients. For A it was weighed with a gate per
+// modulation row; a shared gate is constant in it.
+VOMNI_DEV void store_shared(const SumParams& p, int q, int col, float sum) {
+  float* out = q == 0 ? p.dgate : q == 1 ? p.dmul : p.dadd;
+  if (q == 0) {
+    const bool per = p.per & kPerGate;
+    if (p.dpost_w) p.dpost_w[col] = per || !p.gate ? sum : sum * p.gate[col];
+    if (out && !per) out[col] = p.post_w ? sum * p.post_w[col] : sum;
+  } else if (out && !(p.per & (q == 1 ? kPerMul : kPerAdd))) {
+    out[col] = sum;
+  }
+}
+
+// The gradient of one modulation row, where its vector has one per row; returns what is added over the rows.
+VOMNI_DEV float store_row(const SumParams& p, int q, int mod, int col, float t) {
+  float* out = q == 0 ? p.dgate : q == 1 ? p.dmul : p.dadd;
+  const bool per = p.per & (q == 0 ? kPerGate : q == 1 ? kPerMul : kPerAdd);
+  if (per && out) out[static_cast<long long>(mod) * p.H + col] = q == 0 && p.post_w ? t * p.post_w[col] : t;
+  return q == 0 && per && p.gate ? t * p.gate[mod * p.gate_step + col] : t;
+}
+VOMNI_DEV bool asked(const SumParams& p, int q) { return q == 0 ? p.dgate || p.dpost_w : q == 1 ? p.dmul != nullptr : p.dadd != nullptr; }
 
 // 32 columns x 32 lanes a CTA; blockIdx.y: A, M or D. Sums each modulation row's parts in the order lane, lane + 32, ...,
 // then the 32 lanes as a tree, and forms the outputs; those shared by the modulation rows are added over them in order.
@@ -884,11 +907,9 @@ __global__ void __launch_bounds__(1024) sandwich_sum_kernel(const __grid_constan
   __shared__ float red[32][33];
   const int col = blockIdx.x * 32 + threadIdx.x, q = blockIdx.y;
   const bool in = col < p.H;
-  float* out = q == 0 ? p.dgate : q == 1 ? p.dmul : p.dadd;
-  const bool per = p.per & (q == 0 ? kPerGate : q == 1 ? kPerMul : kPerAdd);
   pdl_wait();  // launched as a dependent of the rows' kernel
-  if (!out && !(q == 0 && p.dpost_w)) return;
-  float shared_out = 0.f, dw = 0.f;
+  if (!asked(p, q)) return;
+  float sum = 0.f;
   const int mine = blockIdx.x * 32 + threadIdx.y;  // the column whose lanes this warp adds
   for (int mod = 0; mod < p.n_mod; ++mod) {
     float s = 0.f;
@@ -902,21 +923,35 @@ __global__ void __launch_bounds__(1024) sandwich_sum_kernel(const __grid_constan
     float t = red[threadIdx.x][threadIdx.y];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-    if (threadIdx.x == 0 && mine < p.H) {
-      if (q == 0 && p.dpost_w) dw = fmaf(t, p.gate ? p.gate[mod * p.gate_step + mine] : 1.f, dw);
-      if (q == 0 && p.post_w) t *= p.post_w[mine];
-      if (per) {
-        if (out) out[static_cast<long long>(mod) * p.H + mine] = t;
-      } else {
-        shared_out += t;
-      }
-    }
+    if (threadIdx.x == 0 && mine < p.H) sum += store_row(p, q, mod, mine, t);
     __syncthreads();
   }
-  if (threadIdx.x == 0 && mine < p.H) {
-    if (out && !per) out[mine] = shared_out;
-    if (q == 0 && p.dpost_w) p.dpost_w[mine] = dw;
+  if (threadIdx.x == 0 && mine < p.H) store_shared(p, q, mine, sum);
+}
+
+// The same for many modulation rows, of which each then has few parts: a thread per column and range of `mods` rows
+// (blockIdx.z). Its sum over the rows goes to the range's first part (read by no other thread), sandwich_shared_kernel adds the ranges'.
+__global__ void __launch_bounds__(256) sandwich_ranges_kernel(const __grid_constant__ SumParams p) {
+  const int col = blockIdx.x * blockDim.x + threadIdx.x, q = blockIdx.y;
+  pdl_wait();  // launched as a dependent of the rows' kernel
+  if (col >= p.H || !asked(p, q)) return;
+  const int first = blockIdx.z * p.mods, last = min(first + p.mods, p.n_mod);
+  float sum = 0.f;
+  for (int mod = first; mod < last; ++mod) {
+    const float* at = p.parts + (static_cast<long long>(mod) * p.lanes * 3 + q) * p.H + col;
+    float t = 0.f;
+#pragma unroll 8
+    for (int l = 0; l < p.lanes; ++l) t += at[static_cast<long long>(l) * 3 * p.H];
+    sum += store_row(p, q, mod, col, t);
   }
+  p.parts[(static_cast<long long>(first) * p.lanes * 3 + q) * p.H + col] = sum;
+}
+__global__ void __launch_bounds__(256) sandwich_shared_kernel(const __grid_constant__ SumParams p) {
+  const int col = blockIdx.x * blockDim.x + threadIdx.x, q = blockIdx.y;
+  if (col >= p.H || !asked(p, q)) return;
+  float sum = 0.f;
+  for (int mod = 0; mod < p.n_mod; mod += p.mods) sum += p.parts[(static_cast<long long>(mod) * p.lanes * 3 + q) * p.H + col];
+  store_shared(p, q, col, sum);
 }
 
 // How a call is laid out: a row or more per warp, or R rows at a time per CTA with NV chunks a thread.
@@ -1136,15 +1171,26 @@ extern "C" int vomni_sandwich_norm_bwd(const void* grad_residual_out, const void
   s.dpost_w = dpost_weight;
   s.dmul = dmul;
   s.dadd = dadd;
+  // sandwich_sum_kernel takes its modulation rows one after another, the other kernel a row's parts; the other one's second launch is
+  // 3 us. Whole passes, sum / ranges: 64 x 100 x 1536 (12 parts) 127 / 57 us, 20000 x 1 x 5120 (1) 77 900 / 2200, 4 x 1000 x 5120 (37)
+  // 84 / 72, 8 x 333 x 1536 (92) 39 / 37, 4 x 2000 x 128 (74) 18 / 22, 4 x 333 x 1536 (167) 25 / 33.
+  const bool many = n_mod >= 4 && s.lanes <= 64;
+  s.mods = static_cast<int>((n_mod + 63) / 64);
+  const unsigned ranges = static_cast<unsigned>((n_mod + s.mods - 1) / s.mods);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((h + 31) / 32, 3);
-  cfg.blockDim = dim3(32, 32);
+  cfg.gridDim = many ? dim3((h + 255) / 256, 3, ranges) : dim3((h + 31) / 32, 3);
+  cfg.blockDim = many ? dim3(256) : dim3(32, 32);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  VOMNI_CUDA_TRY(cudaLaunchKernelEx(&cfg, sandwich_sum_kernel, s));
+  VOMNI_CUDA_TRY(cudaLaunchKernelEx(&cfg, many ? sandwich_ranges_kernel : sandwich_sum_kernel, s));
+  const bool shared = dpost_weight || (dgate && !(per_mod & kPerGate)) || (dmul && !(per_mod & kPerMul)) || (dadd && !(per_mod & kPerAdd));
+  if (many && shared) {
+    sandwich_shared_kernel<<<dim3((h + 255) / 256, 3), 256, 0, st>>>(s);
+    VOMNI_CUDA_TRY(cudaGetLastError());
+  }
   return VOMNI_OK;
 }
