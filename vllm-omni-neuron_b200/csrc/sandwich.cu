@@ -970,7 +970,7 @@ Shape shape_of(long long rows_per_mod, long long n_mod, int h, int tensors, bool
   if (s.row_lanes) {
     const int rows = kRowWarps * 32 / s.row_lanes;  // of a CTA at a time; two or four CTAs fit an SM
     const long long need = (rows_per_mod + rows - 1) / rows;
-    const long long cap = (static_cast<long long>(num_sms()) * (backward ? 2 : 4) + n_mod - 1) / n_mod;
+    const long long cap = std::max(1ll, num_sms() * (backward ? 2ll : 4ll) / n_mod);
     s.blocks = static_cast<unsigned>(need < cap ? need : cap);
     s.lanes = static_cast<int>(s.blocks);
     return s;
@@ -987,7 +987,8 @@ Shape shape_of(long long rows_per_mod, long long n_mod, int h, int tensors, bool
   s.slots = static_cast<int>(std::max<size_t>(2, std::min<size_t>(kMaxSlots, room / slot)));
   s.smem = slot * s.slots;
   const long long need = (rows_per_mod + s.rows - 1) / s.rows;
-  const long long cap = (static_cast<long long>(num_sms()) * per_sm + n_mod - 1) / n_mod;
+  // rounded down: one CTA more than fits would run after all the others (3 x 1000 x 5120 backward: 96 us with 150 CTAs)
+  const long long cap = std::max(1ll, static_cast<long long>(num_sms()) * per_sm / n_mod);
   s.blocks = static_cast<unsigned>(need < cap ? need : cap);
   s.lanes = static_cast<int>(s.blocks);
   return s;
