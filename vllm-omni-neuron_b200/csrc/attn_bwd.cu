@@ -84,7 +84,7 @@ struct Params {
 };
 
 // Device status sites (VOMNI_DEV_TIMEOUT_BASE + site).
-enum Site : int { kSiteProducer = 0x10, kSiteMma = 0x11, kSiteScores = 0x12, kSiteOut = 0x13, kSiteDrain = 0x14 };
+enum Site : int { kSiteProducer = 0x10, kSiteMma = 0x11, kSiteScores = 0x12, kSiteOut = 0x13, kSiteDrain = 0x14, kSiteRows = 0x15 };
 
 // mbar_wait whose thread is suspended for 40 ns at a time at most (without the hint it wakes some hundred clocks late), and
 // looks at the abort flag and the clock once in 64 polls.
@@ -199,13 +199,14 @@ VOMNI_DEV void drain(uint64_t* bar, int uses, int* status, int code) {
   mbar_wait(bar, (uses - 1) & 1, &ignored, status, code);
 }
 
-// A float as the sum of three bf16 (8 bits each: 2^-24 relative), in the low halves of three words.
+// A float as the sum of three bf16, exactly: each takes the 8 leading bits that are left, so that none is larger than the
+// float and their sum, in any order, needs no more bits than it has. In the low halves of three words.
 VOMNI_DEV void pieces_of(float v, uint32_t (&w)[3]) {
 #pragma unroll
   for (int i = 0; i < 3; ++i) {
-    const __nv_bfloat16 h = __float2bfloat16_rn(v);
-    w[i] = __bfloat16_as_ushort(h);
-    v -= __bfloat162float(h);
+    const uint32_t h = __float_as_uint(v) & 0xffff0000u;
+    w[i] = h >> 16;
+    v -= __uint_as_float(h);
   }
 }
 VOMNI_DEV uint4 stats_of(float neg_lse_over_scale, float neg_delta) {
@@ -413,8 +414,9 @@ VOMNI_DEV void body(const Maps<N>& maps, const Params& p, uint8_t* smem, int pai
         if (!wait(S_READ + (j & 1), j >> 1, kSiteMma)) break;
         tc_fence_after();
         const uint32_t region = tbase + kColR + (j & 1) * 128;
-        mma_f16_ss_pair(region, ones, desc_aux(smem + kSmemAux + (j % kLSlots) * kAuxBytes), kIdescScores, 0);
-        issue_scores(region, a, desc_k(smem + smem_of(kOr, j)), true);
+        issue_scores(region, a, desc_k(smem + smem_of(kOr, j)));
+        // -delta comes last: dP is then what the rows' kernel summed, and where delta is that sum the two cancel exactly
+        mma_f16_ss_pair(region, ones, desc_aux(smem + kSmemAux + (j % kLSlots) * kAuxBytes), kIdescScores, 1);
         tc_commit_pair(&bars[DP_FULL + (j & 1)]);
       }
     }
@@ -706,75 +708,114 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 }
 
 // ================================================================ rows: lse and delta
+// delta = dO O^T's diagonal, by the tensor cores in the order in which they sum dP's products: where a row of V is the
+// row of O to the bit (a row with one key), dP - delta is exactly 0, as it should be, and so are dQ and dK. Summed by
+// another order what is left of the two was rounding noise, all of the result (1e-7 of dP; 2 times fp32's own).
+template <int N>
+struct RowMaps {
+  CUtensorMap o[N], d_o[N];  // as Maps
+};
 struct RowParams {
-  const __nv_bfloat16* o;
-  const __nv_bfloat16* d_o;
   const float* lse;   // [b, hq, 128, ceil(s_q / 128)]
   const float* dlse;  // the same, or null (0)
-  long long o_s, o_h, o_b, do_s, do_h, do_b;  // strides in elements
-  int b, hq, s_q, rows, groups;
-  int lens;  // q_len per batch element (b <= kMaxSeqs), else q_len[0]
+  int hq, rows, groups;
   int q_len[kMaxSeqs];
   int b0;
   float scale;
   uint4* stats;
+  int* status;
 };
 
-// A half-warp takes kRowsEach adjacent rows, 8 values a lane and row, all loaded before the first is reduced. Rows behind a
-// sequence's end (up to the tile's) get no probability. HBM-bound: 512 bytes a row (26 us for 8190 x 40 rows at the
-// measured copy rate; 48 us with one row at a time).
-constexpr int kRowsEach = 4;
-__global__ void __launch_bounds__(256) attn_bwd_rows_kernel(const __grid_constant__ RowParams p) {
-  pdl_trigger();
-  const long long n = static_cast<long long>(p.b) * p.hq * p.rows;
-  const long long i = ((static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) >> 4) * kRowsEach;
-  if (i >= n) return;  // n is a multiple of 128, so whole warps leave
-  const int sub = threadIdx.x & 15;
-  const int row = static_cast<int>(i % p.rows);  // p.rows is a multiple of 128: the rows belong to one head
-  const int h = static_cast<int>(i / p.rows % p.hq), seq = static_cast<int>(i / p.rows / p.hq), b = p.b0 + seq;
-  const int len = p.lens ? p.q_len[seq] : p.q_len[0];
-  const __nv_bfloat16* o = p.o + b * p.o_b + h * p.o_h + sub * 8;
-  const __nv_bfloat16* d = p.d_o + b * p.do_b + h * p.do_h + sub * 8;
-  uint4 x[kRowsEach], y[kRowsEach];
-#pragma unroll
-  for (int r = 0; r < kRowsEach; ++r) {
-    x[r] = y[r] = make_uint4(0, 0, 0, 0);
-    if (row + r < len) {
-      x[r] = *reinterpret_cast<const uint4*>(o + (row + r) * p.o_s);
-      y[r] = *reinterpret_cast<const uint4*>(d + (row + r) * p.do_s);
+// A CTA takes a tile of 128 rows of one head: dO's and O's, one 128 x 128 product of them, its diagonal, a thread a row.
+// Rows behind a sequence's end (up to the tile's) get no probability. HBM-bound: 512 bytes a row; three CTAs an SM keep
+// 192 KB of loads under way.
+constexpr uint32_t kRowSmemBytes = 2 * kTileBytes + 1024;
+constexpr uint32_t kIdescRows = idesc_bf16(128, 128, false);
+template <int N>
+__global__ void __launch_bounds__(128) attn_bwd_rows_kernel(const __grid_constant__ RowMaps<N> maps, const __grid_constant__ RowParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ __align__(8) uint64_t bars[2];  // operands there, product done
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_word;
+  volatile int* abort_flag = &abort_word;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tile = blockIdx.x % p.groups, h = blockIdx.x / p.groups % p.hq, seq = blockIdx.x / p.groups / p.hq, b = p.b0 + seq;
+  const int mi = N == 1 ? 0 : seq, bz = N == 1 ? seq : 0;
+  const int row0 = tile * kTile, row = row0 + static_cast<int>(threadIdx.x), len = p.q_len[mi];
+  const bool any = row0 < len;
+  if (any) {
+    if (threadIdx.x == 0) {
+      mbar_init(&bars[0], 1);
+      mbar_init(&bars[1], 1);
+      *abort_flag = 0;
+      fence_mbar_init();
     }
+    if (warp == 0) {
+      tmem_alloc(&tmem_slot, kTile);
+      tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
   }
+  pdl_trigger();  // not before this CTA has its TMEM: the dependents take all of an SM's
   const long long bh = static_cast<long long>(b) * p.hq + h;
-  float mine = 0.f;  // lane r of the half keeps row r's sum
+  float l = p.scale > 0.f ? -kNoKeys : kNoKeys, delta = 0.f;
+  if (any) {
+    const long long at = (bh * 128 + threadIdx.x) * p.groups + tile;
+    const float v = row < len ? p.lse[at] : 0.f, dlse = row < len && p.dlse ? p.dlse[at] : 0.f;
+    if (threadIdx.x == 0) {
+      const uint32_t bar = smem_u32(&bars[0]);
+      mbar_expect_tx(&bars[0], 2 * kTileBytes);
 #pragma unroll
-  for (int r = 0; r < kRowsEach; ++r) {
-    const __nv_bfloat162* a = reinterpret_cast<const __nv_bfloat162*>(&x[r]);
-    const __nv_bfloat162* c = reinterpret_cast<const __nv_bfloat162*>(&y[r]);
-    float acc = 0.f;
+      for (int i = 0; i < 4; ++i) {
+        tma_load_4d(&maps.d_o[mi], bar, smem + i * kBox, (i >> 1) * 64, row0 + (i & 1) * 64, h, bz);
+        tma_load_4d(&maps.o[mi], bar, smem + kTileBytes + i * kBox, (i >> 1) * 64, row0 + (i & 1) * 64, h, bz);
+      }
+      if (mbar_wait(&bars[0], 0, abort_flag, p.status, VOMNI_DEV_TIMEOUT_BASE + kSiteRows)) {
+        tc_fence_after();
+        const uint64_t x = desc_k(smem), y = desc_k(smem + kTileBytes);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float2 f = __bfloat1622float2(a[k]), g = __bfloat1622float2(c[k]);
-      acc = fmaf(f.x, g.x, fmaf(f.y, g.y, acc));
+        for (int kk = 0; kk < 8; ++kk) {
+          const uint64_t off = ((kk >> 2) * 2 * kBox + (kk & 3) * 32) >> 4;
+          mma_f16_ss(tmem_slot, x + off, y + off, kIdescRows, kk > 0);
+        }
+        tc_commit(&bars[1]);
+      } else {
+        drain(&bars[0], 1, p.status, VOMNI_DEV_TIMEOUT_BASE + kSiteDrain);
+      }
     }
+    const bool ok = mbar_wait(&bars[1], 0, abort_flag, p.status, VOMNI_DEV_TIMEOUT_BASE + kSiteRows);
+    if (__all_sync(0xffffffffu, ok)) {
+      tc_fence_after();
+      uint32_t s[32];  // columns 32 warp ... of row threadIdx.x
+      tmem_ld32(tmem_slot + (static_cast<uint32_t>(warp * 32) << 16) + warp * 32, s);
+      tmem_ld_wait(s);
 #pragma unroll
-    for (int s = 8; s > 0; s >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, s);
-    if (sub == r) mine = acc;
-  }
-  if (sub < kRowsEach) {
-    const int mr = row + sub;
-    float l = p.scale > 0.f ? -kNoKeys : kNoKeys;
-    if (mr < len) {
-      const long long at = (bh * 128 + (mr & 127)) * p.groups + (mr >> 7);
-      const float v = p.lse[at];
+      for (int i = 0; i < 32; ++i)
+        if (lane == i) delta = __uint_as_float(s[i]);
+    }
+    if (row < len) {
       if (isinf(v)) {
-        mine = 0.f;  // no probabilities, whatever dlse holds
+        delta = 0.f;  // no probabilities, whatever dlse holds
       } else {
         l = -v / p.scale;
-        if (p.dlse) mine -= p.dlse[at];
+        if (p.dlse) delta -= dlse;
       }
       if (fabsf(l) > kNoKeys) l = l > 0.f ? kNoKeys : -kNoKeys;
+    } else {
+      delta = 0.f;
     }
-    p.stats[bh * p.rows + mr] = stats_of(l, -mine);
+  }
+  p.stats[bh * p.rows + row] = stats_of(l, -delta);
+  if (any) {
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) {
+      tc_fence_after();
+      tmem_dealloc(tmem_slot, kTile);
+    }
   }
 }
 
@@ -880,11 +921,11 @@ bool bad_shape(int b, int s_q, int s_kv, int hq, int hkv, int d) {
          static_cast<long long>(b) * hq * ((s_q + 127) / 128 * 128) > 0x7fffffffll;
 }
 
-int make_maps(CUtensorMap* q, CUtensorMap* k, CUtensorMap* v, CUtensorMap* o, const void* const (&base)[4],
-              const long long (&st)[4][3], int batches, int q_len, int kv_len, int hq, int hkv) {
-  CUtensorMap* maps[4] = {q, k, v, o};
-  for (int i = 0; i < 4; ++i) {
-    const bool query = i == 0 || i == 3;
+// The maps of q, k, v, grad_o, o, in this order.
+int make_maps(CUtensorMap* const (&maps)[5], const void* const (&base)[5], const long long (&st)[5][3], int batches, int q_len,
+              int kv_len, int hq, int hkv) {
+  for (int i = 0; i < 5; ++i) {
+    const bool query = i == 0 || i > 2;
     const uint64_t dims[4] = {kD, static_cast<uint64_t>(query ? q_len : kv_len), static_cast<uint64_t>(query ? hq : hkv),
                               static_cast<uint64_t>(batches)};
     int rc = make_tmap_4d_bf16(maps[i], base[i], dims, st[i], 64, 64);
@@ -910,16 +951,22 @@ extern "C" size_t vomni_attention_bwd_workspace_bytes(int b, int s_q, int s_kv, 
   return abwd::plan_of(b, s_q, s_kv, hq, hkv, q_lens, kv_lens).bytes();
 }
 
-// Launches the pairs of batch elements [p.b0, p.b0 + n) with their maps, as a dependent of the stats' launch.
+// Launches the rows' kernel and then the pairs, as its dependent, of batch elements [p.b0, p.b0 + n) with their maps.
 template <int N>
-static int launch_pairs(const abwd::Maps<N>& maps, abwd::Params p, int n, cudaStream_t st) {
+static int launch_parts(const abwd::RowMaps<N>& row_maps, const abwd::RowParams& r, const abwd::Maps<N>& maps, abwd::Params p, int n,
+                        cudaStream_t st) {
   using namespace abwd;
   const long long k_pairs = static_cast<long long>(p.k_tiles2) * p.hkv * n * p.k_splits;
   const long long pairs = k_pairs + static_cast<long long>(p.q_tiles2) * p.hq * n * p.q_splits;
   if (pairs > (1 << 30)) return VOMNI_EBADSHAPE;
   p.k_pairs = static_cast<int>(k_pairs);
+  auto rows = attn_bwd_rows_kernel<N>;
+  int rc = ensure_max_smem(rows, kRowSmemBytes);
+  if (rc) return rc;
+  rows<<<static_cast<unsigned>(n) * r.hq * r.groups, 128, kRowSmemBytes, st>>>(row_maps, r);  // at most 2^24 (bad_shape)
+  VOMNI_CUDA_TRY(cudaGetLastError());
   auto kern = attn_bwd_kernel<N>;
-  int rc = ensure_max_smem(kern, kSmemBytes);
+  rc = ensure_max_smem(kern, kSmemBytes);
   if (rc) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(2 * pairs));
@@ -954,16 +1001,18 @@ extern "C" int vomni_attention_bwd_lse(const void* grad_o, const float* grad_lse
   const Plan plan = plan_of(b, s_q, s_kv, hq, hkv, q_lens, kv_lens);
   if (workspace_bytes < plan.bytes()) return VOMNI_EWORKSPACE;
   // strides: (row, head, batch) of q, k, v, grad_o, o in elements, multiples of 8 where the extent is over 1
-  long long st4[4][3], so[3];
+  long long st5[5][3];
   for (int t = 0; t < 5; ++t) {
     const int ext[3] = {t == 1 || t == 2 ? s_kv : s_q, t == 1 || t == 2 ? hkv : hq, b};
     for (int i = 0; i < 3; ++i) {
       const long long e = strides[t * 3 + i];
       if (ext[i] > 1 && (e <= 0 || e % 8 || e > (1ll << 38))) return VOMNI_EALIGN;
-      (t < 4 ? st4[t][i] : so[i]) = ext[i] > 1 ? e : 0;
+      st5[t][i] = ext[i] > 1 ? e : 0;
     }
   }
   int rc = require_sm100();
+  if (rc) return rc;
+  rc = bind_context(reinterpret_cast<const void*>(abwd::attn_bwd_join_kernel));
   if (rc) return rc;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const bool lens = q_lens || kv_lens;
@@ -1004,51 +1053,44 @@ extern "C" int vomni_attention_bwd_lse(const void* grad_o, const float* grad_lse
     const int n = std::min(chunk, b - b0);
     fill_lens(b0, n);
     RowParams r = {};
-    r.o = static_cast<const __nv_bfloat16*>(o);
-    r.d_o = static_cast<const __nv_bfloat16*>(grad_o);
     r.lse = lse;
     r.dlse = grad_lse;
-    r.o_s = so[0]; r.o_h = so[1]; r.o_b = so[2];
-    r.do_s = st4[3][0]; r.do_h = st4[3][1]; r.do_b = st4[3][2];
-    r.b = n;
     r.hq = hq;
-    r.s_q = s_q;
     r.rows = plan.rows;
-    r.groups = (s_q + 127) / 128;
-    r.lens = lens;
+    r.groups = plan.rows / kTile;
     for (int i = 0; i < kMaxSeqs; ++i) r.q_len[i] = p.q_len[i];
     r.b0 = b0;
     r.scale = softmax_scale;
     r.stats = const_cast<uint4*>(p.stats);
-    const long long blocks = (static_cast<long long>(n) * hq * plan.rows / kRowsEach * 16 + 255) / 256;
-    if (blocks > 0x7fffffffll) return VOMNI_EBADSHAPE;
-    attn_bwd_rows_kernel<<<static_cast<unsigned>(blocks), 256, 0, st>>>(r);
-    VOMNI_CUDA_TRY(cudaGetLastError());
-    // The maps come after a launch: encoding one needs the thread's driver context, which a thread that has made no
-    // runtime call yet (autograd's) gets from its first launch.
+    r.status = p.status;
     CUtensorMap stats_map;
     rc = make_tmap_2d_plain(&stats_map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, ws, 8, static_cast<uint64_t>(b) * hq * plan.rows, 16,
                             8, 64);
     if (rc) return rc;
-    const __nv_bfloat16* all[4] = {static_cast<const __nv_bfloat16*>(q), static_cast<const __nv_bfloat16*>(k),
-                                   static_cast<const __nv_bfloat16*>(v), static_cast<const __nv_bfloat16*>(grad_o)};
+    const __nv_bfloat16* all[5] = {static_cast<const __nv_bfloat16*>(q), static_cast<const __nv_bfloat16*>(k),
+                                   static_cast<const __nv_bfloat16*>(v), static_cast<const __nv_bfloat16*>(grad_o),
+                                   static_cast<const __nv_bfloat16*>(o)};
     if (!lens) {
       Maps<1> maps;
+      RowMaps<1> row_maps;
       maps.stats = stats_map;
-      const void* const base[4] = {all[0], all[1], all[2], all[3]};
-      rc = make_maps(maps.q, maps.k, maps.v, maps.d_o, base, st4, b, s_q, s_kv, hq, hkv);
-      if (!rc) rc = launch_pairs<1>(maps, p, n, st);
+      const void* const base[5] = {all[0], all[1], all[2], all[3], all[4]};
+      rc = make_maps({maps.q, maps.k, maps.v, maps.d_o, row_maps.o}, base, st5, b, s_q, s_kv, hq, hkv);
+      row_maps.d_o[0] = maps.d_o[0];
+      if (!rc) rc = launch_parts<1>(row_maps, r, maps, p, n, st);
     } else {
       Maps<kMaxSeqs> maps;
+      RowMaps<kMaxSeqs> row_maps;
       maps.stats = stats_map;
       for (int i = 0; i < n && !rc; ++i) {
-        const void* const base[4] = {all[0] + (b0 + i) * st4[0][2], all[1] + (b0 + i) * st4[1][2],
-                                     all[2] + (b0 + i) * st4[2][2], all[3] + (b0 + i) * st4[3][2]};
+        const void* base[5];
+        for (int t = 0; t < 5; ++t) base[t] = all[t] + (b0 + i) * st5[t][2];
         // a length of 0 is never loaded from, but a map has no empty extent
-        rc = make_maps(&maps.q[i], &maps.k[i], &maps.v[i], &maps.d_o[i], base, st4, 1, std::max(p.q_len[i], 1),
-                       std::max(p.kv_len[i], 1), hq, hkv);
+        rc = make_maps({&maps.q[i], &maps.k[i], &maps.v[i], &maps.d_o[i], &row_maps.o[i]},
+                       {base[0], base[1], base[2], base[3], base[4]}, st5, 1, std::max(p.q_len[i], 1), std::max(p.kv_len[i], 1), hq, hkv);
+        row_maps.d_o[i] = maps.d_o[i];
       }
-      if (!rc) rc = launch_pairs<kMaxSeqs>(maps, p, n, st);
+      if (!rc) rc = launch_parts<kMaxSeqs>(row_maps, r, maps, p, n, st);
     }
     if (rc) return rc;
   }

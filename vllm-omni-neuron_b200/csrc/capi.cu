@@ -65,6 +65,16 @@ int require_sm100() {
   return ok ? VOMNI_OK : VOMNI_ENOTSUP;
 }
 
+int bind_context(const void* kernel) {
+  static thread_local int bound = -1;
+  const int dev = current_device();
+  if (dev >= 0 && dev == bound) return VOMNI_OK;
+  cudaFuncAttributes a;
+  VOMNI_CUDA_TRY(cudaFuncGetAttributes(&a, kernel));
+  bound = dev;
+  return VOMNI_OK;
+}
+
 int* device_status_ptr() {
   const int dev = current_device();
   if (dev < 0 || dev >= kMaxDevices) return nullptr;

@@ -156,6 +156,13 @@ VOMNI_DEV void tma_load_2d(const CUtensorMap* m, uint64_t* bar, void* dst, int x
       "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(x), "r"(y)
       : "memory");
 }
+VOMNI_DEV void tma_load_4d(const CUtensorMap* m, uint32_t bar, void* dst, int x, int y, int z, int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], "
+      "[%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
 
 // ---------------------------------------------------------------- tcgen05 / TMEM
 VOMNI_DEV void tmem_alloc(uint32_t* dst_smem, uint32_t ncols) {

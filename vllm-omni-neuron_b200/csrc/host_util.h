@@ -28,6 +28,9 @@ void set_last_cuda_error(cudaError_t e);
 int num_sms();
 // VOMNI_OK on an sm_100 device, VOMNI_ENOTSUP otherwise.
 int require_sm100();
+// Makes the current device's context this thread's, as encoding a tensor map needs (a thread that has made no runtime call
+// yet, as autograd's, has none). `kernel`: any of the library's. May be called while a stream is captured.
+int bind_context(const void* kernel);
 // Device address of the library status word on the current device (nullptr if unavailable).
 int* device_status_ptr();
 
