@@ -142,6 +142,16 @@ VOMNI_API int vomni_cm_attention_local(const void* q, const void* k, const void*
                              int d, float softmax_scale, int flags, void* workspace, size_t workspace_bytes,
                              vomni_stream_t stream);
 
+/* ------------------------------------------------------------------ attention forward for training
+ * softmax(softmax_scale q k^T) v and its log-sum-exp, of any q, k, v whose products fp32 holds: vomni_cm_attention_cross with VOMNI_CM_LSE, then the rows
+ * that its bound does not fit (their probabilities under it are not representable) once more under their own
+ * maximum; every other row is what vomni_cm_attention_cross gives, to the bit. Arguments as there; out [b, h, s_q, 128],
+ * lse fp32 [b, h, 128, ceil(s_q/128)] (entries behind s_q are left as they are). softmax_scale in [1e-20, 1e20]. A row whose
+ * scores are all -inf: 0, lse -inf. workspace: vomni_cm_workspace_bytes(b, s_q, h, d). */
+VOMNI_API int vomni_attention_fwd(const void* q, const void* k, const void* v, void* out, float* lse, int b, int s_q, int s_kv, int h,
+                                  int d, long long q_stride, long long kv_stride, float softmax_scale, void* workspace,
+                                  size_t workspace_bytes, vomni_stream_t stream);
+
 /* ------------------------------------------------------------------ attention backward
  * Gradients of softmax(softmax_scale q k^T) v from the forward's output o and log-sum-exp lse (VOMNI_CM_LSE: the
  * training outputs of ring_attention_const_max_fwd.py:1062-1065); the probabilities are recomputed. q, grad_o, o:

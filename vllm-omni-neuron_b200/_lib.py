@@ -85,6 +85,10 @@ SIGNATURES = {
         c_int,
         [P, P, P, P, P, P, c_int, c_int, c_int, c_int, ctypes.c_longlong, ctypes.c_longlong, c_float, c_int, P],
     ),
+    "vomni_attention_fwd": (
+        c_int,
+        [P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_longlong, c_longlong, c_float, P, c_size_t, P],
+    ),
     "vomni_attention_bwd_workspace_bytes": (c_size_t, [c_int] * 6 + [ctypes.POINTER(c_int)] * 2),
     "vomni_attention_bwd": (
         c_int,

@@ -324,9 +324,9 @@ def _cross_fwd(q, k, v, scale):
     lse = torch.full((b, h, 128, -(-sq // 128)), -math.inf, dtype=torch.float32, device=q.device)
     ws_bytes = lib.vomni_cm_workspace_bytes(b, sq, h, d)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
-    rc = lib.vomni_cm_attention_cross(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), b, sq, skv, h, d,
-                                      qs, ks, scale, _lib.CM_LSE, ws.data_ptr(), ws_bytes, _stream_ptr(q.device))
-    _lib.check(rc, "vomni_cm_attention_cross")
+    rc = lib.vomni_attention_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), b, sq, skv, h, d, qs, ks, scale,
+                                 ws.data_ptr(), ws_bytes, _stream_ptr(q.device))
+    _lib.check(rc, "vomni_attention_fwd")
     return o, lse
 
 
@@ -338,8 +338,8 @@ def attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, softmax_sca
     ``h // (hq // hkv)``). ``lse[.., r, g]`` belongs to token ``128 g + r``, as in :func:`ring_attention_const_max_fwd`.
     ``q_lens`` / ``kv_lens``: tokens of each batch element (host ints); rows behind them are not read, and their output
     is 0 with an lse of -inf, as is that of rows without keys. ``softmax_scale`` (positive) defaults to ``1 / sqrt(128)``.
-    Like every forward here it sums under the bound ``softmax_scale * |q_i| * max_j |k_j|``: a row whose largest score lies
-    more than about 87 below that bound has no representable probabilities.
+    Rows sum under the bound ``softmax_scale * |q_i| * max_j |k_j|`` as in :func:`ring_attention_const_max_fwd`; those whose
+    probabilities under it are not representable are computed again under their own maximum.
     """
     b, sq, skv, hq, hkv, q_lens, kv_lens = _check_training(q, k, v, q_lens, kv_lens)
     scale = _training_scale(softmax_scale)
@@ -388,8 +388,10 @@ def attention_bwd(grad_o: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: tor
     used too, as when parts are merged by it; the other arguments as in :func:`attention_fwd`. The
     probabilities are recomputed as ``exp(softmax_scale q k^T - lse)``, so with the ``lse`` and ``o`` of a whole sequence
     and a part of its keys the result is that part's share of the gradients (for a context-parallel ring: the parts'
-    ``dq`` add up). Rows behind ``q_lens`` / ``kv_lens`` are not read and get zero gradients; a row whose lse is -inf
-    has probabilities 0 and no ``grad_lse``. The same call gives the same bits (no atomics).
+    ``dq`` add up). ``lse`` has to be that of a softmax: :func:`attention_fwd`'s is, ``ring_attention_const_max_fwd``'s where
+    no row's largest score lies more than about 50 below its bound ``softmax_scale * |q_i| * max_j |k_j|``. Rows behind
+    ``q_lens`` / ``kv_lens`` are not read and get zero gradients; a row whose lse is -inf has probabilities 0 and no
+    ``grad_lse``. The same call gives the same bits (no atomics).
     """
     b, sq, skv, hq, hkv, q_lens, kv_lens = _check_training(q, k, v, q_lens, kv_lens)
     for name, t in (("grad_o", grad_o), ("o", o)):
