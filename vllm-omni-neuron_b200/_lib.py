@@ -12,6 +12,7 @@ import threading
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 HERE = Path(__file__).resolve().parent
 LIB_PATH = HERE / "libvomni_b200.so"
@@ -181,6 +182,14 @@ def one_device(*tensors) -> int:
                     raise ValueError(f"tensors are on different devices: cuda:{index} and cuda:{i}")
                 index = i
     return index
+
+
+def for_autograd(*tensors) -> bool:
+    """Whether a call on these tensors (None entries aside) goes through its autograd function: one of them requires a gradient, or a
+    forward-mode level is open, where one may carry a tangent (which the autograd functions refuse)."""
+    if forward_ad._current_level >= 0:
+        return True
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def on_device(index: int, fn, *args):

@@ -21,8 +21,8 @@ the result of group i returns to pinned host memory while group i+1 computes. He
 independent, so the result is identical to the device-resident call; the output is a pinned CPU
 tensor, complete on return.
 
-Training: :func:`wan_attention` is the differentiable form, made of :func:`attention_fwd` (output and log-sum-exp; keys of
-another sequence, shared key heads and uneven batches included) and :func:`attention_bwd` (the gradients).
+Training: :func:`attention_fwd` (output and log-sum-exp; keys of another sequence, shared key heads and uneven batches
+included) is differentiable through :func:`attention_bwd` (the gradients); :func:`wan_attention` is its output alone.
 """
 
 from __future__ import annotations
@@ -330,19 +330,10 @@ def _cross_fwd(q, k, v, scale):
     return o, lse
 
 
-def attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, softmax_scale: float | None = None, *, q_lens=None,
-                  kv_lens=None):
-    """``(o [b, hq, s_q, 128] bf16, lse [b, hq, 128, ceil(s_q / 128)] fp32)`` of ``softmax(softmax_scale q k^T) v``.
-
-    ``q [b, s_q, hq, 128]``, ``k, v [b, s_kv, hkv, 128]`` token-major bf16, ``hq % hkv == 0`` (query head ``h`` reads key head
-    ``h // (hq // hkv)``). ``lse[.., r, g]`` belongs to token ``128 g + r``, as in :func:`ring_attention_const_max_fwd`.
-    ``q_lens`` / ``kv_lens``: tokens of each batch element (host ints); rows behind them are not read, and their output
-    is 0 with an lse of -inf, as is that of rows without keys. ``softmax_scale`` (positive) defaults to ``1 / sqrt(128)``.
-    Rows sum under the bound ``softmax_scale * |q_i| * max_j |k_j|`` as in :func:`ring_attention_const_max_fwd`; those whose
-    probabilities under it are not representable are computed again under their own maximum.
-    """
-    b, sq, skv, hq, hkv, q_lens, kv_lens = _check_training(q, k, v, q_lens, kv_lens)
-    scale = _training_scale(softmax_scale)
+def _attention(q, k, v, scale, q_lens, kv_lens):
+    """:func:`attention_fwd` of checked arguments."""
+    b, sq, hq, _ = q.shape
+    skv, hkv = k.shape[1:3]
     dev = _lib.one_device(q, k, v)
     device = q.device
     q, k, v = (t if t.data_ptr() % 16 == 0 else t.clone() for t in (q, k, v))
@@ -360,6 +351,45 @@ def attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, softmax_sca
                 o[i, :, :m] = oi[0]
                 lse[i, :, :, : li.shape[-1]] = li[0]
         return o, lse
+
+
+class _AttentionFwd(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, scale, q_lens, kv_lens):
+        ctx.set_materialize_grads(False)
+        o, lse = _attention(q, k, v, scale, q_lens, kv_lens)
+        ctx.save_for_backward(q, k, v, o, lse)
+        ctx.rest = (scale, q_lens, kv_lens)
+        return o, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_o, grad_lse):
+        if grad_o is None and grad_lse is None:
+            return (None,) * 6
+        scale, q_lens, kv_lens = ctx.rest
+        q, k, v, o, lse = ctx.saved_tensors
+        if grad_o is None:
+            grad_o = torch.zeros_like(o)
+        grads = attention_bwd(grad_o, q, k, v, o, lse, scale, q_lens=q_lens, kv_lens=kv_lens, grad_lse=grad_lse)
+        return tuple(g if need else None for g, need in zip(grads, ctx.needs_input_grad)) + (None, None, None)
+
+
+def attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, softmax_scale: float | None = None, *, q_lens=None,
+                  kv_lens=None):
+    """``(o [b, hq, s_q, 128] bf16, lse [b, hq, 128, ceil(s_q / 128)] fp32)`` of ``softmax(softmax_scale q k^T) v``.
+
+    ``q [b, s_q, hq, 128]``, ``k, v [b, s_kv, hkv, 128]`` token-major bf16, ``hq % hkv == 0`` (query head ``h`` reads key head
+    ``h // (hq // hkv)``). ``lse[.., r, g]`` belongs to token ``128 g + r``, as in :func:`ring_attention_const_max_fwd`.
+    ``q_lens`` / ``kv_lens``: tokens of each batch element (host ints); rows behind them are not read, and their output
+    is 0 with an lse of -inf, as is that of rows without keys. ``softmax_scale`` (positive) defaults to ``1 / sqrt(128)``.
+    Rows sum under the bound ``softmax_scale * |q_i| * max_j |k_j|`` as in :func:`ring_attention_const_max_fwd`; those whose
+    probabilities under it are not representable are computed again under their own maximum.
+    Differentiable through both results, by :func:`attention_bwd`.
+    """
+    *_, q_lens, kv_lens = _check_training(q, k, v, q_lens, kv_lens)
+    args = (q, k, v, _training_scale(softmax_scale), q_lens, kv_lens)
+    return _AttentionFwd.apply(*args) if _lib.for_autograd(q, k, v) else _attention(*args)
 
 
 _Strides = ctypes.c_longlong * 15  # (token, head, batch) of q, k, v, grad_o, o
@@ -430,25 +460,8 @@ def attention_bwd(grad_o: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: tor
     return dq, dk, dv
 
 
-class _WanAttention(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, scale, q_lens, kv_lens):
-        o, lse = attention_fwd(q, k, v, scale, q_lens=q_lens, kv_lens=kv_lens)
-        ctx.save_for_backward(q, k, v, o, lse)
-        ctx.rest = (scale, q_lens, kv_lens)
-        return o
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad_o):
-        scale, q_lens, kv_lens = ctx.rest
-        grads = attention_bwd(grad_o, *ctx.saved_tensors, scale, q_lens=q_lens, kv_lens=kv_lens)
-        return tuple(g if need else None for g, need in zip(grads, ctx.needs_input_grad)) + (None, None, None)
-
-
 def wan_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, softmax_scale: float | None = None, *, q_lens=None,
                   kv_lens=None) -> torch.Tensor:
     """Differentiable attention ``[b, hq, s_q, 128]`` of one device's ``q [b, s_q, hq, 128]``, ``k, v [b, s_kv, hkv, 128]``;
     the arguments are those of :func:`attention_fwd`, the gradients those of :func:`attention_bwd`."""
-    q_lens, kv_lens = (n if n is None or isinstance(n, torch.Tensor) else tuple(int(i) for i in n) for n in (q_lens, kv_lens))
-    return _WanAttention.apply(q, k, v, softmax_scale, q_lens, kv_lens)
+    return attention_fwd(q, k, v, softmax_scale, q_lens=q_lens, kv_lens=kv_lens)[0]
