@@ -192,6 +192,12 @@ def for_autograd(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
+def refuse_tangents(what: str, *tensors) -> None:
+    """Raise where a tensor carries a forward-mode tangent, which a call outside autograd would lose."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{what} has no forward-mode derivative")
+
+
 def on_device(index: int, fn, *args):
     """``fn(*args)`` with device ``index`` current."""
     if torch.cuda.current_device() == index:

@@ -421,8 +421,9 @@ def attention_bwd(grad_o: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: tor
     ``dq`` add up). ``lse`` has to be that of a softmax: :func:`attention_fwd`'s is, ``ring_attention_const_max_fwd``'s where
     no row's largest score lies more than about 50 below its bound ``softmax_scale * |q_i| * max_j |k_j|``. Rows behind
     ``q_lens`` / ``kv_lens`` are not read and get zero gradients; a row whose lse is -inf has probabilities 0 and no
-    ``grad_lse``. The same call gives the same bits (no atomics).
+    ``grad_lse``. The same call gives the same bits (no atomics). Not differentiable themselves.
     """
+    _lib.refuse_tangents("attention_bwd", grad_o, q, k, v, o, lse, grad_lse)
     b, sq, skv, hq, hkv, q_lens, kv_lens = _check_training(q, k, v, q_lens, kv_lens)
     for name, t in (("grad_o", grad_o), ("o", o)):
         if t.dtype is not torch.bfloat16:

@@ -25,7 +25,8 @@ output shapes and dtypes, so a traced or compiled caller sees one opaque node pe
 ``b200omni::sandwich_norm_bwd``        its gradients
 =====================================  =====================================================
 
-Importing this module registers the operators once; the package imports it.
+Importing this module registers the operators once; the package imports it. The differentiable ones are so in reverse mode; they
+refuse forward-mode tangents, except that ``torch.func.jvp`` hides its tangents from any custom operator.
 """
 
 from __future__ import annotations

@@ -211,7 +211,7 @@ def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor
         raise ValueError(f"theta must be positive and finite, got {theta}")
     _lib.one_device(q, k, positions)
     args = (q, k, positions, axes_dims, float(theta), _PAIRINGS[pairing], bool(inverse))
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+    if _lib.for_autograd(q, k):
         out = _RotaryAxes.apply(*args)
     else:
         out = _rotary(*args)

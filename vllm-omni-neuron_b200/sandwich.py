@@ -192,7 +192,7 @@ def sandwich_norm(
     Arithmetic is fp32; ``out`` comes from the unrounded residual, and each result is rounded to bf16 once. The backward pass
     reads ``x`` and ``residual_out`` and recomputes the statistics; it gives the same bits every time.
     """
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, gate, mul, add, post_weight)):
+    if _lib.for_autograd(x, residual, gate, mul, add, post_weight):
         res = _SandwichNorm.apply(x, residual, gate, mul, add, post_weight, float(eps), post_norm, norm_type)
         return (residual, res) if x is None else res
     res_out, out = _forward(x, residual, gate, mul, add, post_weight, float(eps), post_norm, norm_type)
@@ -214,7 +214,8 @@ def sandwich_norm_bwd(
     norm_type: str = "layer_norm",
 ) -> SandwichGrads:
     """Gradients of :func:`sandwich_norm` from those of its two results (one of them may be None: zero), its arguments and
-    the ``residual_out`` it returned (``residual`` itself where ``x`` is None)."""
+    the ``residual_out`` it returned (``residual`` itself where ``x`` is None). Not differentiable themselves."""
+    _lib.refuse_tangents("sandwich_norm_bwd", grad_residual_out, grad_out, x, residual_out, gate, mul, add, post_weight)
     if grad_residual_out is None and grad_out is None:
         raise ValueError("at least one of grad_residual_out and grad_out is needed")
     return _backward(grad_residual_out, grad_out, x, residual_out, gate, mul, add, post_weight, float(eps), post_norm, norm_type,
