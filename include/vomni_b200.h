@@ -172,6 +172,14 @@ VOMNI_API int vomni_attention_bwd(const void* grad_o, const void* q, const void*
                                   void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes,
                                   vomni_stream_t stream);
 
+/* vomni_attention_bwd where lse was used too: grad_lse (or NULL: 0) is its gradient, in its layout; that of a row whose lse is -inf is
+ * ignored. */
+VOMNI_API int vomni_attention_bwd_lse(const void* grad_o, const float* grad_lse, const void* q, const void* k, const void* v,
+                                      const void* o, const float* lse, int b, int s_q, int s_kv, int hq, int hkv, int d,
+                                      const long long* strides, const int* q_lens, const int* kv_lens, float softmax_scale,
+                                      void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes,
+                                      vomni_stream_t stream);
+
 /* ------------------------------------------------------------------ fused adaLN + FP8 quant
  * Replaces adaln_quant_kernel (kernels/nkilib/experimental/norm/adaln_quant.py:117-810) as called
  * by the bridge adaln_modulate (diffusion/quantization/adaln_kernels.py:87-201):
@@ -187,14 +195,6 @@ VOMNI_API int vomni_adaln_modulate(const void* hidden, const void* residual, con
                                    const float* gate, long long rows, int h, long long rows_per_mod, float eps,
                                    int norm_type, int quant, int ocp, int packed, void* out, void* out_scale,
                                    void* residual_out, vomni_stream_t stream);
-
-/* The same where lse was used too: grad_lse (or NULL: 0) is its gradient, in its layout; that of a row whose lse is -inf is
- * ignored. */
-VOMNI_API int vomni_attention_bwd_lse(const void* grad_o, const float* grad_lse, const void* q, const void* k, const void* v,
-                                      const void* o, const float* lse, int b, int s_q, int s_kv, int hq, int hkv, int d,
-                                      const long long* strides, const int* q_lens, const int* kv_lens, float softmax_scale,
-                                      void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes,
-                                      vomni_stream_t stream);
 
 /* ------------------------------------------------------------------ norms around a block
  * The gated residual of adaln_modulate with a norm before it as well as after, and its gradients:

@@ -455,9 +455,12 @@ def attention_bwd(grad_o: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: tor
         q_lens, kv_lens = (n if n is None else (ctypes.c_int * b)(*n) for n in (q_lens, kv_lens))
         ws_bytes = _lib.on_device(dev, _lib.load().vomni_attention_bwd_workspace_bytes, b, sq, skv, hq, hkv, _HEAD_DIM, q_lens, kv_lens)
     ws = _lib.workspace(ws_bytes, q.device)
-    _lib.launch(dev, "vomni_attention_bwd_lse", grad_o.data_ptr(), None if grad_lse is None else grad_lse.data_ptr(), q.data_ptr(),
-                k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), b, sq, skv, hq, hkv, _HEAD_DIM, strides, q_lens, kv_lens,
-                scale, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), ws_bytes)
+    args = (q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), b, sq, skv, hq, hkv, _HEAD_DIM, strides, q_lens, kv_lens,
+            scale, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), ws_bytes)
+    if grad_lse is None:
+        _lib.launch(dev, "vomni_attention_bwd", grad_o.data_ptr(), *args)
+    else:
+        _lib.launch(dev, "vomni_attention_bwd_lse", grad_o.data_ptr(), grad_lse.data_ptr(), *args)
     return dq, dk, dv
 
 
