@@ -203,7 +203,7 @@ VOMNI_API int vomni_adaln_modulate(const void* hidden, const void* residual, con
  * x, residual, residual_out, out: bf16 [rows, h], h <= 8192, h % 8 == 0; vectors fp32, each optional: post_weight
  * [h]; gate, mul, add [rows / rows_per_mod, h] where their VOMNI_PER_* bit is set in per_mod, else [h] (shared).
  * post_norm / norm_type: 0 layer / 1 rms / 2 none, variance + eps (eps > 0). rows % rows_per_mod == 0. x NULL: r = residual
- * (then gate, post_weight and residual_out must be NULL). residual_out may alias x or residual, and out may alias either.
+ * (then gate, post_weight and residual_out must be NULL: VOMNI_EINVAL). residual_out may alias x or residual, and out may alias either.
  *
  * _bwd: from the gradients of residual_out and out (either may be NULL: zero), x and the stored residual_out it
  * writes dx (x NULL: NULL), dresidual (bf16) and, where the pointer is not NULL, the fp32 column sums dgate,

@@ -1106,7 +1106,7 @@ extern "C" int vomni_sandwich_norm(const void* x, const void* residual, const fl
                                    vomni_stream_t stream) {
   using namespace sandwich;
   if (!residual || !out || (x && !residual_out) || (per_mod & ~7)) return VOMNI_EINVAL;
-  if (!x && (gate || post_weight)) return VOMNI_EINVAL;
+  if (!x && (gate || post_weight || residual_out)) return VOMNI_EINVAL;
   int rc = check(rows, h, rows_per_mod, post_norm, norm_type, eps);
   if (rc) return rc;
   if (misaligned(x, residual, residual_out, out) || misaligned(gate, post_weight, mul, add)) return VOMNI_EALIGN;
