@@ -44,7 +44,7 @@ struct Params {
   const float* post_w;            // [H] or null (1)
   const float* mul;               // [n_mod or 1, H] or null (1)
   const float* add;               // [n_mod or 1, H] or null (0)
-  long long rows, rows_per_mod;
+  long long rows_per_mod;
   long long gate_step, mul_step, add_step;  // H where per modulation row, else 0
   int H, post, norm;
   float eps, inv_h;
@@ -1076,14 +1076,13 @@ bool misaligned(const void* a, const void* b = nullptr, const void* c = nullptr,
           reinterpret_cast<uintptr_t>(d)) & 15;
 }
 void fill(Params& p, const void* x, const void* residual, const float* gate, const float* post_w, const float* mul,
-          const float* add, long long rows, int h, long long rows_per_mod, int per, float eps, int post, int norm) {
+          const float* add, int h, long long rows_per_mod, int per, float eps, int post, int norm) {
   p.x = static_cast<const __nv_bfloat16*>(x);
   p.residual = static_cast<const __nv_bfloat16*>(residual);
   p.gate = gate;
   p.post_w = post_w;
   p.mul = mul;
   p.add = add;
-  p.rows = rows;
   p.rows_per_mod = rows_per_mod;
   p.gate_step = per & kPerGate ? h : 0;
   p.mul_step = per & kPerMul ? h : 0;
@@ -1113,7 +1112,7 @@ extern "C" int vomni_sandwich_norm(const void* x, const void* residual, const fl
   rc = require_sm100();
   if (rc) return rc;
   Params p = {};
-  fill(p, x, residual, gate, post_weight, mul, add, rows, h, rows_per_mod, per_mod, eps, post_norm, norm_type);
+  fill(p, x, residual, gate, post_weight, mul, add, h, rows_per_mod, per_mod, eps, post_norm, norm_type);
   p.out0 = static_cast<__nv_bfloat16*>(residual_out);
   p.out1 = static_cast<__nv_bfloat16*>(out);
   const long long n_mod = rows / rows_per_mod;
@@ -1148,7 +1147,7 @@ extern "C" int vomni_sandwich_norm_bwd(const void* grad_residual_out, const void
   rc = require_sm100();
   if (rc) return rc;
   Params p = {};
-  fill(p, x, residual_out, gate, post_weight, mul, nullptr, rows, h, rows_per_mod, per_mod, eps, post_norm, norm_type);
+  fill(p, x, residual_out, gate, post_weight, mul, nullptr, h, rows_per_mod, per_mod, eps, post_norm, norm_type);
   p.d_res = static_cast<const __nv_bfloat16*>(grad_residual_out);
   p.d_out = static_cast<const __nv_bfloat16*>(grad_out);
   p.out0 = static_cast<__nv_bfloat16*>(dx);
