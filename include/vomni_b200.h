@@ -160,8 +160,8 @@ VOMNI_API int vomni_attention_fwd(const void* q, const void* k, const void* v, v
  * d = 128). lse: fp32 [b, hq, 128, ceil(s_q/128)] dense. hq % hkv == 0: query head h reads key head h / (hq / hkv), whose
  * gradients are summed over its query heads. dq, dk, dv: bf16, dense, token-major. q_lens / kv_lens (host arrays of b
  * counts, or NULL): the tokens of each batch element; those behind are neither read nor counted, whatever they hold,
- * and their gradients are 0. A row whose lse is -inf has no probabilities. Given the lse of a whole sequence
- * and a part of its keys, the result is that part's share (the parts' dq add up). Bitwise reproducible (no
+ * and their gradients are 0. A row whose lse is -inf has no probabilities (its grad_o has to be finite all the same). Given the
+ * lse of a whole sequence and a part of its keys, the result is that part's share (the parts' dq add up). Bitwise reproducible (no
  * atomics). |softmax_scale| in [1e-20, 1e20]. workspace: vomni_attention_bwd_workspace_bytes for the same lengths
  * (depends on the current device's size; 0 = unsupported shape), not shared by calls that may overlap. */
 VOMNI_API size_t vomni_attention_bwd_workspace_bytes(int b, int s_q, int s_kv, int hq, int hkv, int d, const int* q_lens,

@@ -385,7 +385,7 @@ def attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, softmax_sca
     is 0 with an lse of -inf, as is that of rows without keys. ``softmax_scale`` (positive) defaults to ``1 / sqrt(128)``.
     Rows sum under the bound ``softmax_scale * |q_i| * max_j |k_j|`` as in :func:`ring_attention_const_max_fwd`; those whose
     probabilities under it are not representable are computed again under their own maximum.
-    Differentiable through both results, by :func:`attention_bwd`.
+    Differentiable through both results, by :func:`attention_bwd`. ``b * hq`` is at most 8192, per element where lengths are given.
     """
     *_, q_lens, kv_lens = _check_training(q, k, v, q_lens, kv_lens)
     args = (q, k, v, _training_scale(softmax_scale), q_lens, kv_lens)
@@ -421,7 +421,7 @@ def attention_bwd(grad_o: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: tor
     ``dq`` add up). ``lse`` has to be that of a softmax: :func:`attention_fwd`'s is, ``ring_attention_const_max_fwd``'s where
     no row's largest score lies more than about 50 below its bound ``softmax_scale * |q_i| * max_j |k_j|``. Rows behind
     ``q_lens`` / ``kv_lens`` are not read and get zero gradients; a row whose lse is -inf has probabilities 0 and no
-    ``grad_lse``. The same call gives the same bits (no atomics). Not differentiable themselves.
+    ``grad_lse`` (its ``grad_o`` has to be finite all the same). The same call gives the same bits (no atomics). Not differentiable themselves.
     """
     _lib.refuse_tangents("attention_bwd", grad_o, q, k, v, o, lse, grad_lse)
     b, sq, skv, hq, hkv, q_lens, kv_lens = _check_training(q, k, v, q_lens, kv_lens)

@@ -25,8 +25,9 @@
 // two issuers' products in turn, so X lets Y's batch go ahead where the score warps need it first.
 // Matrix products per 128 x 128 scores of a CTA: 512 clocks each; exponentials: 1024 clocks of the MUFU unit.
 // Measured, clocks a step of a pair at 32760 tokens: dkdv 2450 (its products alone 2180), dq 2250 (1540), at which the GPU is at
-// its power cap (1.59 to 1.75 GHz). 4096 tokens x 40 heads 0.95 to 1.08 ms (796 to 904 TFLOP/s of the 5 products, 1.1 to 1.3 PFLOP/s
-// of the 7), 32760 x 8 heads 11.3 to 11.9 ms (924 to 972), 8190 x 512 x 40 heads 0.36 to 0.38 ms.
+// its power cap (1.59 to 1.75 GHz). Over several GPUs, among other passes and alone: 4096 tokens x 40 heads 0.94 to 1.09 ms (788 to 914
+// TFLOP/s of the 5 products, 1.1 to 1.3 PFLOP/s of the 7), 32760 x 8 heads 11.3 to 11.9 ms (924 to 972), 8190 x 512 x 40 heads 0.36 to
+// 0.39 ms, 0.41 to 0.46 with a cold L2.
 //
 // Rounding: P and dS are rounded to bf16 as tensor-core operands (2^-8 relative each, at most); everything else is fp32 until the
 // gradients are rounded once.
@@ -50,7 +51,9 @@ constexpr int kGroups = 4;              // score warpgroups: each owns kCols col
 constexpr int kCols = kTile / kGroups;  // 32: one TMEM load
 constexpr int kControl = 4;             // warps ahead of them: TMA producer, two MMA issuers, one idle
 constexpr int kThreads = 32 * kControl + 128 * kGroups;
-constexpr int kMaxSeqs = 16;            // batch elements of a launch with lengths of their own
+// Batch elements of a launch with lengths of their own: more run as launches one after another, each with its own tail (the split rule
+// looks at the batch as one launch).
+constexpr int kMaxSeqs = 16;
 constexpr uint32_t kBox = 64 * 64 * 2;  // 8 KB: one TMA box, 64 rows x 64 dims, 128-byte swizzled
 constexpr uint32_t kTileBytes = 4 * kBox;  // resident operand: [2 dim halves][2 row halves] boxes
 constexpr uint32_t kHalfTile = 2 * kBox;   // a CTA's half of a streamed operand
@@ -728,7 +731,8 @@ struct RowParams {
 
 // A CTA takes a tile of 128 rows of one head: dO's and O's, one 128 x 128 product of them, its diagonal, a thread a row.
 // Rows behind a sequence's end (up to the tile's) get no probability. HBM-bound: 512 bytes a row; three CTAs an SM keep
-// 192 KB of loads under way.
+// 192 KB of loads under way. 8190 x 40 rows 34 us, 4.9 TB/s (38 with plain loads and fused multiply-adds, four rows a half-warp);
+// a single tile takes 2 us more than by those.
 constexpr uint32_t kRowSmemBytes = 2 * kTileBytes + 1024;
 constexpr uint32_t kIdescRows = idesc_bf16(128, 128, false);
 template <int N>

@@ -18,7 +18,8 @@
 // time through a ring in shared memory; a thread owns chunks of 8 adjacent columns of all of them. The kernels are persistent, so
 // that in the backward pass a thread's column sums stay in its registers over all rows of its CTA; the CTAs' sums
 // go to a workspace and are added in a fixed order by a second kernel (no atomics: the same call gives the same bits).
-// Measured, 32760 x 5120: forward 225 us (0.91 of the measured copy rate), backward 356 us (0.86).
+// Measured over several GPUs, 32760 x 5120: forward 224 to 236 us (0.87 to 0.91 of the measured copy rate), backward 354 to 382 us (0.80
+// to 0.87).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -982,12 +983,17 @@ Shape shape_of(long long rows_per_mod, long long n_mod, int h, int tensors, bool
   s.threads = ((chunks + s.nv - 1) / s.nv + 31) / 32 * 32;
   s.rows = chunks > 640 || !many ? 1 : backward ? 2 : 4;
   const size_t slot = static_cast<size_t>(s.rows) * h * 2 * tensors;
+  // What the registers hold: 640 threads an SM forward, 320 backward. The quotient is rounded down, so just over half of them one CTA
+  // is left with an SM to itself (backward, 16384 rows: 3000 columns 1.7 times the bytes' time, 5120 1.2 times); rows over 5120 columns go one
+  // at a time (8192 columns 1.6 times).
   const int per_sm = std::max(1, std::min((backward && many ? 320 : 640) / s.threads, 8));
   const size_t room = (kSmemPerSm / per_sm);
   s.slots = static_cast<int>(std::max<size_t>(2, std::min<size_t>(kMaxSlots, room / slot)));
   s.smem = slot * s.slots;
   const long long need = (rows_per_mod + s.rows - 1) / s.rows;
-  // rounded down: one CTA more than fits would run after all the others (3 x 1000 x 5120 backward: 96 us with 150 CTAs)
+  // Rounded down: one CTA more than fits would run after all the others (3 x 1000 x 5120 backward: 96 us with 150 CTAs, 70 with 147).
+  // Between half of what fits and all of it each modulation row gets one CTA and the rest idles, and past all of it the last ones do run
+  // after the others: backward, 200 tokens of 5120 columns each, 74 rows 163 us, 75 to 148 rows 305, 149 to 296 rows 600.
   const long long cap = std::max(1ll, static_cast<long long>(num_sms()) * per_sm / n_mod);
   s.blocks = static_cast<unsigned>(need < cap ? need : cap);
   s.lanes = static_cast<int>(s.blocks);

@@ -177,8 +177,9 @@ def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor
 
     * ``q [b, s, hq, d]``, ``k [b, s, hk, d]`` (or None) token-major, bf16 / fp16 / fp32, ``d % 16 == 0``, ``d <= 256``; the
       column slices of a fused projection are read in place, other strides are copied first.
-    * ``positions`` ``[s, n_axes]`` or ``[b, s, n_axes]``, int32 / int64 / fp32 (fractions for interpolated positions),
-      any magnitude: angles are reduced in 64 bits. Not differentiated.
+    * ``positions`` ``[s, n_axes]`` or ``[b, s, n_axes]``, int32 / int64 / fp32 (fractions for interpolated positions).
+      Angles are formed and reduced in 64 bits, so they are off by some 2^-52 of their size: less than fp32 holds of
+      the reduced angle up to positions of 10^8. Not differentiated.
     * ``pairing``: ``"interleaved"`` pairs values ``(2p, 2p + 1)``, ``"half"`` pairs ``(p, p + d / 2)``.
     * ``inverse`` turns by the negative angles (what the gradient does).
 
