@@ -732,7 +732,7 @@ struct RowParams {
 // A CTA takes a tile of 128 rows of one head: dO's and O's, one 128 x 128 product of them, its diagonal, a thread a row.
 // Rows behind a sequence's end (up to the tile's) get no probability. HBM-bound: 512 bytes a row; three CTAs an SM keep
 // 192 KB of loads under way. 8190 x 40 rows 34 us, 4.9 TB/s (38 with plain loads and fused multiply-adds, four rows a half-warp);
-// a single tile takes 2 us more than by those.
+// a single tile takes 2 us more than by those with a cold L2, the same with a warm one.
 constexpr uint32_t kRowSmemBytes = 2 * kTileBytes + 1024;
 constexpr uint32_t kIdescRows = idesc_bf16(128, 128, false);
 template <int N>
